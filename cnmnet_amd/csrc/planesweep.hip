@@ -647,9 +647,9 @@ __global__ __launch_bounds__(SWEEP_NT) __attribute__((amdgpu_waves_per_eu(SWEEP_
     // The queue.  A workgroup's first two units are static (blockIdx.x, blockIdx.x + gridDim.x: no burst of 512 atomics on one
     // word when the launch starts - a word serves ~85 tickets per us).  From its second unit on, the LAST wave draws the unit
     // after the current one at the top of the current one, while wave 0 works out the footprints and everybody else waits at
-    // that barrier anyway, through the SCALAR cache path (s_atomic_add: lgkmcnt; a vector atomic would return behind the
-    // wave's own output stores in vmcnt order), and parks it in the LDS header; the barrier publishes it, the waves read it
-    // when the unit is done.
+    // that barrier anyway (a vector atomic by one lane: it returns behind that wave's own output stores, in vmcnt order, which
+    // the footprint pass mostly covers), and parks it in the LDS header; the barrier publishes it, the waves read it when the
+    // unit is done.
     int unit = blockIdx.x;
     bool first_unit = true;
     Unit cur = decode(min(unit, nunits - 1));
@@ -665,14 +665,10 @@ __global__ __launch_bounds__(SWEEP_NT) __attribute__((amdgpu_waves_per_eu(SWEEP_
 #ifdef SWEEP_TRACE
         const unsigned long long trace_t0 = __builtin_amdgcn_s_memrealtime();
 #endif
-        if (tid >= SWEEP_NT - 64) {
+        if (tid == SWEEP_NT - 64) {
             unsigned nxt = (unsigned)unit + gridDim.x;                         // the first unit's successor, and every one without a queue: a fixed stride
-            if (a.queue && !first_unit) {
-                nxt = 1u;
-                asm volatile("s_atomic_add %0, %1, 0x0 glc\n\ts_waitcnt lgkmcnt(0)" : "+s"(nxt) : "s"(a.queue) : "memory");
-                nxt += 2u * gridDim.x;
-            }
-            if (tid == SWEEP_NT - 64) hdr[2 * parity + 1] = (int)nxt;
+            if (a.queue && !first_unit) nxt = __hip_atomic_fetch_add(a.queue, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 2u * gridDim.x;
+            hdr[2 * parity + 1] = (int)nxt;
         }
         first_unit = false;
         const int p = cur.p, tx0 = cur.tx0, ty0 = cur.ty0, obeg = cur.obeg, ocnt = cur.ocnt;
