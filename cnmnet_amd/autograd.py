@@ -730,3 +730,72 @@ def scalar_maps_to_group(*maps):
 def nearest_up2(d):
     """F.upsample(disp, scale_factor=2) (nearest; depthNet_model.py:247,252,257)."""
     return d.repeat_interleave(2, 2).repeat_interleave(2, 3)
+
+
+class LinearFP8(torch.autograd.Function):
+    """y = x w^T with both operands quantised to 8 bits here (ops.quantize_fp8: x per row and 128 columns, w per 128 x 128), and its backward in
+    the same arithmetic: dx = Q(dy) w8 with the forward's 8-bit weight, dw = Q(dy^T) Q(x^T)^T blocked along the rows.  Kept for the backward
+    pass: the 8-bit transposed forms, a quarter of float32."""
+
+    @staticmethod
+    def forward(ctx, x, weight):
+        if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:
+            raise _lib.EngineError("linear_fp8: x %s against weight %s" % (tuple(x.shape), tuple(weight.shape)))
+        ops._dev_any(x, weight)
+        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        wq = ops.quantize_fp8(weight, 128, transposed=need_x)
+        xq = ops.quantize_fp8(x, 1, transposed=need_w)
+        ctx.save_for_backward(*(wq[2:] if need_x else (None, None)), *(xq[2:] if need_w else (None, None)))
+        ctx.info = x.shape, x.dtype, weight.shape, weight.dtype
+        return ops.matmul_fp8(xq[0], xq[1], wq[0], wq[1], x.dtype).view(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        wt, wts, xt, xts = ctx.saved_tensors
+        x_shape, x_dtype, w_shape, w_dtype = ctx.info
+        need_x, need_w = wt is not None, xt is not None
+        dx = dw = None
+        if dy.numel() == 0:                                              # no rows
+            return (torch.zeros(x_shape, device=dy.device, dtype=x_dtype) if need_x else None,
+                    torch.zeros(w_shape, device=dy.device, dtype=w_dtype) if need_w else None)
+        q = ops.quantize_fp8(dy, 1, transposed=need_w)
+        if need_x:
+            dx = ops.matmul_fp8(q[0], q[1], wt, wts, x_dtype).view(x_shape)
+        if need_w:
+            dw = ops.matmul_fp8(q[2], q[3], xt, xts, w_dtype)
+        return dx, dw
+
+
+def linear_fp8(x, weight):
+    """x [..., K], weight [N, K] (float32 / float16 / bfloat16, each its own) -> [..., N] of x's type, through 8-bit products both ways."""
+    return LinearFP8.apply(x, weight)
+
+
+class TopLogitsDistill(torch.autograd.Function):
+    """ops.top_logits_distill on the tape; gradient to the logits only.  For "mean" and "sum" the gradient is written by the forward launch, which
+    has the row at hand, and the backward pass only looks at the upstream gradient: where it is 1 (the loss is the root) there is nothing left
+    to do, otherwise the kernel recomputes the gradient from the logits with it -- never by scaling what was already rounded."""
+
+    @staticmethod
+    def forward(ctx, logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction):
+        call = ops.DistillCall(logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction)
+        ctx.dz = call.new_grad() if ctx.needs_input_grad[0] and call.reduction else None
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(logits, top_idx, top_logits, top_lse, weight)
+            ctx.how = temperature, dim, reduction
+            ctx.captured = torch.cuda.is_current_stream_capturing()
+        return call.run(True, ctx.dz)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, go):
+        call = ops.DistillCall(*ctx.saved_tensors, *ctx.how)
+        # the forward's gradient serves one backward pass (its buffer is given away), and not a captured one of an eager forward, which is replayed
+        dz = ctx.dz if ctx.captured == torch.cuda.is_current_stream_capturing() else None
+        ctx.dz = None
+        skip = dz is not None
+        if dz is None:
+            dz = call.new_grad()
+        call.run(False, dz, go.contiguous().float(), skip)
+        return call.c.back(dz), None, None, None, None, None, None, None

@@ -1,0 +1,721 @@
+// A teacher's top logits and the loss that a student takes from them.
+//
+// top_logits: per row of V classes the k largest logits in order (ties to the lowest class, NaN above everything, -0 equal to +0), their
+// classes, and lse = log sum_v exp(z_v / T).
+//
+// distillation, per row with teacher entries (i_k, t_k), an index outside 0 .. V-1 marking no entry:
+//     p_k = exp(t_k / T - L),  L = the teacher's log-sum-exp at T if given, else log sum_k exp(t_k / T) (the entries renormalised);
+//     q = softmax(z / T);   loss = T^2 [ sum_k p_k (log p_k - log q_{i_k}) + p_r (log p_r - log q_r) ]
+// with p_r = max(0, 1 - sum p_k) and q_r = sum of q over the classes that no entry names, only if L is given and such classes have mass.
+//     d loss / d z_v = T (q_v - sum_{k: i_k = v} p_k)      for a named class, and for every class when renormalised;
+//                    = T q_v (1 - p_r / q_r)               for the others when L is given.
+// The same class may be named twice (its p add up).  A row without entries: loss 0, gradient 0.
+//
+// Numerics: q_v = 2^((z_v - o) c) / S with c = log2(e) / T and the row's largest logit o: fp32; the difference first, so that a row of the type's
+// lowest values neither overflows nor loses its ratios.  Sums of exponentials in fp32 per thread, joined across threads with their offsets.  The row's few scalars -- lse, log p, log q,
+// p_r, the loss -- are fp64: a small loss is the difference of logarithms that nearly cancel.
+#include "cnm_common.h"
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int KMAX = 256;                    // entries per row
+constexpr int VMAX = 1 << 20;                // classes per row: one LDS bit each (128 KB)
+constexpr size_t LDS_BYTES = 160 * 1024;
+constexpr double LOG2E_D = 1.4426950408889634074, LN2_D = 0.69314718055994530942;
+
+template <int DT> struct Elem;
+template <> struct Elem<CNM_F32> { typedef float T; };
+template <> struct Elem<CNM_F16> { typedef _Float16 T; };
+template <> struct Elem<CNM_BF16> { typedef __bf16 T; };
+
+__device__ inline float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// (offset, sum) of exponentials 2^((x - offset) c); offset = -inf: none yet
+struct Lse { float o, s; };
+__device__ inline Lse lse_join(Lse a, Lse b, float c) {
+    const float o = fmaxf(a.o, b.o);                                     // (fmaxf drops a NaN: it is in the sum then)
+    const float so = o == -__builtin_huge_valf() ? 0.f : o;
+    // an empty side has s = 0 and offset -inf: 0 * 2^-inf = 0
+    return {o, a.s * exp2_((a.o - so) * c) + b.s * exp2_((b.o - so) * c)};
+}
+__device__ inline Lse lse_wave(Lse a, float c) {
+    for (int d = 32; d; d >>= 1) a = lse_join(a, Lse{__shfl_xor(a.o, d), __shfl_xor(a.s, d)}, c);
+    return a;
+}
+// the natural logarithm of the sum, in units of 1 / T
+__device__ inline float lse_value(Lse l, float T) {
+    return l.s == 0.f ? -__builtin_huge_valf() : (float)((double)(l.o == -__builtin_huge_valf() ? 0.f : l.o) / (double)T + log((double)l.s));
+}
+// joined over NT threads in a fixed order; every thread gets the result.  `sh` holds 2 * NT / 64 floats
+template <int NT>
+__device__ inline Lse lse_block(Lse a, float c, float* sh) {
+    a = lse_wave(a, c);
+    if (NT == 64) return a;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) { sh[2 * (threadIdx.x >> 6)] = a.o; sh[2 * (threadIdx.x >> 6) + 1] = a.s; }
+    __syncthreads();
+    const int l = threadIdx.x & 63;
+    a = l < NT / 64 ? Lse{sh[2 * l], sh[2 * l + 1]} : Lse{-__builtin_huge_valf(), 0.f};
+    return lse_wave(a, c);
+}
+template <int NT>
+__device__ inline double sum_block(double a, double* sh) {
+    for (int d = 32; d; d >>= 1) a += __shfl_xor(a, d);
+    if (NT == 64) return a;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
+    __syncthreads();
+    a = (threadIdx.x & 63) < NT / 64 ? sh[threadIdx.x & 63] : 0.0;
+    for (int d = 32; d; d >>= 1) a += __shfl_xor(a, d);
+    return a;
+}
+template <int NT>
+__device__ inline double max_block(double a, double* sh) {
+    for (int d = 32; d; d >>= 1) a = fmax(a, __shfl_xor(a, d));
+    if (NT == 64) return a;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
+    __syncthreads();
+    a = (threadIdx.x & 63) < NT / 64 ? sh[threadIdx.x & 63] : -__builtin_huge_val();
+    for (int d = 32; d; d >>= 1) a = fmax(a, __shfl_xor(a, d));
+    return a;
+}
+
+// f(first index, E values, how many of them count) over a row in units of 16 bytes where the row allows it: a head up to the first aligned
+// element, vectors, a tail; head and tail elements come one at a time, the rest of E being -inf
+template <int DT, int NT, class F>
+__device__ inline void sweep(const typename Elem<DT>::T* row, int V, int t, F f) {
+    typedef typename Elem<DT>::T T;
+    constexpr int E = 16 / sizeof(T);
+    const int mis = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    const int head = min(V, mis ? E - mis : 0), nvec = (V - head) / E, tail = head + nvec * E;
+    typedef T TV __attribute__((ext_vector_type(E)));
+    const TV* rv = reinterpret_cast<const TV*>(row + head);
+    float x[E];
+    for (int i = t; i < nvec; i += NT) {
+        const TV v = rv[i];
+#pragma unroll
+        for (int j = 0; j < E; ++j) x[j] = (float)v[j];
+        f(head + i * E, x, E);
+    }
+#pragma unroll
+    for (int j = 1; j < E; ++j) x[j] = -__builtin_huge_valf();
+    if (t < head) { x[0] = (float)row[t]; f(t, x, 1); }
+    if (tail + t < V) { x[0] = (float)row[tail + t]; f(tail + t, x, 1); }   // fewer than E <= NT elements
+}
+
+// running largest value and sum of the exponentials 2^((x - o) c), o = the largest value (0 while there is none but -inf)
+struct Run {
+    float m = -__builtin_huge_valf(), o = 0.f, s = 0.f;
+    __device__ void raise(float x, float c) {                            // a new largest value
+        if (m != -__builtin_huge_valf()) s *= exp2_((m - x) * c);
+        m = o = x;
+    }
+    __device__ Lse lse() const { return {m == -__builtin_huge_valf() ? m : o, s}; }
+};
+
+__device__ inline long long load_index(const void* idx, bool wide, size_t at) {
+    return wide ? static_cast<const long long*>(idx)[at] : (long long)static_cast<const int*>(idx)[at];
+}
+__device__ inline float load_any(const void* p, int dt, size_t at) {
+    return dt == CNM_F32 ? static_cast<const float*>(p)[at] : dt == CNM_F16 ? (float)static_cast<const _Float16*>(p)[at] : (float)static_cast<const __bf16*>(p)[at];
+}
+
+struct DistillArgs {
+    const void* z; long long ldz;            // rows of V classes, ldz apart; or [outer][V][inner]
+    const void* idx; int wide;               // [rows][K] or [outer][K][inner], int32 / int64
+    const void* val; int vdt;                // the entries' logits
+    const float* lse;                        // [rows] or null: renormalised
+    float T;
+    const float* weight;                     // [rows] or null
+    const double* wpart; int nwpart;         // the weights' partial sums (gradients are divided by their sum), or null
+    double inv_norm;                         // otherwise multiplied by this
+    const float* go; int go_rows;            // upstream gradient: one value, or one per row; null: 1
+    int skip_if_one;                         // *go == 1: the gradient is already there (written by the forward pass)
+    float* loss;                             // [rows] or null
+    double* lpart;                           // per workgroup: sum of weight * loss, or null
+    void* dz;                                // as z but dense, or null
+    long long rows; int V, K; long long inner;
+};
+
+// sum of up to 64 partial sums, in a fixed order, by a whole wave
+__device__ inline double wave_total(const double* part, int n) {
+    double s = (int)(threadIdx.x & 63) < n ? part[threadIdx.x & 63] : 0.0;
+    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+    return s;
+}
+
+// One row per NT threads.  LDS: one bit per class (named by an entry), the entries.  Two sweeps over the row: statistics of the unnamed
+// classes, then the gradient; the second one finds the row in the L2.
+template <int DT, int NT>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_rows_kernel(const DistillArgs a) {
+    typedef typename Elem<DT>::T T;
+    constexpr int RPB = NT == 64 ? 4 : 1, E = 16 / sizeof(T);
+    extern __shared__ unsigned lds_words[];
+    __shared__ double shd_[RPB][16];
+    __shared__ float shf_[RPB][32];
+    __shared__ int eidx_[RPB][KMAX];
+    __shared__ float ep_[RPB][KMAX];
+    const int sub = NT == 64 ? threadIdx.x >> 6 : 0, t = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
+    const int nw = a.V / 32 + 2;                                         // one word more than the bits need: eight bits are read from any of them on
+    unsigned* bits = lds_words + sub * nw;
+    double* shd = shd_[sub]; float* shf = shf_[sub]; int* eidx = eidx_[sub]; float* ep = ep_[sub];
+    float go = 1.f;
+    if (a.go && !a.go_rows) {
+        go = a.go[0];
+        if (a.skip_if_one && go == 1.f) return;
+    }
+    const long long row = (long long)blockIdx.x * RPB + sub;
+    const bool live = row < a.rows;
+    const long long r = live ? row : 0;
+    const T* z = static_cast<const T*>(a.z) + (size_t)r * a.ldz;
+    double norm = a.inv_norm;
+    if (a.wpart) { const double w = wave_total(a.wpart, a.nwpart); norm = w > 0.0 ? a.inv_norm / w : 0.0; }
+    if (a.go && a.go_rows) go = a.go[r];
+    const float wrow = a.weight ? a.weight[r] : 1.f;
+    const float c = (float)(LOG2E_D / (double)a.T);
+    auto sync = [&]() { if (NT == 64) { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier(); } else __syncthreads(); };
+
+    for (int i = t; i < nw; i += NT) bits[i] = 0u;
+    sync();
+    double best = -__builtin_huge_val();
+    int have = 0;
+    for (int k = t; k < a.K; k += NT) {
+        const long long i = load_index(a.idx, a.wide, (size_t)r * a.K + k);
+        const bool ok = i >= 0 && i < a.V;
+        eidx[k] = ok ? (int)i : -1;
+        if (ok) {
+            atomicOr(&bits[i >> 5], 1u << (i & 31));
+            have = 1;
+            best = fmax(best, (double)load_any(a.val, a.vdt, (size_t)r * a.K + k) / (double)a.T);
+        }
+    }
+    sync();
+    have = (int)max_block<NT>((double)have, shd);
+    double L;
+    if (a.lse) L = (double)a.lse[r];
+    else {
+        best = max_block<NT>(best, shd);
+        if (best == -__builtin_huge_val()) best = 0.0;
+        double s = 0.0;
+        for (int k = t; k < a.K; k += NT)
+            if (eidx[k] >= 0) s += (double)exp2_((float)(((double)load_any(a.val, a.vdt, (size_t)r * a.K + k) / (double)a.T - best) * LOG2E_D));
+        s = sum_block<NT>(s, shd);
+        L = best + log(s);
+    }
+    // statistics of the unnamed classes
+    Run run;
+    sweep<DT, NT>(z, a.V, t, [&](int v, const float* x, int) {
+        const unsigned mask = (unsigned)(((unsigned long long)bits[(v >> 5) + 1] << 32 | bits[v >> 5]) >> (v & 31));
+        float m = -__builtin_huge_valf();
+#pragma unroll
+        for (int j = 0; j < E; ++j) m = fmaxf(m, mask >> j & 1u ? -__builtin_huge_valf() : x[j]);
+        if (m > run.m) run.raise(m, c);
+#pragma unroll
+        for (int j = 0; j < E; ++j) run.s += mask >> j & 1u ? 0.f : exp2_((x[j] - run.o) * c);
+    });
+    Lse rest = run.lse();
+    rest = lse_block<NT>(rest, c, shf);
+    // the named classes, each once: its first entry stands for it
+    Lse named = {-__builtin_huge_valf(), 0.f};
+    for (int k = t; k < a.K; k += NT) {
+        const int i = eidx[k];
+        bool first = i >= 0;
+        for (int j = 0; j < k && first; ++j) first = eidx[j] != i;
+        if (first) {
+            const float x = (float)z[i];
+            named = lse_join(named, Lse{x, x == -__builtin_huge_valf() ? 0.f : x == x ? 1.f : x}, c);
+        }
+    }
+    named = lse_block<NT>(named, c, shf);
+    const Lse all = lse_join(rest, named, c);
+    const float oall = all.o == -__builtin_huge_valf() ? 0.f : all.o, orest = rest.o == -__builtin_huge_valf() ? 0.f : rest.o;
+    const double lq0 = -log2((double)all.s);                             // log2 q_v = (z_v - oall) c + lq0
+    // entries
+    double P = 0.0, loss = 0.0;
+    for (int k = t; k < a.K; k += NT) {
+        const int i = eidx[k];
+        float p = 0.f;
+        if (i >= 0) {
+            const double lp = ((double)load_any(a.val, a.vdt, (size_t)r * a.K + k) / (double)a.T - L) * LOG2E_D;
+            p = exp2_((float)lp);
+            if (p > 0.f) loss += (double)p * LN2_D * (lp - (((double)(float)z[i] - (double)oall) * (double)c + lq0));
+            P += (double)p;
+        }
+        ep[k] = p;
+    }
+    P = sum_block<NT>(P, shd);
+    loss = sum_block<NT>(loss, shd);
+    double ratio = 0.0;                                                  // p_r / (sum of the unnamed exponentials)
+    if (a.lse && rest.s > 0.f) {
+        const double pr = 1.0 - P;
+        if (pr > 0.0) {
+            const double lqr = ((double)orest - (double)oall) * (double)c + log2((double)rest.s) + lq0;
+            loss += pr * (log(pr) - lqr * LN2_D);
+            ratio = pr / (double)rest.s;
+        }
+    }
+    loss *= (double)a.T * (double)a.T;
+    if (!have) loss = 0.0;
+    if (t == 0 && live) {
+        if (a.loss) a.loss[r] = (float)loss;
+        if (a.lpart) a.lpart[r] = (wrow != 0.f ? (double)wrow * loss : 0.0);
+    }
+    if (!a.dz || !live) return;
+    T* dz = static_cast<T*>(a.dz) + (size_t)r * a.V;
+    const double scale = have && wrow != 0.f ? (double)a.T * (double)go * (double)wrow * norm : 0.0;
+    const bool zero = scale == 0.0;                                      // rows that count for nothing: zeros, whatever the logits hold
+    const double inv = (double)exp2_((orest - oall) * c) / (double)all.s;
+    const float A = (float)(scale * (inv - ratio)), Bp = (float)scale;
+    sync();
+    auto grad = [&](int v, float x) -> float {
+        if (zero) return 0.f;
+        const float e = exp2_((x - orest) * c);
+        if (!(bits[v >> 5] >> (v & 31) & 1u)) return A * e;
+        float p = 0.f;
+        for (int k = 0; k < a.K; ++k) p += eidx[k] == v ? ep[k] : 0.f;
+        // a named class may lie far above the unnamed ones: its own exponent against the whole row's
+        return Bp * (exp2_((x - oall) * c) / all.s - p);
+    };
+    const int mis = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
+    if (((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0) {
+        typedef T TV __attribute__((ext_vector_type(E)));
+        const int head = min(a.V, mis ? E - mis : 0), nvec = (a.V - head) / E, tail = head + nvec * E;
+        if (t < head) dz[t] = (T)grad(t, (float)z[t]);
+        const TV* zv = reinterpret_cast<const TV*>(z + head);
+        TV* dv = reinterpret_cast<TV*>(dz + head);
+        for (int i = t; i < nvec; i += NT) {
+            const TV x = zv[i];
+            TV g;
+#pragma unroll
+            for (int j = 0; j < E; ++j) g[j] = (T)grad(head + i * E + j, (float)x[j]);
+            dv[i] = g;
+        }
+        if (tail + t < a.V) dz[tail + t] = (T)grad(tail + t, (float)z[tail + t]);
+    } else {
+        for (int v = t; v < a.V; v += NT) dz[v] = (T)grad(v, (float)z[v]);
+    }
+}
+
+// The same with the classes in the middle: [outer][V][inner], a workgroup takes 64 neighbouring positions ("pixels"), one per lane; its four
+// waves share the classes and the entries.  The tile is read once, into LDS, and the gradient leaves from there: the entries' threads correct
+// the named classes in place.  LDS: 64 floats per class, one bit per class and pixel, the entries.
+template <int DT>
+__global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a, int tiles) {
+    typedef typename Elem<DT>::T T;
+    extern __shared__ unsigned lds_words[];
+    const int V = a.V, K = a.K, nw = (V + 31) / 32;
+    float* tile = reinterpret_cast<float*>(lds_words);                   // [V][64]
+    unsigned* bits = lds_words + V * 64;                                 // [nw][64]
+    int* eidx = reinterpret_cast<int*>(bits + nw * 64);                  // [K][64]
+    float* ep = reinterpret_cast<float*>(eidx + K * 64);                 // [K][64]: the entry's logit, then its p
+    double* shd = reinterpret_cast<double*>(ep + K * 64);                // [4][64]
+    double* shd2 = shd + 256;                                            // [4][64]
+    float go = 1.f;
+    if (a.go && !a.go_rows) {
+        go = a.go[0];
+        if (a.skip_if_one && go == 1.f) return;
+    }
+    const int px = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const long long ob = blockIdx.x / tiles;
+    const long long p0 = (long long)(blockIdx.x % tiles) * 64;
+    const bool live = p0 + px < a.inner;
+    const size_t at = live ? p0 + px : 0;                                // position in a plane
+    const T* z = static_cast<const T*>(a.z) + (size_t)ob * V * a.inner + at;
+    const size_t ebase = (size_t)ob * K * a.inner + at, r = (size_t)ob * a.inner + at;
+    double norm = a.inv_norm;
+    if (a.wpart) { const double s = wave_total(a.wpart, a.nwpart); norm = s > 0.0 ? a.inv_norm / s : 0.0; }
+    if (a.go && a.go_rows) go = a.go[r];
+    const float wrow = live ? (a.weight ? a.weight[r] : 1.f) : 0.f;
+    const float c = (float)(LOG2E_D / (double)a.T);
+    const float ninf = -__builtin_huge_valf();
+
+    for (int i = w; i < nw; i += 4) bits[i * 64 + px] = 0u;
+    for (int v = w; v < V; v += 4) tile[v * 64 + px] = live ? (float)z[(size_t)v * a.inner] : 0.f;
+    __syncthreads();
+    for (int k = w; k < K; k += 4) {
+        const long long i = live ? load_index(a.idx, a.wide, ebase + (size_t)k * a.inner) : -1;
+        const bool ok = i >= 0 && i < V;
+        eidx[k * 64 + px] = ok ? (int)i : -1;
+        ep[k * 64 + px] = ok ? load_any(a.val, a.vdt, ebase + (size_t)k * a.inner) : 0.f;
+        if (ok) atomicOr(&bits[(int)(i >> 5) * 64 + px], 1u << (i & 31));
+    }
+    __syncthreads();
+    // statistics: this wave's share of the unnamed classes and of the named ones (each once: its first entry stands for it)
+    Run run;
+    for (int v = w; v < V; v += 4)
+        if (!(bits[(v >> 5) * 64 + px] >> (v & 31) & 1u)) {
+            const float x = tile[v * 64 + px];
+            if (x > run.m) run.raise(x, c);
+            run.s += exp2_((x - run.o) * c);
+        }
+    Lse rest = run.lse(), named = {ninf, 0.f};
+    for (int k = w; k < K; k += 4) {
+        const int i = eidx[k * 64 + px];
+        bool first = i >= 0;
+        for (int j = 0; j < k; ++j) first = first && eidx[j * 64 + px] != i;
+        if (first) {
+            const float x = tile[i * 64 + px];
+            named = lse_join(named, Lse{x, x == ninf ? 0.f : x == x ? 1.f : x}, c);
+        }
+    }
+    float* shf = reinterpret_cast<float*>(shd);
+    float* shf2 = reinterpret_cast<float*>(shd2);
+    shf[w * 64 + px] = rest.o; shf[256 + w * 64 + px] = rest.s;
+    shf2[w * 64 + px] = named.o; shf2[256 + w * 64 + px] = named.s;
+    __syncthreads();
+    rest = Lse{shf[px], shf[256 + px]}; named = Lse{shf2[px], shf2[256 + px]};
+    for (int i = 1; i < 4; ++i) {
+        rest = lse_join(rest, Lse{shf[i * 64 + px], shf[256 + i * 64 + px]}, c);
+        named = lse_join(named, Lse{shf2[i * 64 + px], shf2[256 + i * 64 + px]}, c);
+    }
+    const Lse all = lse_join(rest, named, c);
+    const float oall = all.o == ninf ? 0.f : all.o, orest = rest.o == ninf ? 0.f : rest.o;
+    const double lq0 = -log2((double)all.s);
+    // the teacher's log-sum-exp: given, or over the entries
+    double L;
+    bool have = false;
+    {
+        float best = ninf;
+        for (int k = 0; k < K; ++k) if (eidx[k * 64 + px] >= 0) { have = true; best = fmaxf(best, ep[k * 64 + px]); }
+        if (a.lse) L = (double)a.lse[r];
+        else {
+            if (best == ninf) best = 0.f;
+            double s = 0.0;
+            for (int k = 0; k < K; ++k) if (eidx[k * 64 + px] >= 0) s += (double)exp2_((float)(((double)ep[k * 64 + px] - (double)best) * (LOG2E_D / (double)a.T)));
+            L = (double)best / (double)a.T + log(s);
+        }
+    }
+    __syncthreads();                                                     // every wave has read the entries' logits and the partial sums
+    double P = 0.0, loss = 0.0;
+    for (int k = w; k < K; k += 4) {
+        const int i = eidx[k * 64 + px];
+        float p = 0.f;
+        if (i >= 0) {
+            const double lp = ((double)ep[k * 64 + px] / (double)a.T - L) * LOG2E_D;
+            p = exp2_((float)lp);
+            if (p > 0.f) loss += (double)p * LN2_D * (lp - (((double)tile[i * 64 + px] - (double)oall) * (double)c + lq0));
+            P += (double)p;
+        }
+        ep[k * 64 + px] = p;
+    }
+    shd[w * 64 + px] = P; shd2[w * 64 + px] = loss;
+    __syncthreads();
+    P = (shd[px] + shd[64 + px]) + (shd[128 + px] + shd[192 + px]);
+    loss = (shd2[px] + shd2[64 + px]) + (shd2[128 + px] + shd2[192 + px]);
+    double ratio = 0.0;
+    if (a.lse && rest.s > 0.f) {
+        const double pr = 1.0 - P;
+        if (pr > 0.0) {
+            const double lqr = ((double)orest - (double)oall) * (double)c + log2((double)rest.s) + lq0;
+            loss += pr * (log(pr) - lqr * LN2_D);
+            ratio = pr / (double)rest.s;
+        }
+    }
+    loss *= (double)a.T * (double)a.T;
+    if (!have) loss = 0.0;
+    if (w == 0) {
+        if (a.loss && live) a.loss[r] = (float)loss;
+        if (a.lpart) {
+            double l = wrow != 0.f ? (double)wrow * loss : 0.0;
+            for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+            if (px == 0) a.lpart[blockIdx.x] = l;
+        }
+    }
+    if (!a.dz) return;
+    const double scale = have && wrow != 0.f ? (double)a.T * (double)go * (double)wrow * norm : 0.0;
+    const bool zero = scale == 0.0;
+    const float inv = 1.f / all.s, A = (float)(scale * ((double)exp2_((orest - oall) * c) / (double)all.s - ratio)), Bp = (float)scale;
+    for (int v = w; v < V; v += 4) {
+        const float x = tile[v * 64 + px];
+        const bool in = bits[(v >> 5) * 64 + px] >> (v & 31) & 1u;
+        const float e = exp2_((x - (in ? oall : orest)) * c);
+        tile[v * 64 + px] = zero ? 0.f : in ? e * inv : A * e;           // a named class: q, until its first entry has passed
+    }
+    __syncthreads();
+    for (int k = w; k < K; k += 4) {
+        const int i = eidx[k * 64 + px];
+        bool first = i >= 0 && !zero;
+        for (int j = 0; j < k; ++j) first = first && eidx[j * 64 + px] != i;
+        if (first) {
+            float p = ep[k * 64 + px];
+            for (int j = k + 1; j < K; ++j) p += eidx[j * 64 + px] == i ? ep[j * 64 + px] : 0.f;
+            tile[i * 64 + px] = Bp * (tile[i * 64 + px] - p);
+        }
+    }
+    __syncthreads();
+    if (!live) return;
+    T* dz = static_cast<T*>(a.dz) + (size_t)ob * V * a.inner + at;
+    for (int v = w; v < V; v += 4) dz[(size_t)v * a.inner] = (T)tile[v * 64 + px];
+}
+
+size_t planes_lds(int V, int K) { return (size_t)64 * 4 * ((size_t)V + (V + 31) / 32 + 2 * (size_t)K) + 2 * 256 * sizeof(double); }
+
+// partial sums of the weights, one per workgroup, each in a fixed order
+constexpr int WPARTS = 64;
+__global__ __launch_bounds__(1024) void weight_parts_kernel(const float* __restrict__ w, long long n, double* __restrict__ part) {
+    __shared__ double sh[16];
+    double s = 0.0;
+    for (long long i = (long long)blockIdx.x * 1024 + threadIdx.x; i < n; i += (long long)gridDim.x * 1024) s += (double)w[i];
+    s = sum_block<1024>(s, sh);
+    if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+
+// loss = sum of the workgroups' sums * inv_norm / (sum of the weights); no weight at all: 0
+__global__ __launch_bounds__(1024) void loss_total_kernel(const double* __restrict__ part, long long n, const double* __restrict__ wpart, int nwpart, double inv_norm, float* __restrict__ out) {
+    __shared__ double sh[16];
+    double s = 0.0;
+    for (long long i = threadIdx.x; i < n; i += 1024) s += part[i];
+    s = sum_block<1024>(s, sh);
+    if (threadIdx.x >= 64) return;
+    double norm = inv_norm;
+    if (wpart) { const double w = wave_total(wpart, nwpart); norm = w > 0.0 ? inv_norm / w : 0.0; }
+    if (threadIdx.x == 0) out[0] = norm != 0.0 ? (float)(s * norm) : 0.f;
+}
+
+template <int DT>
+int launch_distill(const DistillArgs& a, hipStream_t stream) {
+    if (a.inner > 1) {
+        const int tiles = (int)cnm_ceil_div_ll(a.inner, 64);
+        const long long blocks = (a.rows / a.inner) * tiles;
+        distill_planes_kernel<DT><<<(unsigned)blocks, 256, planes_lds(a.V, a.K), stream>>>(a, tiles);
+    } else {
+        const size_t words = ((size_t)a.V / 32 + 2) * 4;
+        if (a.V <= 1024) distill_rows_kernel<DT, 64><<<(unsigned)cnm_ceil_div_ll(a.rows, 4), 256, 4 * words, stream>>>(a);
+        else if (a.V <= 8192) distill_rows_kernel<DT, 256><<<(unsigned)a.rows, 256, words, stream>>>(a);
+        else distill_rows_kernel<DT, 1024><<<(unsigned)a.rows, 1024, words, stream>>>(a);
+    }
+    CNM_LAUNCH_CHECK();
+    return CNM_OK;
+}
+
+// ------------------------------------------------------------------ top logits
+// order-preserving key of a logit: larger value, larger key; NaN above everything, -0 as +0
+__device__ inline unsigned key_of(float x) {
+    if (x != x) return 0xFFFFFFFFu;
+    const unsigned u = __float_as_uint(x + 0.f);                         // -0 + 0 = +0
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+struct TopArgs {
+    const void* z; long long ldz;
+    float T;
+    void* val; int* idx; float* lse;
+    long long rows; int V, K; long long inner;
+};
+
+// One workgroup per row.  Radix selection of the K-th largest key, eight bits at a time, then everything above it, and of its equals the
+// lowest classes; the row is re-read from the caches.
+template <int DT, int NT>
+__global__ __launch_bounds__(NT) void top_rows_kernel(const TopArgs a) {
+    typedef typename Elem<DT>::T T;
+    constexpr int E = 16 / sizeof(T);
+    __shared__ unsigned hist[256];
+    __shared__ unsigned sel[4];                                          // digit, rank left within it, its count, output cursor
+    __shared__ unsigned long long cand[KMAX];
+    __shared__ float shf[32];
+    const int t = threadIdx.x;
+    const long long r = blockIdx.x;
+    const T* z = static_cast<const T*>(a.z) + (size_t)r * a.ldz;
+    const float c = (float)(LOG2E_D / (double)a.T);
+    Run run;
+    sweep<DT, NT>(z, a.V, t, [&](int, const float* x, int) {
+        float m = x[0];
+#pragma unroll
+        for (int j = 1; j < E; ++j) m = fmaxf(m, x[j]);
+        if (m > run.m) run.raise(m, c);
+#pragma unroll
+        for (int j = 0; j < E; ++j) run.s += exp2_((x[j] - run.o) * c);
+    });
+    const Lse l = lse_block<NT>(run.lse(), c, shf);
+    if (t == 0) a.lse[r] = lse_value(l, a.T);
+
+    // picks the digit that holds the `left`-th largest of what matches so far
+    auto pick = [&](unsigned left) {
+        __syncthreads();
+        if (t < 64) {                                                    // four digits per lane, from the highest down
+            unsigned n[4], own = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { n[j] = hist[255 - (4 * t + j)]; own += n[j]; }
+            unsigned before = own;
+            for (int d = 1; d < 64; d <<= 1) { const unsigned u = __shfl_up(before, d); if (t >= d) before += u; }
+            before -= own;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (before < left && left <= before + n[j]) { sel[0] = 255 - (4 * t + j); sel[1] = left - before; sel[2] = n[j]; }
+                before += n[j];
+            }
+        }
+        __syncthreads();
+    };
+    auto clear = [&]() { __syncthreads(); for (int i = t; i < 256; i += NT) hist[i] = 0u; __syncthreads(); };
+
+    unsigned prefix = 0, left = (unsigned)a.K, equal = 0;                // after the rounds: the K-th largest key, how many of its equals belong, how many there are
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        clear();
+        sweep<DT, NT>(z, a.V, t, [&](int, const float* x, int n) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                const unsigned k = key_of(x[j]);
+                if (j < n && (shift == 24 || (k ^ prefix) >> (shift + 8) == 0)) atomicAdd(&hist[k >> shift & 255u], 1u);
+            }
+        });
+        pick(left);
+        prefix |= sel[0] << shift; left = sel[1]; equal = sel[2];
+    }
+    unsigned last = 0xFFFFFFFFu;                                         // of the equals, the classes up to this one
+    if (equal != left) {                                                 // the left-th LOWEST class among them: the same selection on the inverted class
+        unsigned p2 = 0;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            clear();
+            sweep<DT, NT>(z, a.V, t, [&](int v, const float* x, int n) {
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    const unsigned k = ~(unsigned)(v + j);
+                    if (j < n && key_of(x[j]) == prefix && (shift == 24 || (k ^ p2) >> (shift + 8) == 0)) atomicAdd(&hist[k >> shift & 255u], 1u);
+                }
+            });
+            pick(left);
+            p2 |= sel[0] << shift; left = sel[1];
+        }
+        last = ~p2;
+    }
+    if (t == 0) sel[3] = 0u;
+    __syncthreads();
+    sweep<DT, NT>(z, a.V, t, [&](int v, const float* x, int n) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const unsigned k = key_of(x[j]);
+            if (j < n && (k > prefix || (k == prefix && (unsigned)(v + j) <= last))) cand[atomicAdd(&sel[3], 1u)] = (unsigned long long)k << 32 | ~(unsigned)(v + j);
+        }
+    });
+    __syncthreads();
+    for (int i = t; i < a.K; i += NT) {                                  // exactly K distinct candidates: a candidate's place is the number of those above it
+        const unsigned long long mine = cand[i];
+        int place = 0;
+        for (int j = 0; j < a.K; ++j) place += cand[j] > mine;
+        const unsigned v = ~(unsigned)mine;
+        a.idx[(size_t)r * a.K + place] = (int)v;
+        static_cast<T*>(a.val)[(size_t)r * a.K + place] = z[v];
+    }
+}
+
+// Classes in the middle, [outer][V][inner]: a lane per position keeps the KM largest of what it has seen, in order, in registers.  Classes come
+// in ascending order, so "strictly larger" keeps the lowest of equals in front.
+template <int DT, int KM>
+__global__ __launch_bounds__(256) void top_planes_kernel(const TopArgs a) {
+    typedef typename Elem<DT>::T T;
+    const long long r = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (r >= a.rows) return;
+    const long long ob = r / a.inner, at = r % a.inner;
+    const T* z = static_cast<const T*>(a.z) + (size_t)ob * a.V * a.inner + at;
+    const float c = (float)(LOG2E_D / (double)a.T);
+    unsigned key[KM];                                                    // 0 is below every key
+    int cls[KM];
+#pragma unroll
+    for (int i = 0; i < KM; ++i) { key[i] = 0u; cls[i] = 0; }
+    Run run;
+#pragma unroll 4
+    for (int v = 0; v < a.V; ++v) {
+        const float x = (float)z[(size_t)v * a.inner];
+        if (x > run.m) run.raise(x, c);
+        run.s += exp2_((x - run.o) * c);
+        const unsigned k = key_of(x);
+        if (k > key[KM - 1]) {                                           // from the last place up: a place takes its upper neighbour if k goes above that, k if it goes here
+#pragma unroll
+            for (int i = KM - 1; i > 0; --i) {
+                cls[i] = k > key[i - 1] ? cls[i - 1] : k > key[i] ? v : cls[i];
+                key[i] = k > key[i - 1] ? key[i - 1] : k > key[i] ? k : key[i];
+            }
+            cls[0] = k > key[0] ? v : cls[0];
+            key[0] = k > key[0] ? k : key[0];
+        }
+    }
+    const Lse l = run.lse();
+    a.lse[r] = lse_value(l, a.T);
+    const size_t base = (size_t)ob * a.K * a.inner + at;
+#pragma unroll
+    for (int i = 0; i < KM; ++i)
+        if (i < a.K) {
+            a.idx[base + (size_t)i * a.inner] = cls[i];
+            static_cast<T*>(a.val)[base + (size_t)i * a.inner] = z[(size_t)cls[i] * a.inner];
+        }
+}
+
+constexpr int TOP_PLANES_KMAX = 16;
+
+template <int DT>
+int launch_top(const TopArgs& a, hipStream_t stream) {
+    if (a.inner > 1) {
+        const unsigned blocks = (unsigned)cnm_ceil_div_ll(a.rows, 256);
+        if (a.K <= 4) top_planes_kernel<DT, 4><<<blocks, 256, 0, stream>>>(a);
+        else if (a.K <= 8) top_planes_kernel<DT, 8><<<blocks, 256, 0, stream>>>(a);
+        else top_planes_kernel<DT, 16><<<blocks, 256, 0, stream>>>(a);
+    } else {
+        if (a.V <= 4096) top_rows_kernel<DT, 256><<<(unsigned)a.rows, 256, 0, stream>>>(a);
+        else top_rows_kernel<DT, 1024><<<(unsigned)a.rows, 1024, 0, stream>>>(a);
+    }
+    CNM_LAUNCH_CHECK();
+    return CNM_OK;
+}
+
+}  // namespace
+
+extern "C" int cnm_top_logits_planes_max_entries(void) { return TOP_PLANES_KMAX; }
+extern "C" int cnm_distill_max_entries(void) { return KMAX; }
+extern "C" int cnm_distill_max_classes(void) { return VMAX; }
+extern "C" int cnm_distill_planes_ok(int classes, int entries) { return classes > 0 && entries > 0 && entries <= KMAX && classes <= VMAX && planes_lds(classes, entries) <= LDS_BYTES; }
+
+extern "C" int cnm_top_logits(const void* z, int dtype, long long ldz, float temperature, void* values, int* indices, float* lse,
+                              long long rows, int classes, int entries, long long inner, void* stream) {
+    CNM_REQUIRE(z && values && indices && lse && rows > 0 && classes > 0 && inner > 0 && temperature > 0.f && temperature < __builtin_huge_valf(), CNM_ERR_BAD_ARG);
+    CNM_REQUIRE(entries > 0 && entries <= classes && entries <= (inner > 1 ? TOP_PLANES_KMAX : KMAX) && rows % inner == 0 && (inner > 1 || ldz >= classes), CNM_ERR_BAD_ARG);
+    CNM_REQUIRE(rows < (1ll << 31) && classes <= (1 << 30), CNM_ERR_BAD_SHAPE);
+    const TopArgs a = {z, ldz, temperature, values, indices, lse, rows, classes, entries, inner};
+    switch (dtype) {
+        case CNM_F32: return launch_top<CNM_F32>(a, cnm_stream(stream));
+        case CNM_F16: return launch_top<CNM_F16>(a, cnm_stream(stream));
+        case CNM_BF16: return launch_top<CNM_BF16>(a, cnm_stream(stream));
+    }
+    return CNM_ERR_BAD_ARG;
+}
+
+extern "C" size_t cnm_distill_workspace_doubles(long long rows, long long inner) {
+    if (rows <= 0 || inner <= 0 || rows % inner) return 0;
+    return (size_t)WPARTS + (inner > 1 ? (size_t)(rows / inner) * (size_t)cnm_ceil_div_ll(inner, 64) : (size_t)rows);
+}
+
+extern "C" int cnm_distill(const void* z, int dtype, long long ldz, const void* indices, int wide_indices, const void* entry_logits, int entry_dtype,
+                           const float* teacher_lse, float temperature, const float* weight, const float* grad_out, int grad_out_rows, int skip_if_one,
+                           int reduction, float* loss, void* dz, double* workspace, size_t workspace_doubles,
+                           long long rows, int classes, int entries, long long inner, void* stream) {
+    CNM_REQUIRE(z && indices && entry_logits && rows > 0 && classes > 0 && entries > 0 && inner > 0 && (loss || dz), CNM_ERR_BAD_ARG);
+    CNM_REQUIRE(temperature > 0.f && temperature < __builtin_huge_valf() && reduction >= 0 && reduction <= 2 && entries <= KMAX, CNM_ERR_BAD_ARG);
+    CNM_REQUIRE(rows % inner == 0 && (inner > 1 || ldz >= classes) && entry_dtype >= CNM_F32 && entry_dtype <= CNM_BF16, CNM_ERR_BAD_ARG);
+    CNM_REQUIRE(!grad_out_rows || (grad_out && reduction == 0), CNM_ERR_BAD_ARG);
+    CNM_REQUIRE(rows < (1ll << 31) && classes <= VMAX && (inner == 1 || cnm_distill_planes_ok(classes, entries)), CNM_ERR_BAD_SHAPE);
+    CNM_REQUIRE(reduction == 0 || (workspace && workspace_doubles >= cnm_distill_workspace_doubles(rows, inner)), CNM_ERR_WORKSPACE);
+    const hipStream_t st = cnm_stream(stream);
+    const bool mean = reduction == 1;
+    double* const wpart = workspace;
+    double* const lpart = workspace ? workspace + WPARTS : nullptr;
+    const int nw = mean && weight ? (int)(cnm_ceil_div_ll(rows, 4096) < WPARTS ? cnm_ceil_div_ll(rows, 4096) : WPARTS) : 0;
+    if (nw) { weight_parts_kernel<<<nw, 1024, 0, st>>>(weight, rows, wpart); CNM_LAUNCH_CHECK(); }
+    const double inv_norm = mean && !weight ? 1.0 / (double)rows : 1.0;
+    const bool total = reduction != 0 && loss;
+    const DistillArgs a = {z, ldz, indices, wide_indices, entry_logits, entry_dtype, teacher_lse, temperature, weight, nw ? wpart : nullptr, nw, inv_norm,
+                           grad_out, grad_out_rows, skip_if_one, total ? nullptr : loss, total ? lpart : nullptr, dz, rows, classes, entries, inner};
+    int rc = CNM_ERR_BAD_ARG;
+    switch (dtype) {
+        case CNM_F32: rc = launch_distill<CNM_F32>(a, st); break;
+        case CNM_F16: rc = launch_distill<CNM_F16>(a, st); break;
+        case CNM_BF16: rc = launch_distill<CNM_BF16>(a, st); break;
+    }
+    if (rc != CNM_OK || !total) return rc;
+    const long long parts = inner > 1 ? (rows / inner) * cnm_ceil_div_ll(inner, 64) : rows;
+    loss_total_kernel<<<1, 1024, 0, st>>>(lpart, parts, nw ? wpart : nullptr, nw, inv_norm, loss);
+    CNM_LAUNCH_CHECK();
+    return CNM_OK;
+}

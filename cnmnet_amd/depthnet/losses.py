@@ -115,3 +115,21 @@ def surface_normal_loss(prediction, surface_normal, valid_region, probability_ma
         loss = total((1 - sim) * w) / total(w)
     angle = total(torch.acos(sim.clamp(-1, 1)) * k) / n
     return loss, angle / math.pi * 180
+
+
+class TopLogitsDistillLoss(nn.Module):
+    """Distillation from a teacher's stored top logits (cnmnet_amd.ops.top_logits at the same temperature), next to the map losses above for
+    students that predict a distribution: over depth planes ([B, planes, H, W], dim=1) or over any classes along the last dim.
+
+    forward(logits, top_idx, top_logits, top_lse=None, weight=None): T^2 KL(teacher || student); with top_lse the teacher's remaining mass is one
+    class of its own, without it the entries are renormalised.  weight: per-row, e.g. the frame's valid mask as float32; "mean" divides by
+    its sum (0 for an empty mask).  Rows without entries (index -1 throughout) give 0.  Unlike the losses above this is an engine operator
+    (GPU tensors only); the gradient reaches the logits, the teacher's side is constant."""
+
+    def __init__(self, temperature=1.0, dim=-1, reduction="mean"):
+        super().__init__()
+        self.temperature, self.dim, self.reduction = temperature, dim, reduction
+
+    def forward(self, logits, top_idx, top_logits, top_lse=None, weight=None):
+        from ..autograd import TopLogitsDistill
+        return TopLogitsDistill.apply(logits, top_idx, top_logits, top_lse, weight, self.temperature, self.dim, self.reduction)

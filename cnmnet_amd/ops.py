@@ -741,3 +741,238 @@ def inverse_warp(feat, depth, pose, intrinsics, intrinsics_inv, padding_mode="ze
         _lib.check(_lib.load().cnm_inverse_warp_pad_f32(_p(feat), _p(depth), _p(pose), _p(intrinsics), _p(intrinsics_inv),
                                                         _p(out), B, Cc, H, W, PADDING_MODES[padding_mode], _stream()))
     return out
+
+
+# ------------------------------------------------------------------ 8-bit linear layer
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}       # cnm_dtype of the operators that take more than float32
+
+
+def _dev_any(*tensors):
+    """Tensors of one GPU, each of a type the 8-bit and distillation operators take (float32, float16, bfloat16)."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise _lib.EngineError("cnmnet_amd operators run on the GPU only; got a %s tensor" % t.device)
+        if t.dtype not in DTYPES:
+            raise _lib.EngineError("this operator takes float32, float16 or bfloat16 tensors; got %s" % t.dtype)
+        if dev is not None and t.device != dev:
+            raise _lib.EngineError("tensors on %s and %s" % (dev, t.device))
+        dev = t.device
+    return dev
+
+
+def _rows2d(x, what):
+    """x [..., C] -> (2-D view or copy with dense rows, its row stride)."""
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise _lib.EngineError("%s needs at least one column; got shape %s" % (what, tuple(x.shape)))
+    C = x.shape[-1]
+    if x.dim() != 2:
+        x = x.reshape(-1, C)
+    if x.shape[0] > 1 and (x.stride(1) != 1 and C > 1 or x.stride(0) < C) or x.shape[0] == 1 and x.stride(1) != 1 and C > 1:
+        x = x.contiguous()
+    return x, (x.stride(0) if x.shape[0] > 1 else C)
+
+
+def quantize_fp8(x, block_rows=1, transposed=False):
+    """x [..., C] float32 / float16 / bfloat16 -> (q [R, C padded to 128] float8_e4m3fn, scale float8_e8m0fnu), R the product of the leading
+    sizes: one power of two per 1 x 128 block (block_rows 1: scale [R, ceil(C/128)]) or 128 x 128 block (block_rows 128: scale [ceil(R/128),
+    ceil(C/128)]); include/cnm_engine.h states the format.  transposed=True also returns (q_t [C, R padded to 128], scale_t), the same for x^T
+    (blocked along the rows), from the same pass over x."""
+    dev = _dev_any(x)
+    if block_rows not in (1, 128):
+        raise _lib.EngineError("block_rows must be 1 or 128; got %r" % (block_rows,))
+    x, ld = _rows2d(x, "quantize_fp8")
+    R, C = x.shape
+    Cb, Rb = (C + 127) // 128, (R + 127) // 128
+    q = torch.empty(R, Cb * 128, device=dev, dtype=torch.float8_e4m3fn)
+    s = torch.empty(R if block_rows == 1 else Rb, Cb, device=dev, dtype=torch.float8_e8m0fnu)
+    out = (q, s)
+    if transposed:
+        out += (torch.empty(C, Rb * 128, device=dev, dtype=torch.float8_e4m3fn),
+                torch.empty(C if block_rows == 1 else Cb, Rb, device=dev, dtype=torch.float8_e8m0fnu))
+    if R:
+        with torch.cuda.device(dev):
+            _lib.check(_lib.load().cnm_quantize_fp8(_p(x), DTYPES[x.dtype], ld, R, C, block_rows, _p(q), _p(s), *([_p(t) for t in out[2:]] or [0, 0]), _stream()))
+    return out
+
+
+def pack_linear_fp8(weight):
+    """weight [N, K] -> (w_packed [N, K padded to 128] float8_e4m3fn, w_scale [ceil(N/128), ceil(K/128)] float8_e8m0fnu) for linear_fp8."""
+    if weight.dim() != 2:
+        raise _lib.EngineError("pack_linear_fp8 takes a [N, K] weight; got shape %s" % (tuple(weight.shape),))
+    return quantize_fp8(weight, 128)
+
+
+def _fp8_operand(q, s, what, per_row=True, per_block=False):
+    """Checks of one operand of matmul_fp8; returns the rows per scale (1 or 128)."""
+    if not (q.is_cuda and s.is_cuda) or q.device != s.device:
+        raise _lib.EngineError("%s: values on %s, scale on %s" % (what, q.device, s.device))
+    if q.dtype != torch.float8_e4m3fn or s.dtype != torch.float8_e8m0fnu:
+        raise _lib.EngineError("%s: float8_e4m3fn values with float8_e8m0fnu scales; got %s, %s" % (what, q.dtype, s.dtype))
+    if q.dim() != 2 or q.shape[1] == 0 or q.shape[1] % 128 or not q.is_contiguous() or not s.is_contiguous() or (q.numel() and q.data_ptr() % 16):
+        raise _lib.EngineError("%s: values must be a dense [rows, K] matrix on a 16-byte boundary, K a multiple of 128 (quantize_fp8 pads); got %s" % (what, tuple(q.shape)))
+    R, Kb = q.shape[0], q.shape[1] // 128
+    if per_row and tuple(s.shape) == (R, Kb):
+        return 1
+    if per_block and tuple(s.shape) == ((R + 127) // 128, Kb):
+        return 128
+    raise _lib.EngineError("%s: scale %s does not belong to values %s" % (what, tuple(s.shape), tuple(q.shape)))
+
+
+def matmul_fp8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
+    """a [M, K], b [N, K] as quantize_fp8 makes them -> a b^T [M, N] of `dtype`; a with one scale per row and block, b with either kind."""
+    _fp8_operand(a, a_scale, "matmul_fp8 a")
+    bb = _fp8_operand(b, b_scale, "matmul_fp8 b", per_block=True)
+    if a.device != b.device or a.shape[1] != b.shape[1]:
+        raise _lib.EngineError("matmul_fp8: operands %s on %s and %s on %s" % (tuple(a.shape), a.device, tuple(b.shape), b.device))
+    if dtype not in DTYPES:
+        raise _lib.EngineError("matmul_fp8 gives float32, float16 or bfloat16; got %s" % dtype)
+    M, N, K = a.shape[0], b.shape[0], a.shape[1]
+    c = torch.empty(M, N, device=a.device, dtype=dtype)
+    if M and N:
+        with torch.cuda.device(a.device):
+            _lib.check(_lib.load().cnm_matmul_fp8(_p(a), _p(a_scale), _p(b), _p(b_scale), bb, _p(c), DTYPES[dtype], N, M, N, K, _stream()))
+    return c
+
+
+def linear_fp8(x, w_packed, w_scale):
+    """x [..., K] times a packed weight (pack_linear_fp8, [N, K]) -> [..., N] of x's type.  x is quantised here, one scale per row and 128
+    columns.  Inference; autograd.linear_fp8 is the training form."""
+    dev = _dev_any(x)
+    if _fp8_operand(w_packed, w_scale, "linear_fp8 weight", per_row=False, per_block=True) != 128 or w_packed.device != dev:
+        raise _lib.EngineError("linear_fp8: x on %s, weight on %s" % (dev, w_packed.device))
+    if x.dim() == 0 or (x.shape[-1] + 127) // 128 * 128 != w_packed.shape[1]:
+        raise _lib.EngineError("linear_fp8: x %s does not fit a weight packed as %s" % (tuple(x.shape), tuple(w_packed.shape)))
+    q, s = quantize_fp8(x)
+    return matmul_fp8(q, s, w_packed, w_scale, x.dtype).view(*x.shape[:-1], w_packed.shape[0])
+
+
+# ------------------------------------------------------------------ distillation from a teacher's top logits
+class _Classes:
+    """How a tensor of logits with classes along `dim` is handed to the engine: rows of contiguous classes, or [outer, V, inner] planes where
+    `planes_ok(V)`; any other arrangement is copied into rows."""
+
+    def __init__(self, z, dim, planes_ok):
+        if z.dim() == 0 or not -z.dim() <= dim < z.dim() or z.shape[dim] == 0:
+            raise _lib.EngineError("logits of shape %s have no classes along dim %r" % (tuple(z.shape), dim))
+        self.dim = dim % z.dim()
+        self.V, self.shape = z.shape[self.dim], z.shape
+        self.row_shape = z.shape[:self.dim] + z.shape[self.dim + 1:]
+        self.rows = 1
+        for n in self.row_shape:
+            self.rows *= n
+        inner = 1
+        for n in z.shape[self.dim + 1:]:
+            inner *= n
+        self.moved = inner > 1 and not planes_ok(self.V)                 # the copy into rows
+        self.inner = 1 if self.moved or inner == 0 else inner
+        self.ld = self.V
+        if self.moved:
+            z = z.movedim(self.dim, -1).contiguous()
+        elif z.dim() == 2 and self.dim == 1 and z.shape[0] > 1 and z.stride(1) == 1 and z.stride(0) >= self.V:
+            self.ld = z.stride(0)
+        else:
+            z = z.contiguous()
+        self.z = z
+
+    def entries(self, t):
+        """Per-row entries [.., K along dim, ..] in the engine's order."""
+        return t.movedim(self.dim, -1).contiguous() if self.moved else t.contiguous()
+
+    def sized(self, K):
+        """The engine's arrangement of K numbers per row."""
+        return self.row_shape + (K,) if self.moved else self.shape[:self.dim] + (K,) + self.shape[self.dim + 1:]
+
+    def back(self, t):
+        return t.movedim(-1, self.dim).contiguous() if self.moved else t
+
+
+def _temperature(t):
+    t = float(t)
+    if not 0.0 < t < float("inf"):
+        raise _lib.EngineError("temperature must be positive and finite; got %r" % t)
+    return t
+
+
+def top_logits(logits, k, dim=-1, temperature=1.0):
+    """What a teacher's cache holds of its logits: (values, indices int32, lse) with the k largest logits along `dim` in descending order --
+    ties: the lower class first; NaN above everything --, their classes, and lse = log sum exp(logits / temperature) over all classes
+    (float32).  logits: float32 / float16 / bfloat16, any shape; classes along the last dim are read in place (row stride allowed), classes
+    along an inner dim ([B, planes, H, W], dim=1) too for k <= 16.  k <= 256."""
+    dev = _dev_any(logits)
+    T = _temperature(temperature)
+    lib = _lib.load()
+    c = _Classes(logits, dim, lambda V: k <= lib.cnm_top_logits_planes_max_entries())
+    if not 1 <= k <= min(c.V, lib.cnm_distill_max_entries()):
+        raise _lib.EngineError("top_logits: k = %r of %d classes (at most %d)" % (k, c.V, lib.cnm_distill_max_entries()))
+    val = torch.empty(c.sized(k), device=dev, dtype=logits.dtype)
+    idx = torch.empty(c.sized(k), device=dev, dtype=torch.int32)
+    lse = torch.empty(c.row_shape, device=dev, dtype=torch.float32)
+    if c.rows:
+        with torch.cuda.device(dev):
+            _lib.check(lib.cnm_top_logits(_p(c.z), DTYPES[logits.dtype], c.ld, T, _p(val), _p(idx), _p(lse), c.rows, c.V, k, c.inner, _stream()))
+    return c.back(val), c.back(idx), lse
+
+
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+class DistillCall:
+    """One checked call of the distillation loss, its arguments laid out for the engine (ops.top_logits_distill, autograd.TopLogitsDistill)."""
+
+    def __init__(self, logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction):
+        self.dev = _dev_any(logits, top_logits, top_lse, weight)
+        self.T = _temperature(temperature)
+        self.lib = _lib.load()
+        if reduction not in REDUCTIONS:
+            raise _lib.EngineError("reduction must be one of %s; got %r" % (", ".join(REDUCTIONS), reduction))
+        self.reduction = REDUCTIONS[reduction]
+        if top_idx.device != self.dev or top_idx.dtype not in (torch.int32, torch.int64):
+            raise _lib.EngineError("top_idx must be int32 or int64 on %s; got %s on %s" % (self.dev, top_idx.dtype, top_idx.device))
+        if top_idx.dim() != logits.dim() or top_idx.dim() == 0 or not -logits.dim() <= dim < logits.dim():
+            raise _lib.EngineError("top_idx %s against logits %s along dim %r" % (tuple(top_idx.shape), tuple(logits.shape), dim))
+        self.K = K = top_idx.shape[dim]
+        self.c = c = _Classes(logits, dim, lambda V: bool(self.lib.cnm_distill_planes_ok(V, K)))
+        if not 1 <= K <= self.lib.cnm_distill_max_entries() or c.V > self.lib.cnm_distill_max_classes():
+            raise _lib.EngineError("%d entries over %d classes: at most %d over %d" % (K, c.V, self.lib.cnm_distill_max_entries(), self.lib.cnm_distill_max_classes()))
+        want = tuple(c.shape[:c.dim]) + (K,) + tuple(c.shape[c.dim + 1:])
+        if tuple(top_idx.shape) != want or tuple(top_logits.shape) != want:
+            raise _lib.EngineError("top_idx %s and top_logits %s: both must be %s" % (tuple(top_idx.shape), tuple(top_logits.shape), want))
+        for name, t in (("top_lse", top_lse), ("weight", weight)):
+            if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != tuple(c.row_shape)):
+                raise _lib.EngineError("%s must be float32 %s; got %s %s" % (name, tuple(c.row_shape), t.dtype, tuple(t.shape)))
+        self.dtype = logits.dtype
+        self.idx, self.val = c.entries(top_idx), c.entries(top_logits)
+        self.lse = None if top_lse is None else top_lse.contiguous()
+        self.weight = None if weight is None else weight.contiguous()
+
+    def new_grad(self):
+        return torch.empty(self.c.sized(self.c.V), device=self.dev, dtype=self.dtype)
+
+    def run(self, need_loss, dz, grad_out=None, skip_if_one=False):
+        """Launches; returns the loss (or None).  dz: a new_grad() buffer to fill, or None."""
+        c = self.c
+        loss = torch.empty(c.row_shape if self.reduction == 0 else (), device=self.dev, dtype=torch.float32) if need_loss else None
+        if c.rows == 0:
+            return loss.zero_() if need_loss else None
+        n = self.lib.cnm_distill_workspace_doubles(c.rows, c.inner) if self.reduction else 0
+        ws = torch.empty(n, device=self.dev, dtype=torch.float64) if n else None
+        with torch.cuda.device(self.dev):
+            _lib.check(self.lib.cnm_distill(_p(c.z), DTYPES[self.dtype], c.ld, _p(self.idx), int(self.idx.dtype == torch.int64), _p(self.val), DTYPES[self.val.dtype],
+                                            _p(self.lse), self.T, _p(self.weight), _p(grad_out), int(grad_out is not None and self.reduction == 0), int(skip_if_one),
+                                            self.reduction, _p(loss), _p(dz), _p(ws), n, c.rows, c.V, self.K, c.inner, _stream()))
+        return loss
+
+
+def top_logits_distill(logits, top_idx, top_logits, top_lse=None, weight=None, temperature=1.0, dim=-1, reduction="mean", grad=False):
+    """Distillation loss of a student's logits against a teacher's stored top logits (ops.top_logits of the teacher at the same temperature):
+    T^2 KL(teacher || student) with the teacher's classes outside the entries lumped into one (top_lse given), or the entries renormalised
+    (top_lse None); include/cnm_engine.h states the formula.  top_idx (int32 / int64; an index outside the classes is no entry) and top_logits
+    have K in the place of the classes; top_lse and weight are float32 without that dim.  reduction "mean": sum weight loss / sum weight, "sum",
+    or "none".  grad=True: (loss, gradient of the logits) in one pass over them, for programs that call backward on the logits themselves."""
+    call = DistillCall(logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction)
+    dz = call.new_grad() if grad else None
+    loss = call.run(True, dz)
+    return (loss, call.c.back(dz)) if grad else loss

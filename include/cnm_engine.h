@@ -115,6 +115,9 @@ typedef enum cnm_status {
     CNM_ERR_WORKSPACE = -5      /* workspace smaller than *_workspace_floats() */
 } cnm_status;
 
+/* element types of the entry points that take more than one (void pointers next to a dtype) */
+typedef enum cnm_dtype { CNM_F32 = 0, CNM_F16 = 1, CNM_BF16 = 2 } cnm_dtype;
+
 int cnm_abi_version(void);
 const char* cnm_status_string(int status);
 
@@ -852,6 +855,55 @@ int cnm_refinenet_forward_multi_cpu(const cnm_layer_weights* weights, float idep
                                     const float* idepth_pairs, const float* iconv_pairs_c4, int S,
                                     float* disp_refined, float* prob_map, float* iconv1_depth_c4,
                                     float* ws, size_t ws_floats, int B, int H, int W);                            /* eval.py:635-663,885-929 */
+
+/* ------------------------------------------------------------------ 8-bit linear layer
+ * The reference has no dense layer and no 8-bit arithmetic; this is the engine's own next step below the fp16 engine.
+ * A matrix [R][C] in 8 bits is e4m3 values [R][C padded with zeros to a multiple of 128] and one power of two 2^e per block of 128 along the
+ * row, held as the byte e + 127: e = the smallest integer >= -127 with max|x| <= 448 * 2^e over the block's finite values, value =
+ * e4m3(x * 2^-e), ties to even; inf and NaN become NaN.  block_rows 1: one byte per row and block (activations, gradients), scale
+ * [R][ceil(C/128)]; block_rows 128: one per 128 x 128 (weights), scale [ceil(R/128)][ceil(C/128)].
+ *
+ * cnm_quantize_fp8: x [rows][ldx] of dtype (ldx >= cols, any alignment) -> q, scale and / or the transposed matrix's form q_t [cols][rows
+ * padded to 128], scale_t (block_rows 1: blocked along the rows, [cols][ceil(rows/128)]; 128: the same blocks, [ceil(cols/128)][ceil(rows/128)])
+ * in one pass over x.  q / q_t (with their scales) may be NULL, not both; q and q_t on 16 bytes. */
+int cnm_quantize_fp8(const void* x, int dtype, long long ldx, long long rows, long long cols, int block_rows,
+                     void* q, void* scale, void* q_t, void* scale_t, void* stream);
+/* c [M][ldc] of dtype = a b^T: a [M][K], b [N][K] as above (K a multiple of 128, at most 2^23; a, b on 16 bytes), a_scale [M][K/128],
+ * b_scale [N][K/128] (b_block_rows 1) or [ceil(N/128)][K/128] (128).  fp32 accumulation, one rounding.  Any M, N >= 1; ldc >= N. */
+int cnm_matmul_fp8(const void* a, const void* a_scale, const void* b, const void* b_scale, int b_block_rows, void* c, int dtype,
+                   long long ldc, long long M, long long N, long long K, void* stream);
+
+/* ------------------------------------------------------------------ distillation from a teacher's top logits
+ * Beside the reference's losses (depthnet/losses.py), which compare maps: these compare distributions over classes (depth planes, tokens).
+ * A set of `rows` distributions over `classes` is either [rows][ldz], classes contiguous (inner = 1), or [rows / inner][classes][inner]
+ * (inner > 1: e.g. [B, planes, H, W], inner = H W; ldz is ignored).  Entries, values, indices and per-row numbers follow the same order
+ * ([rows][entries] or [rows / inner][entries][inner]; [rows]).
+ *
+ * cnm_top_logits: the `entries` largest logits per row in descending order (ties: the lower class first; NaN above everything, -0 equal to
+ * +0), their classes, and lse = log sum exp(z / temperature).  entries <= classes, <= cnm_distill_max_entries() (inner = 1) or
+ * cnm_top_logits_planes_max_entries() (inner > 1). */
+int cnm_top_logits(const void* z, int dtype, long long ldz, float temperature, void* values, int* indices, float* lse,
+                   long long rows, int classes, int entries, long long inner, void* stream);
+int cnm_top_logits_planes_max_entries(void);
+int cnm_distill_max_entries(void);
+int cnm_distill_max_classes(void);
+/* 1 if cnm_distill takes this many classes and entries with inner > 1 (they share 160 KB of LDS per 64 positions), else 0 */
+int cnm_distill_planes_ok(int classes, int entries);
+/* Loss and / or gradient of a student's logits z against the entries (class index, teacher logit), T = temperature:
+ *   p_k = exp(t_k / T - L), L = teacher_lse[row] or, NULL, log sum_k exp(t_k / T);  q = softmax(z / T)
+ *   loss = T^2 [ sum_k p_k (log p_k - log q_{i_k}) + p_r (log p_r - log q_r) ], p_r = max(0, 1 - sum p_k) and q_r = the probability of the
+ *   classes that no entry names, with teacher_lse only and only if these classes have any.
+ * An index outside 0 .. classes-1 is no entry; a row without entries has loss 0 and gradient 0; a class may be named more than once.
+ * reduction 0: loss [rows]; 1: loss [1] = sum weight loss / sum weight (0 if the weights sum to 0); 2: loss [1] = sum weight loss.
+ * weight [rows] or NULL (1).  dz (dense, z's dtype) = the gradient of what `loss` is (reduction 0: of sum weight loss), times grad_out[0], or
+ * grad_out[row] with grad_out_rows (reduction 0 only), or 1 (NULL).  skip_if_one: if grad_out[0] == 1 the launch leaves dz as it is.
+ * loss or dz may be NULL, not both.  workspace: cnm_distill_workspace_doubles(rows, inner) doubles, needed for reduction 1 and 2, contents
+ * irrelevant.  Every sum has a fixed order: results repeat bit by bit. */
+size_t cnm_distill_workspace_doubles(long long rows, long long inner);
+int cnm_distill(const void* z, int dtype, long long ldz, const void* indices, int wide_indices, const void* entry_logits, int entry_dtype,
+                const float* teacher_lse, float temperature, const float* weight, const float* grad_out, int grad_out_rows, int skip_if_one,
+                int reduction, float* loss, void* dz, double* workspace, size_t workspace_doubles,
+                long long rows, int classes, int entries, long long inner, void* stream);
 
 #ifdef __cplusplus
 }
