@@ -25,6 +25,8 @@ namespace {
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -58,20 +60,15 @@ __device__ inline unsigned pack4(float a, float b, float c, float d) {
     return u;
 }
 
-// eight consecutive values of a row, zero beyond `have`
-template <int DT, bool VEC>
+// eight consecutive values of a row, zero beyond `have` (16-byte loads whatever the row's alignment: global memory takes them)
+template <int DT>
 __device__ inline void load8(const typename Elem<DT>::T* p, int have, float v[8]) {
-    if (VEC && have >= 8) {
-        if constexpr (DT == CNM_F32) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+    typedef typename Elem<DT>::T T;
+    if (have >= 8) {
+        T a[8];
+        __builtin_memcpy(a, p, sizeof(a));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
-        } else {
-            typedef typename Elem<DT>::T T8 __attribute__((ext_vector_type(8)));
-            const T8 a = *reinterpret_cast<const T8*>(p);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = Elem<DT>::up(a[j]);
-        }
+        for (int j = 0; j < 8; ++j) v[j] = Elem<DT>::up(a[j]);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = j < have ? Elem<DT>::up(p[j]) : 0.f;
@@ -81,7 +78,7 @@ __device__ inline void load8(const typename Elem<DT>::T* p, int have, float v[8]
 // One workgroup quantises a 128 x 128 tile, read once: 16 lanes per row (8 values each), a thread's eight rows consecutive, so that the
 // transposed copy leaves as 8-byte columns through LDS.  Row form: q [R][Cp], s [R][Cp/128] (BLK = false) or s [R/128][Cp/128] (BLK = true).
 // Transposed form (optional): qt [C][Rp], blocked along R: st [C][Rp/128], or the same 128 x 128 block's byte at st [C/128][Rp/128].
-template <int DT, bool BLK, bool VEC>
+template <int DT, bool BLK>
 __global__ __launch_bounds__(256) void quantize_kernel(const typename Elem<DT>::T* __restrict__ x, long long ldx, int R, int C, int Cb, int Rb,
                                                        unsigned char* __restrict__ q, unsigned char* __restrict__ s,
                                                        unsigned char* __restrict__ qt, unsigned char* __restrict__ st) {
@@ -95,7 +92,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(const typename Elem<DT>::
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
         const int r = r0 + p;
-        load8<DT, VEC>(x + (size_t)(r < R ? r : 0) * ldx + (c0 < C ? c0 : 0), r < R ? C - c0 : 0, v[p]);
+        load8<DT>(x + (size_t)(r < R ? r : 0) * ldx + (c0 < C ? c0 : 0), r < R ? C - c0 : 0, v[p]);
     }
     int byte[8];
     float am[8];
@@ -183,31 +180,15 @@ template <int DT, bool BLK>
 int launch_quantize(const void* x, long long ldx, int R, int C, void* q, void* s, void* qt, void* st, hipStream_t stream) {
     typedef typename Elem<DT>::T T;
     const int Cb = cnm_ceil_div(C, QB), Rb = cnm_ceil_div(R, QB);
-    const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * (long long)sizeof(T)) % 16 == 0;   // every row starts on 16 bytes, so does every group of eight
     auto* xp = static_cast<const T*>(x);
     auto* qp = static_cast<unsigned char*>(q); auto* sp = static_cast<unsigned char*>(s);
     auto* qtp = static_cast<unsigned char*>(qt); auto* stp = static_cast<unsigned char*>(st);
-    if (vec) quantize_kernel<DT, BLK, true><<<Cb * Rb, 256, 0, stream>>>(xp, ldx, R, C, Cb, Rb, qp, sp, qtp, stp);
-    else quantize_kernel<DT, BLK, false><<<Cb * Rb, 256, 0, stream>>>(xp, ldx, R, C, Cb, Rb, qp, sp, qtp, stp);
+    quantize_kernel<DT, BLK><<<Cb * Rb, 256, 0, stream>>>(xp, ldx, R, C, Cb, Rb, qp, sp, qtp, stp);
     CNM_LAUNCH_CHECK();
     return CNM_OK;
 }
 
 // ------------------------------------------------------------------ product
-// Four consecutive scale bytes of a row (blocks kb .. kb + 3) as one word: an unaligned load that never leaves the array -- near its end it
-// reads the last four bytes and shifts; bytes beyond the row belong to the next one and are not used.
-__device__ inline unsigned scale_word(const unsigned char* s, size_t off, size_t total) {
-    if (total < 4) {
-        unsigned w = 0;
-        for (size_t i = 0; i < 4; ++i) if (off + i < total) w |= (unsigned)s[off + i] << (8 * i);
-        return w;
-    }
-    const size_t at = off < total - 4 ? off : total - 4;
-    unsigned w;
-    __builtin_memcpy(&w, s + at, 4);
-    return w >> (8 * (off - at));
-}
-
 // eight e4m3 bytes times 2^(byte - 127) -> bf16
 __device__ inline bf16x8 widen(int lo, int hi, float scale) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
@@ -224,119 +205,419 @@ struct MatArgs {
     int tiles_m, tiles_n;
 };
 
-// TM x TN outputs per workgroup, WM x WN waves; a k-step is one block of 128: 128 bytes per operand row, brought to LDS by DMA one step ahead.
-// LDS: row r at r * 128, its eight 16-byte chunks permuted by (r >> 1) & 7: the 16 rows that a fragment read touches at one chunk then fall on
+// Tiles in an order that keeps neighbours on one XCD near each other: workgroups are dealt to XCDs in contiguous ranges (xcd_remap), and a
+// range walks bands of four tile rows, column by column, so that the 32 CUs of an XCD share four row blocks and eight column blocks in its L2.
+__device__ inline void tile_of(int id, const MatArgs& g, int& tm, int& tn) {
+    const int band = id / (4 * g.tiles_n), in = id - band * 4 * g.tiles_n;
+    const int rows = min(4, g.tiles_m - 4 * band);
+    tm = 4 * band + in % rows; tn = in / rows;
+}
+
+// TM x TN outputs per workgroup, WM x WN waves, each IM x IN tiles of 32 x 32.  The reduced axis goes by in half blocks of 64: both operands' rows
+// (64 bytes each) come to LDS by DMA, a ring of four half blocks, three ahead of their use; a wave reads the fragments of the next half block
+// under the matrix instructions of this one (two register sets).  One barrier per half block, behind a counted vmcnt: two half blocks stay
+// in flight across it.
+// LDS: row r at r * 64, its four 16-byte chunks permuted by (r >> 2) & 3: the 16 rows that a fragment read touches at one chunk then fall on
 // all 64 banks.  The DMA writes 64 lanes x 16 bytes in order, so the permutation is in the lanes' source addresses.
-// The weight is the instruction's first operand: a lane then holds four consecutive outputs of one row.
-template <int TM, int TN, int WM, int WN, int DT>
+// Scale bytes: rows of SC blocks in LDS, refilled every SC blocks; a lane reads four blocks' bytes as one word.
+// The weight is the instruction's first operand: a lane then holds outputs of one row, in fours.
+// The order within a half block: its NM matrix instructions start at once, the next fragments' ND reads and the NV DMA instructions go evenly
+// between them (left alone, the scheduler puts all of these in front, or the matrix instructions of two half blocks behind one barrier).
+template <int I, int NM, int ND, int NV>
+struct Interleave {
+    static __device__ __forceinline__ void go() {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if constexpr (ND * (I + 1) / NM > ND * I / NM) __builtin_amdgcn_sched_group_barrier(0x100, ND * (I + 1) / NM - ND * I / NM, 0);
+        if constexpr (NV * (I + 1) / NM > NV * I / NM) __builtin_amdgcn_sched_group_barrier(0x010, NV * (I + 1) / NM - NV * I / NM, 0);
+        if constexpr (I + 1 < NM) Interleave<I + 1, NM, ND, NV>::go();
+    }
+};
+
+template <int TM, int TN, int WM, int WN, int DT, bool BLK>
+struct Mat {
+    static constexpr int NW = WM * WN, NT = NW * 64, IM = TM / WM / 32, IN = TN / WN / 32, NST = 4;
+    static constexpr int STAGE = (TM + TN) * 64, PA = TM / 16 / NW, PB = TN / 16 / NW, DMA = PA + PB;   // DMA instructions per wave and half block: 16 rows each
+    static constexpr int SC = BLK ? 64 : 32, SROW = SC + 4, BROWS = BLK ? TN / QB : TN;                 // scale rows: four bytes apart from a power of two
+    static constexpr int LDS = NST * STAGE + (TM + BROWS) * SROW;
+    static_assert(TM % (16 * NW) == 0 && TN % (16 * NW) == 0 && LDS <= 160 * 1024 && (!BLK || (TN % QB == 0 && TN / WN <= QB)), "tile");
+};
+
+template <int TM, int TN, int WM, int WN, int DT, bool BLK>
 __global__ __launch_bounds__(WM * WN * 64) void matmul_fp8_kernel(const MatArgs g) {
-    constexpr int NW = WM * WN, IM = TM / WM / 16, IN = TN / WN / 16;
-    constexpr int ROWS = TM + TN, STAGE = ROWS * QB, PIECES = ROWS / 8 / NW;   // a piece: one DMA instruction, eight rows
-    extern __shared__ char smem[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    typedef Mat<TM, TN, WM, WN, DT, BLK> C;
+    constexpr int IM = C::IM, IN = C::IN;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    char* const sca = smem + C::NST * C::STAGE;
+    char* const scb = sca + TM * C::SROW;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN;
-    const int blk = xcd_remap(blockIdx.x, gridDim.x);
-    const int tm = blk / g.tiles_n, tn = blk % g.tiles_n;
-    const int m0 = tm * TM, n0 = tn * TN;
-    const int K = g.Kb * QB;
-    const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(g.a) + (size_t)m0 * K, 0, (unsigned)min(g.M - m0, TM) * (unsigned)K, 0x00020000);
-    const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(g.b) + (size_t)n0 * K, 0, (unsigned)min(g.N - n0, TN) * (unsigned)K, 0x00020000);
-    auto issue = [&](int kb, int buf) {
+    int tm, tn;
+    tile_of(xcd_remap(blockIdx.x, gridDim.x), g, tm, tn);
+    const int m0 = tm * TM, n0 = tn * TN, Kb = g.Kb, K = Kb * QB;
+    // buffer ranges that end with the operands' last rows: beyond them the DMA writes zeros
+    const unsigned bytes_a = (unsigned)min(g.M - m0, TM) * (unsigned)K, bytes_b = (unsigned)min(g.N - n0, TN) * (unsigned)K;
+    const int S = 2 * Kb;
+    const unsigned chunk = (unsigned)((lane & 3) ^ ((lane >> 4) & 3)) * 16u;
+    const unsigned va = (unsigned)(wave * C::PA * 16 + (lane >> 2)) * (unsigned)K + chunk, vb = (unsigned)(wave * C::PB * 16 + (lane >> 2)) * (unsigned)K + chunk;
+    auto issue = [&](int s) {                                            // half block s into its place in the ring; beyond the last one an empty range: zeros, no traffic, the same count
+        const auto ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(g.a) + (size_t)m0 * K, 0, s < S ? bytes_a : 0u, 0x00020000);
+        const auto rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(g.b) + (size_t)n0 * K, 0, s < S ? bytes_b : 0u, 0x00020000);
+        char* const dst = smem + (s & (C::NST - 1)) * C::STAGE;
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p) {
-            const int piece = wave * PIECES + p, row = piece * 8 + (lane >> 3);
-            const int chunk = (lane & 7) ^ ((row >> 1) & 7);
-            char* dst = smem + buf * STAGE + piece * 1024;
-            if (piece * 8 < TM) __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr)dst, 16, (unsigned)row * (unsigned)K + chunk * 16, kb * QB, 0, 0);
-            else __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr)dst, 16, (unsigned)(row - TM) * (unsigned)K + chunk * 16, kb * QB, 0, 0);
+        for (int p = 0; p < C::PA; ++p)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_ptr)(dst + (wave * C::PA + p) * 1024), 16, va + (unsigned)p * 16u * (unsigned)K, s * 64, 0, 0);
+#pragma unroll
+        for (int p = 0; p < C::PB; ++p)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_ptr)(dst + TM * 64 + (wave * C::PB + p) * 1024), 16, vb + (unsigned)p * 16u * (unsigned)K, s * 64, 0, 0);
+    };
+    // scale bytes of blocks kb .. kb + SC - 1: 16 at a time, never beyond the arrays
+    auto fill = [&](char* dst, const unsigned char* s, int row0, int rows, int last, int kb) {
+        constexpr int P = C::SC / 16;
+        for (int i = tid; i < rows * P; i += C::NT) {
+            const int r = i / P, p = i % P;
+            if (kb + 16 * p >= Kb) continue;
+            const size_t off = (size_t)min(row0 + r, last) * Kb + kb + 16 * p, total = ((size_t)last + 1) * Kb;
+            unsigned w[4] = {0u, 0u, 0u, 0u};
+            if (off + 16 <= total) __builtin_memcpy(w, s + off, 16);
+            else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) if (off + j < total) w[j >> 2] |= (unsigned)s[off + j] << (8 * (j & 3));
+            }
+            unsigned* const d = reinterpret_cast<unsigned*>(dst + r * C::SROW + 16 * p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[j] = w[j];
         }
     };
-    f32x4 acc[IM][IN] = {};
-    const int fr = lane & 15, fg = lane >> 4;
-    size_t oa[IM], ob[IN];
-    const size_t ta = (size_t)g.M * g.Kb, tb = (size_t)(((g.N - 1) >> g.bshift) + 1) * g.Kb;
+    f32x16 acc[IM][IN] = {};
+    const int fr = lane & 31, fh = lane >> 5;
+    const int sw = (fr >> 2) & 3, c0 = ((2 * fh) ^ sw) * 16, c1 = ((2 * fh + 1) ^ sw) * 16;
+    const char* const pa = smem + (wm * (TM / WM) + fr) * 64;
+    const char* const pb = smem + (TM + wn * (TN / WN) + fr) * 64;
+    i32x8 fa[2][IM], fb[2][IN];
+    // (typed f16x8: with integer vectors hipcc orders the reads behind vmcnt(0), i.e. behind the DMA just issued for later half blocks)
+    auto frag = [&](const char* p) {
+        const i32x4 lo = __builtin_bit_cast(i32x4, *reinterpret_cast<const f16x8*>(p + c0)), hi = __builtin_bit_cast(i32x4, *reinterpret_cast<const f16x8*>(p + c1));
+        return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+    auto load = [&](int s, int set) {
+        const int base = (s & (C::NST - 1)) * C::STAGE;
 #pragma unroll
-    for (int i = 0; i < IM; ++i) oa[i] = (size_t)min(m0 + wm * (TM / WM) + i * 16 + fr, g.M - 1) * g.Kb;
+        for (int j = 0; j < IN; ++j) fb[set][j] = frag(pb + base + j * 32 * 64);
 #pragma unroll
-    for (int j = 0; j < IN; ++j) ob[j] = (size_t)(min(n0 + wn * (TN / WN) + j * 16 + fr, g.N - 1) >> g.bshift) * g.Kb;
+        for (int i = 0; i < IM; ++i) fa[set][i] = frag(pa + base + i * 32 * 64);
+    };
     unsigned wa[IM], wb[IN];
-    issue(0, 0);
-    for (int kb = 0; kb < g.Kb; ++kb) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();                                                 // step kb is in LDS; everyone has read step kb - 1
-        if ((kb & 3) == 0) {
+    auto words = [&](int kb) {
+        const int at = kb & (C::SC - 1);
 #pragma unroll
-            for (int i = 0; i < IM; ++i) wa[i] = scale_word(g.sa, oa[i] + kb, ta);
+        for (int i = 0; i < IM; ++i) wa[i] = *reinterpret_cast<const unsigned*>(sca + (wm * (TM / WM) + i * 32 + fr) * C::SROW + at);
 #pragma unroll
-            for (int j = 0; j < IN; ++j) wb[j] = scale_word(g.sb, ob[j] + kb, tb);
-        }
-        if (kb + 1 < g.Kb) issue(kb + 1, (kb + 1) & 1);
-        const char* base = smem + (kb & 1) * STAGE;
-        i32x8 fb[IN];
+        for (int j = 0; j < IN; ++j) wb[j] = *reinterpret_cast<const unsigned*>(scb + (BLK ? (wn * (TN / WN) + j * 32) / QB : wn * (TN / WN) + j * 32 + fr) * C::SROW + at);
+    };
+    auto ready = [&]() {                                                 // all but the newest half block in flight have landed, for every wave
+        __builtin_amdgcn_sched_barrier(0);
+        // not __syncthreads(): its fence would drain the DMA left in flight
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_waitcnt lgkmcnt(0)\n\ts_barrier" :: "n"(C::DMA) : "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto multiply = [&](int set, int sh) {
+        if constexpr (DT == CNM_F32) {
 #pragma unroll
-        for (int j = 0; j < IN; ++j) {
-            const int r = TM + wn * (TN / WN) + j * 16 + fr, sw = (r >> 1) & 7;
-            const i32x4 lo = *reinterpret_cast<const i32x4*>(base + r * QB + ((2 * fg) ^ sw) * 16), hi = *reinterpret_cast<const i32x4*>(base + r * QB + ((2 * fg + 1) ^ sw) * 16);
-            fb[j] = i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        }
-        const int sh = 8 * (kb & 3);
+            for (int h = 0; h < 4; ++h) {
+                bf16x8 xb[IN];
 #pragma unroll
-        for (int i = 0; i < IM; ++i) {
-            const int r = wm * (TM / WM) + i * 16 + fr, sw = (r >> 1) & 7;
-            const i32x4 lo = *reinterpret_cast<const i32x4*>(base + r * QB + ((2 * fg) ^ sw) * 16), hi = *reinterpret_cast<const i32x4*>(base + r * QB + ((2 * fg + 1) ^ sw) * 16);
-            const i32x8 fa = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            if constexpr (DT == CNM_F32) {
+                for (int j = 0; j < IN; ++j) xb[j] = widen(fb[set][j][2 * h], fb[set][j][2 * h + 1], scale_float(wb[j], sh));
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    const bf16x8 xa = widen(fa[2 * h], fa[2 * h + 1], scale_float(wa[i], sh));
+                for (int i = 0; i < IM; ++i) {
+                    const bf16x8 xa = widen(fa[set][i][2 * h], fa[set][i][2 * h + 1], scale_float(wa[i], sh));
 #pragma unroll
-                    for (int j = 0; j < IN; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(fb[j][2 * h], fb[j][2 * h + 1], scale_float(wb[j], sh)), xa, acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < IN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xb[j], xa, acc[i][j], 0, 0, 0);
                 }
-            } else {
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < IM; ++i)
 #pragma unroll
                 for (int j = 0; j < IN; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa, acc[i][j], 0, 0, 0, (int)((wb[j] >> sh) & 255u), 0, (int)((wa[i] >> sh) & 255u));
-            }
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[set][j], fa[set][i], acc[i][j], 0, 0, 0, (int)((wb[j] >> sh) & 255u), 0, (int)((wa[i] >> sh) & 255u));
         }
+    };
+
+    issue(0);
+    issue(1);
+    fill(sca, g.sa, m0, TM, g.M - 1, 0);
+    fill(scb, g.sb, n0 >> g.bshift, C::BROWS, (g.N - 1) >> g.bshift, 0);
+    issue(2);
+    __syncthreads();                                                     // everything issued so far is in LDS
+    load(0, 0);
+    for (int kb = 0; kb < Kb; ++kb) {
+        if (kb && (kb & (C::SC - 1)) == 0) {
+            __syncthreads();
+            fill(sca, g.sa, m0, TM, g.M - 1, kb);
+            fill(scb, g.sb, n0 >> g.bshift, C::BROWS, (g.N - 1) >> g.bshift, kb);
+            __syncthreads();
+        }
+        if ((kb & 3) == 0) words(kb);
+        const int s = 2 * kb, sh = 8 * (kb & 3);
+        ready();                                                         // half block s + 1 is in LDS; nobody reads s - 1 any more
+        issue(s + 3);
+        load(s + 1, 1);
+        multiply(0, sh);
+        if constexpr (DT != CNM_F32) Interleave<0, IM * IN, 2 * (IM + IN), C::DMA>::go();
+        ready();
+        issue(s + 4);
+        load(s + 2, 0);                                                  // (behind the last one: a stale or zeroed half block, not used)
+        multiply(1, sh);
+        if constexpr (DT != CNM_F32) Interleave<0, IM * IN, 2 * (IM + IN), C::DMA>::go();
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                     // no DMA outlives the loop
     // the last products stay above the stores' bounds checks: a matrix instruction sunk into divergent code would find its scales written for
     // some lanes only
 #pragma unroll
     for (int i = 0; i < IM; ++i)
 #pragma unroll
         for (int j = 0; j < IN; ++j) asm volatile("" : "+v"(acc[i][j]));
+    // the wave's outputs through LDS (its own part of the ring), so that they leave as whole 128-byte lines: straight from the accumulators a
+    // store instruction would touch 32 rows, 16 bytes each
     typedef typename Elem<DT>::T T;
-    T* c = static_cast<T*>(g.c);
-    const bool four = (g.ldc & 3) == 0 && (reinterpret_cast<uintptr_t>(c) & (4 * sizeof(T) - 1)) == 0;
+    constexpr int WTM = TM / WM, WTN = TN / WN, E = 16 / (int)sizeof(T), CH = WTN / E;    // 16-byte chunks per row, permuted by the row
+    static_assert(TM * TN * (int)sizeof(T) <= C::NST * C::STAGE && CH % 8 == 0, "epilogue");
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    typedef T TE __attribute__((ext_vector_type(E)));
+    asm volatile("s_barrier" ::: "memory");                              // every wave has read its last fragments
+    char* const mine = smem + wave * WTM * WTN * (int)sizeof(T);
 #pragma unroll
     for (int i = 0; i < IM; ++i) {
-        const int m = m0 + wm * (TM / WM) + i * 16 + fr;
+        const int row = i * 32 + fr;
 #pragma unroll
-        for (int j = 0; j < IN; ++j) {
-            const int n = n0 + wn * (TN / WN) + j * 16 + 4 * fg;
-            if (m < g.M && n < g.N) {
-                T* p = c + (size_t)m * g.ldc + n;
-                if (four && n + 3 < g.N) {
-                    typedef T T4 __attribute__((ext_vector_type(4)));
-                    *reinterpret_cast<T4*>(p) = T4{Elem<DT>::down(acc[i][j][0]), Elem<DT>::down(acc[i][j][1]), Elem<DT>::down(acc[i][j][2]), Elem<DT>::down(acc[i][j][3])};
-                } else {
+        for (int j = 0; j < IN; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) if (n + e < g.N) p[e] = Elem<DT>::down(acc[i][j][e]);
+            for (int q = 0; q < 4; ++q) {
+                const int n = j * 32 + 8 * q + 4 * fh;
+                const T4 v = {Elem<DT>::down(acc[i][j][4 * q]), Elem<DT>::down(acc[i][j][4 * q + 1]), Elem<DT>::down(acc[i][j][4 * q + 2]), Elem<DT>::down(acc[i][j][4 * q + 3])};
+                *reinterpret_cast<T4*>(mine + (row * CH + ((n / E) ^ (row & 7))) * 16 + (n % E) * (int)sizeof(T)) = v;
+            }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    T* const c = static_cast<T*>(g.c);
+    const bool whole = g.ldc % E == 0 && (reinterpret_cast<uintptr_t>(c) & 15) == 0;
+    constexpr int RPI = 64 / CH;                                         // rows per store instruction
+#pragma unroll 4
+    for (int p = 0; p < WTM / RPI; ++p) {
+        const int row = p * RPI + lane / CH, ch = lane % CH;
+        const int m = m0 + wm * WTM + row, n = n0 + wn * WTN + ch * E;
+        const TE v = *reinterpret_cast<const TE*>(mine + (row * CH + (ch ^ (row & 7))) * 16);
+        if (m < g.M && n < g.N) {
+            T* const d = c + (size_t)m * g.ldc + n;
+            if (whole && n + E <= g.N) *reinterpret_cast<TE*>(d) = v;
+            else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) if (n + e < g.N) d[e] = v[e];
+            }
+        }
+    }
+}
+
+template <int TM, int TN, int WM, int WN, int DT>
+int launch_tiles(MatArgs g, hipStream_t stream) {
+    g.tiles_m = cnm_ceil_div(g.M, TM); g.tiles_n = cnm_ceil_div(g.N, TN);
+    if (g.bshift) matmul_fp8_kernel<TM, TN, WM, WN, DT, true><<<g.tiles_m * g.tiles_n, WM * WN * 64, Mat<TM, TN, WM, WN, DT, true>::LDS, stream>>>(g);
+    else matmul_fp8_kernel<TM, TN, WM, WN, DT, false><<<g.tiles_m * g.tiles_n, WM * WN * 64, Mat<TM, TN, WM, WN, DT, false>::LDS, stream>>>(g);
+    CNM_LAUNCH_CHECK();
+    return CNM_OK;
+}
+
+template <int DT>
+int launch_matmul(const MatArgs& g, hipStream_t stream) {
+    // 256 x 256 tiles (eight waves of 128 x 64, one workgroup per CU) from more tiles than half the CUs on; below that twice as many CUs
+    // work on 128 x 128 tiles (four waves of 64 x 64, two workgroups per CU).  bf16, 4096 x 4096 x 8192 (256 / 1024 tiles): 117 us against
+    // 166; 2048 x 2048 x 2048 (64 / 256 tiles): 25 us against 13.5.  fp32 results convert their operands on the way: 128 x 128 only
+    // (64 accumulators per lane leave room for the bf16 fragments).
+    if constexpr (DT != CNM_F32)
+        if ((long long)cnm_ceil_div(g.M, 256) * cnm_ceil_div(g.N, 256) > 128) return launch_tiles<256, 256, 2, 4, DT>(g, stream);
+    return launch_tiles<128, 128, 2, 2, DT>(g, stream);
+}
+
+// ------------------------------------------------------------------ few rows, or few columns
+// Where one side is small the product reads the other side once and is bound by that: no LDS staging, fragments straight from memory, MT tiles
+// of 16 rows of x against NT_ tiles of 16 rows of w per wave, PF blocks of 128 requested before the first is used.
+//   few rows (single tokens up to 64): a workgroup takes 16 weight rows, its eight waves share the reduced axis (KS = 8) and join their sums in LDS
+//     in a fixed order;
+//   few columns (N <= 128): a wave takes 16 MT rows of x and all of w, which stays in the caches (KS = 1).
+// QUANT: x comes as it is (float32 / float16 / bfloat16) and is quantised in registers: a lane holds 32 consecutive values of one row, its
+// block's maximum is two exchanges away; x is then read once and never written in 8 bits.
+struct StreamArgs {
+    const void* x; long long ldx;            // [M][ldx] as it is, or e4m3 [M][Kb * 128] with scale sx [M][Kb]
+    const unsigned char *sx, *w, *sw;
+    void* c; long long ldc;
+    int M, N, K, Kb, bshift;                 // K: columns of x that exist (QUANT)
+};
+
+template <int DT, bool QUANT, int MT, int NT_, int KS, int PF>
+__global__ __launch_bounds__(512) void stream_kernel(const StreamArgs g) {
+    typedef typename Elem<DT>::T T;
+    constexpr int MG = 8 / KS;                                           // row groups per workgroup
+    __shared__ float part[KS > 1 ? KS : 1][KS > 1 ? NT_ * 16 : 1][KS > 1 ? MT * 16 + 1 : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ks = wave % KS, mg = wave / KS, fr = lane & 15, fg = lane >> 4;
+    const int nblocks = (g.N + NT_ * 16 - 1) / (NT_ * 16);
+    const int nb = blockIdx.x % nblocks;
+    const int n0 = nb * NT_ * 16, m0 = (int)(blockIdx.x / nblocks * MG + mg) * MT * 16;
+    const unsigned char* wp[NT_]; const unsigned char* swp[NT_];
+#pragma unroll
+    for (int j = 0; j < NT_; ++j) {
+        const int n = min(n0 + j * 16 + fr, g.N - 1);
+        wp[j] = g.w + (size_t)n * g.Kb * QB + fg * 32;
+        swp[j] = g.sw + (size_t)(n >> g.bshift) * g.Kb;
+    }
+    const T* xp[MT]; const unsigned char* qp[MT]; const unsigned char* sxp[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int m = min(m0 + i * 16 + fr, g.M - 1);
+        if (QUANT) xp[i] = static_cast<const T*>(g.x) + (size_t)m * g.ldx + fg * 32;
+        else { qp[i] = static_cast<const unsigned char*>(g.x) + (size_t)m * g.Kb * QB + fg * 32; sxp[i] = g.sx + (size_t)m * g.Kb; }
+    }
+    f32x4 acc[MT][NT_] = {};
+    for (int g0 = ks; g0 < g.Kb; g0 += KS * PF) {
+        i32x8 fw[PF][NT_], fx[PF][QUANT ? 1 : MT];
+        int bw[PF][NT_], bx[PF][MT];
+        T raw[PF][QUANT ? MT : 1][32];
+#pragma unroll
+        for (int p = 0; p < PF; ++p) {
+            const int kb = g0 + p * KS;
+            if (kb < g.Kb) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    if constexpr (QUANT) {
+                        const T* const src = xp[i] + (size_t)kb * QB;
+                        const int have = g.K - kb * QB - fg * 32;
+                        if (have >= 32) __builtin_memcpy(raw[p][i], src, 32 * sizeof(T));
+                        else {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) raw[p][i][e] = e < have ? src[e] : (T)0.f;
+                        }
+                    } else {
+                        __builtin_memcpy(&fx[p][i], qp[i] + (size_t)kb * QB, 32);
+                        bx[p][i] = sxp[i][kb];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < NT_; ++j) {
+                    __builtin_memcpy(&fw[p][j], wp[j] + (size_t)kb * QB, 32);
+                    bw[p][j] = swp[j][kb];
+                }
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < PF; ++p) {
+            if (g0 + p * KS < g.Kb) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    i32x8 fa;
+                    int ba;
+                    if constexpr (QUANT) {
+                        float v[32], m = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) { v[e] = Elem<DT>::up(raw[p][i][e]); m = fmaxf(m, fabsf(v[e])); }
+                        m = fmaxf(m, __shfl_xor(m, 16)); m = fmaxf(m, __shfl_xor(m, 32));
+                        if (__any(m == __builtin_huge_valf())) {         // an infinity in some row's block: it does not take part in the maximum
+                            m = 0.f;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) m = fmaxf(m, finite_abs(v[e]));
+                            m = fmaxf(m, __shfl_xor(m, 16)); m = fmaxf(m, __shfl_xor(m, 32));
+                        }
+                        ba = scale_byte(m);
+                        const float k = inv_scale(ba);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) fa[e] = (int)pack4(v[4 * e] * k, v[4 * e + 1] * k, v[4 * e + 2] * k, v[4 * e + 3] * k);
+                    } else {
+                        fa = fx[p][i]; ba = bx[p][i];
+                    }
+                    if constexpr (DT == CNM_F32) {
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            const bf16x8 xa = widen(fa[2 * h], fa[2 * h + 1], scale_float((unsigned)ba, 0));
+#pragma unroll
+                            for (int j = 0; j < NT_; ++j)
+                                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(fw[p][j][2 * h], fw[p][j][2 * h + 1], scale_float((unsigned)bw[p][j], 0)), xa, acc[i][j], 0, 0, 0);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < NT_; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[p][j], fa, acc[i][j], 0, 0, 0, bw[p][j], 0, ba);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT_; ++j) asm volatile("" : "+v"(acc[i][j]));  // above the bounds checks (see the tile kernel)
+    T* const c = static_cast<T*>(g.c);
+    if constexpr (KS > 1) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT_; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) part[ks][j * 16 + 4 * fg + e][i * 16 + fr] = acc[i][j][e];
+        __syncthreads();
+        for (int o = threadIdx.x; o < MT * 16 * NT_ * 16; o += 512) {
+            const int n = o % (NT_ * 16), m = o / (NT_ * 16);
+            float s = part[0][n][m];
+#pragma unroll
+            for (int k = 1; k < KS; ++k) s += part[k][n][m];
+            if (m0 + m < g.M && n0 + n < g.N) c[(size_t)(m0 + m) * g.ldc + n0 + n] = Elem<DT>::down(s);
+        }
+    } else {
+        const bool four = (g.ldc & 3) == 0 && (reinterpret_cast<uintptr_t>(c) & (4 * sizeof(T) - 1)) == 0;
+        typedef T T4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int m = m0 + i * 16 + fr;
+#pragma unroll
+            for (int j = 0; j < NT_; ++j) {
+                const int n = n0 + j * 16 + 4 * fg;
+                if (m < g.M && n < g.N) {
+                    T* const d = c + (size_t)m * g.ldc + n;
+                    if (four && n + 4 <= g.N) *reinterpret_cast<T4*>(d) = T4{Elem<DT>::down(acc[i][j][0]), Elem<DT>::down(acc[i][j][1]), Elem<DT>::down(acc[i][j][2]), Elem<DT>::down(acc[i][j][3])};
+                    else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) if (n + e < g.N) d[e] = Elem<DT>::down(acc[i][j][e]);
+                    }
                 }
             }
         }
     }
 }
 
-template <int DT>
-int launch_matmul(MatArgs g, hipStream_t stream) {
-    constexpr int TM = 128, TN = 128;
-    g.tiles_m = cnm_ceil_div(g.M, TM); g.tiles_n = cnm_ceil_div(g.N, TN);
-    matmul_fp8_kernel<TM, TN, 2, 2, DT><<<g.tiles_m * g.tiles_n, 256, 2 * (TM + TN) * QB, stream>>>(g);
+template <int DT, bool QUANT, int MT, int NT_, int KS, int PF>
+int launch_stream(const StreamArgs& g, hipStream_t stream) {
+    const long long blocks = (long long)cnm_ceil_div(g.N, NT_ * 16) * cnm_ceil_div(g.M, 8 / KS * MT * 16);
+    stream_kernel<DT, QUANT, MT, NT_, KS, PF><<<(unsigned)blocks, 512, 0, stream>>>(g);
     CNM_LAUNCH_CHECK();
     return CNM_OK;
 }
+
+// few rows of 8-bit x
+template <int DT>
+int launch_few_rows(const StreamArgs& g, hipStream_t stream) {
+    if (g.M <= 16) return launch_stream<DT, false, 1, 1, 8, 4>(g, stream);
+    if (g.M <= 32) return launch_stream<DT, false, 2, 1, 8, 4>(g, stream);
+    if (g.M <= 48) return launch_stream<DT, false, 3, 1, 8, 4>(g, stream);
+    return launch_stream<DT, false, 4, 1, 8, 4>(g, stream);
+}
+
+// x as it is: few columns, or at most 16 rows
+template <int DT>
+int launch_quantizing(const StreamArgs& g, hipStream_t stream) {
+    if (g.M <= 16) return launch_stream<DT, true, 1, 1, 8, 4>(g, stream);
+    if (g.N <= 64) return launch_stream<DT, true, 1, 4, 1, 1>(g, stream);
+    return launch_stream<DT, true, 1, 8, 1, 1>(g, stream);
+}
+
+constexpr int FEW_ROWS = 64, FEW_COLS = 128;
 
 }  // namespace
 
@@ -367,10 +648,44 @@ extern "C" int cnm_matmul_fp8(const void* a, const void* a_scale, const void* b,
     CNM_REQUIRE(cnm_ceil_div_ll(M, 16) * cnm_ceil_div_ll(N, 16) < (1ll << 31), CNM_ERR_BAD_SHAPE);
     MatArgs g = {static_cast<const unsigned char*>(a), static_cast<const unsigned char*>(a_scale), static_cast<const unsigned char*>(b), static_cast<const unsigned char*>(b_scale),
                  c, (int)M, (int)N, (int)(K / QB), b_block_rows == 1 ? 0 : 7, ldc, 0, 0};
+    const StreamArgs f = {a, 0, g.sa, g.b, g.sb, c, ldc, g.M, g.N, (int)K, g.Kb, g.bshift};
+    const hipStream_t st = cnm_stream(stream);
+#define CNM_M(DT) return M <= FEW_ROWS ? launch_few_rows<DT>(f, st) : launch_matmul<DT>(g, st)
     switch (dtype) {
-        case CNM_F32: return launch_matmul<CNM_F32>(g, cnm_stream(stream));
-        case CNM_F16: return launch_matmul<CNM_F16>(g, cnm_stream(stream));
-        case CNM_BF16: return launch_matmul<CNM_BF16>(g, cnm_stream(stream));
+        case CNM_F32: CNM_M(CNM_F32);
+        case CNM_F16: CNM_M(CNM_F16);
+        case CNM_BF16: CNM_M(CNM_BF16);
+    }
+#undef CNM_M
+    return CNM_ERR_BAD_ARG;
+}
+
+extern "C" size_t cnm_linear_fp8_workspace_bytes(long long M, long long N, long long K) {
+    if (M <= 0 || N <= 0 || K <= 0 || M <= 16 || N <= FEW_COLS) return 0;
+    const size_t kb = (size_t)cnm_ceil_div_ll(K, QB);
+    return (size_t)M * kb * (QB + 1);
+}
+
+extern "C" int cnm_linear_fp8(const void* x, int dtype, long long ldx, const void* w, const void* w_scale, void* y, long long ldy,
+                              long long M, long long N, long long K, void* workspace, size_t workspace_bytes, void* stream) {
+    CNM_REQUIRE(x && w && w_scale && y && M > 0 && N > 0 && K > 0 && ldx >= K && ldy >= N, CNM_ERR_BAD_ARG);
+    CNM_REQUIRE((reinterpret_cast<uintptr_t>(w) & 15) == 0 && dtype >= CNM_F32 && dtype <= CNM_BF16, CNM_ERR_BAD_ARG);
+    CNM_REQUIRE(M < (1ll << 31) - 256 && N < (1ll << 31) - 256 && K <= (1ll << 23) && cnm_ceil_div_ll(M, 16) * cnm_ceil_div_ll(N, 16) < (1ll << 31), CNM_ERR_BAD_SHAPE);
+    const size_t need = cnm_linear_fp8_workspace_bytes(M, N, K);
+    const long long kb = cnm_ceil_div_ll(K, QB);
+    if (need) {                                                          // quantise, then multiply
+        CNM_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, CNM_ERR_WORKSPACE);
+        unsigned char* const q = static_cast<unsigned char*>(workspace);
+        unsigned char* const s = q + (size_t)M * kb * QB;
+        const int rc = cnm_quantize_fp8(x, dtype, ldx, M, K, 1, q, s, nullptr, nullptr, stream);
+        return rc != CNM_OK ? rc : cnm_matmul_fp8(q, s, w, w_scale, QB, y, dtype, ldy, M, N, kb * QB, stream);
+    }
+    const StreamArgs f = {x, ldx, nullptr, static_cast<const unsigned char*>(w), static_cast<const unsigned char*>(w_scale), y, ldy, (int)M, (int)N, (int)K, (int)kb, 7};
+    const hipStream_t st = cnm_stream(stream);
+    switch (dtype) {
+        case CNM_F32: return launch_quantizing<CNM_F32>(f, st);
+        case CNM_F16: return launch_quantizing<CNM_F16>(f, st);
+        case CNM_BF16: return launch_quantizing<CNM_BF16>(f, st);
     }
     return CNM_ERR_BAD_ARG;
 }

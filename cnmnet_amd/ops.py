@@ -763,6 +763,29 @@ def _dev_any(*tensors):
     return dev
 
 
+class _Here:
+    """`with` for a device that already is the current one."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _on(dev):
+    """torch.cuda.device(dev), free of charge where dev is current: these operators are called for single tokens, where the host's share counts."""
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _raw_stream(dev):
+    """The current stream of dev as an integer, without building a torch.cuda.Stream."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
 def _rows2d(x, what):
     """x [..., C] -> (2-D view or copy with dense rows, its row stride)."""
     if x.dim() == 0 or x.shape[-1] == 0:
@@ -793,8 +816,8 @@ def quantize_fp8(x, block_rows=1, transposed=False):
         out += (torch.empty(C, Rb * 128, device=dev, dtype=torch.float8_e4m3fn),
                 torch.empty(C if block_rows == 1 else Cb, Rb, device=dev, dtype=torch.float8_e8m0fnu))
     if R:
-        with torch.cuda.device(dev):
-            _lib.check(_lib.load().cnm_quantize_fp8(_p(x), DTYPES[x.dtype], ld, R, C, block_rows, _p(q), _p(s), *([_p(t) for t in out[2:]] or [0, 0]), _stream()))
+        with _on(dev):
+            _lib.check(_lib.load().cnm_quantize_fp8(_p(x), DTYPES[x.dtype], ld, R, C, block_rows, _p(q), _p(s), *([_p(t) for t in out[2:]] or [0, 0]), _raw_stream(dev)))
     return out
 
 
@@ -832,8 +855,8 @@ def matmul_fp8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
     M, N, K = a.shape[0], b.shape[0], a.shape[1]
     c = torch.empty(M, N, device=a.device, dtype=dtype)
     if M and N:
-        with torch.cuda.device(a.device):
-            _lib.check(_lib.load().cnm_matmul_fp8(_p(a), _p(a_scale), _p(b), _p(b_scale), bb, _p(c), DTYPES[dtype], N, M, N, K, _stream()))
+        with _on(a.device):
+            _lib.check(_lib.load().cnm_matmul_fp8(_p(a), _p(a_scale), _p(b), _p(b_scale), bb, _p(c), DTYPES[dtype], N, M, N, K, _raw_stream(a.device)))
     return c
 
 
@@ -845,8 +868,16 @@ def linear_fp8(x, w_packed, w_scale):
         raise _lib.EngineError("linear_fp8: x on %s, weight on %s" % (dev, w_packed.device))
     if x.dim() == 0 or (x.shape[-1] + 127) // 128 * 128 != w_packed.shape[1]:
         raise _lib.EngineError("linear_fp8: x %s does not fit a weight packed as %s" % (tuple(x.shape), tuple(w_packed.shape)))
-    q, s = quantize_fp8(x)
-    return matmul_fp8(q, s, w_packed, w_scale, x.dtype).view(*x.shape[:-1], w_packed.shape[0])
+    x2, ld = _rows2d(x, "linear_fp8")
+    (M, K), N = x2.shape, w_packed.shape[0]
+    y = torch.empty(x.shape[:-1] + (N,), device=dev, dtype=x.dtype)
+    if M and N:
+        lib = _lib.load()
+        n = lib.cnm_linear_fp8_workspace_bytes(M, N, K)
+        ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
+        with _on(dev):
+            _lib.check(lib.cnm_linear_fp8(x2.data_ptr(), DTYPES[x.dtype], ld, w_packed.data_ptr(), w_scale.data_ptr(), y.data_ptr(), N, M, N, K, _p(ws), n, _raw_stream(dev)))
+    return y
 
 
 # ------------------------------------------------------------------ distillation from a teacher's top logits
@@ -911,8 +942,8 @@ def top_logits(logits, k, dim=-1, temperature=1.0):
     idx = torch.empty(c.sized(k), device=dev, dtype=torch.int32)
     lse = torch.empty(c.row_shape, device=dev, dtype=torch.float32)
     if c.rows:
-        with torch.cuda.device(dev):
-            _lib.check(lib.cnm_top_logits(_p(c.z), DTYPES[logits.dtype], c.ld, T, _p(val), _p(idx), _p(lse), c.rows, c.V, k, c.inner, _stream()))
+        with _on(dev):
+            _lib.check(lib.cnm_top_logits(_p(c.z), DTYPES[logits.dtype], c.ld, T, _p(val), _p(idx), _p(lse), c.rows, c.V, k, c.inner, _raw_stream(dev)))
     return c.back(val), c.back(idx), lse
 
 
@@ -959,10 +990,10 @@ class DistillCall:
             return loss.zero_() if need_loss else None
         n = self.lib.cnm_distill_workspace_doubles(c.rows, c.inner) if self.reduction else 0
         ws = torch.empty(n, device=self.dev, dtype=torch.float64) if n else None
-        with torch.cuda.device(self.dev):
+        with _on(self.dev):
             _lib.check(self.lib.cnm_distill(_p(c.z), DTYPES[self.dtype], c.ld, _p(self.idx), int(self.idx.dtype == torch.int64), _p(self.val), DTYPES[self.val.dtype],
                                             _p(self.lse), self.T, _p(self.weight), _p(grad_out), int(grad_out is not None and self.reduction == 0), int(skip_if_one),
-                                            self.reduction, _p(loss), _p(dz), _p(ws), n, c.rows, c.V, self.K, c.inner, _stream()))
+                                            self.reduction, _p(loss), _p(dz), _p(ws), n, c.rows, c.V, self.K, c.inner, _raw_stream(self.dev)))
         return loss
 
 

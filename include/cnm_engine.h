@@ -872,6 +872,12 @@ int cnm_quantize_fp8(const void* x, int dtype, long long ldx, long long rows, lo
  * b_scale [N][K/128] (b_block_rows 1) or [ceil(N/128)][K/128] (128).  fp32 accumulation, one rounding.  Any M, N >= 1; ldc >= N. */
 int cnm_matmul_fp8(const void* a, const void* a_scale, const void* b, const void* b_scale, int b_block_rows, void* c, int dtype,
                    long long ldc, long long M, long long N, long long K, void* stream);
+/* y [M][ldy] = x w^T for inference: x [M][ldx] of dtype (ldx >= K, any alignment), quantised here (block_rows 1), w [N][K padded to 128] and w_scale
+ * as cnm_quantize_fp8 makes them with block_rows 128; y of x's dtype.  workspace: cnm_linear_fp8_workspace_bytes (0 for few rows or columns,
+ * which are quantised on the way) on 16 bytes, contents irrelevant. */
+size_t cnm_linear_fp8_workspace_bytes(long long M, long long N, long long K);
+int cnm_linear_fp8(const void* x, int dtype, long long ldx, const void* w, const void* w_scale, void* y, long long ldy,
+                   long long M, long long N, long long K, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------ distillation from a teacher's top logits
  * Beside the reference's losses (depthnet/losses.py), which compare maps: these compare distributions over classes (depth planes, tokens).

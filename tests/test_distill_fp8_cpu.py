@@ -45,6 +45,23 @@ def test_matmul_entry_refuses():
     assert with_(_0=4100) == -1
 
 
+def test_linear_entry_refuses():
+    lib = _lib.load()
+    n = lib.cnm_linear_fp8_workspace_bytes(100, 300, 200)
+    assert n == 100 * 2 * 129 and lib.cnm_linear_fp8_workspace_bytes(16, 300, 200) == 0 and lib.cnm_linear_fp8_workspace_bytes(1000, 64, 200) == 0
+    ok = [64, 0, 200, 4096, 64, 4096, 300, 100, 300, 200, 4096, n, 0]
+    def with_(**kw):
+        a = list(ok)
+        for k, v in kw.items():
+            a[int(k[1:])] = v
+        return lib.cnm_linear_fp8(*a)
+    for i in (0, 3, 4, 5, 7, 8, 9):
+        assert with_(**{"_%d" % i: 0}) == -1
+    assert with_(_1=3) == -1 and with_(_2=199) == -1 and with_(_3=4100) == -1 and with_(_6=299) == -1
+    assert with_(_10=0) == -5 and with_(_11=n - 1) == -5 and with_(_10=4100) == -5
+    assert with_(_9=(1 << 23) + 1, _2=1 << 24) == -2
+
+
 def test_top_and_distill_entries_refuse():
     lib = _lib.load()
     top = [64, 0, 100, 1.0, 64, 64, 64, 4, 100, 8, 1, 0]

@@ -101,6 +101,21 @@ def test_product_larger(dtype):
     product(600, 1030, 1030, dtype, 1, 6)
 
 
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_product_long_reduction(block_rows):
+    """More blocks than a workgroup holds scales for at once; few rows and many."""
+    product(130, 140, 9000, torch.float32, block_rows, 5)
+    product(129, 257, 8320, torch.bfloat16, block_rows, 6)
+    product(20, 50, 9000, torch.float16, block_rows, 7)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_product_wide_tiles(dtype):
+    """Enough 256 x 256 tiles for the large-tile kernel, ragged at both ends, odd row length; per-row and per-block scales."""
+    for block_rows, M, N, K in ((128, 2817, 2999, 130), (1, 3071, 2830, 260)):
+        product(M, N, K, dtype, block_rows, M)
+
+
 def test_product_scales_cover_the_exponent_range():
     """Blocks whose scales are far apart, both ways: every block's own power of two reaches its products and no other's."""
     g = torch.Generator().manual_seed(1)
@@ -137,7 +152,8 @@ def test_product_leaves_the_gap_between_rows():
         assert bool((c[M:] == 5.0).all()) and bool((c[:, N:] == 5.0).all())
 
 
-@pytest.mark.parametrize("shape,N", [((1, 700), 300), ((3, 5, 64), 17), ((130, 1025), 64), ((64,), 9), ((48, 2048), 515), ((20, 384), 1)])
+@pytest.mark.parametrize("shape,N", [((1, 700), 300), ((3, 5, 64), 17), ((130, 1025), 64), ((64,), 9), ((48, 2048), 515), ((20, 384), 1), ((16, 2057), 100), ((7, 5000), 33), ((1000, 200), 100),
+                                     ((5000, 128), 128), ((333, 300), 65), ((300, 301), 200), ((17, 129), 129)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_linear_inference(shape, N, dtype):
     K = shape[-1]
@@ -161,6 +177,33 @@ def test_linear_rows_do_not_depend_on_the_batch():
     for n in (1, 2, 15, 16, 17, 31, 33, 64, 65, 128, 300):
         y = ops.linear_fp8(x[:n].to(DEV), q, s).double().cpu()
         assert bool(((y - want[:n]).abs() <= bound[:n]).all()), n
+
+
+def test_linear_nonfinite_and_extreme_inputs():
+    """What quantize_fp8 makes of them, also where the layer quantises on the way (few rows, few columns)."""
+    for M, N in ((3, 200), (200, 40), (200, 300)):
+        x, w = data(M, 300, torch.float32, 5), data(N, 300, torch.float32, 6)
+        x[0, 5], x[1, 290] = float("inf"), float("nan")
+        x[2] *= 1e-30
+        q, s = ops.pack_linear_fp8(w.to(DEV))
+        y = ops.linear_fp8(x.to(DEV), q, s).cpu().double()
+        assert bool(torch.isnan(y[:2]).all()) and not bool(torch.isnan(y[2:]).any())
+        A, B = bf.Operand(x[2:], 1), bf.Operand(w, 128)
+        want = bf.product(A, B)
+        assert bool(((y[2:] - want).abs() <= bf.product_bound(A, B, want, torch.float32)).all())
+        # finite values next to an infinity keep their own scale: the infinity alone makes the row NaN
+        z = x.clone()
+        z[0, 5] = 0
+        assert torch.equal(ops.quantize_fp8(x.to(DEV))[1][0].view(torch.uint8), ops.quantize_fp8(z.to(DEV))[1][0].view(torch.uint8))
+
+
+def test_linear_row_stride_and_alignment():
+    w = data(150, 200, torch.float32, 6)
+    q, s = ops.pack_linear_fp8(w.to(DEV))
+    for dtype in TYPES:
+        base = data(40, 303, dtype, 4).to(DEV)
+        for v in (base[:, :200], base[:, 1:201], base[:, 103:], base[::3, 7:207], base[:9, 5:205]):
+            assert torch.equal(ops.linear_fp8(v, q, s), ops.linear_fp8(v.contiguous(), q, s))
 
 
 def test_linear_no_rows():
