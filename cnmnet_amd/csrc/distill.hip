@@ -499,138 +499,274 @@ __device__ inline unsigned key_of(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// A logit and its class as one number, unique within a row: larger logit first, then the lower class.  0 is below all of them.
+typedef unsigned long long u64;
+__device__ inline u64 rank_of(float x, unsigned v) { return (u64)key_of(x) << 32 | ~v; }
+
 struct TopArgs {
     const void* z; long long ldz;
     float T;
     void* val; int* idx; float* lse;
+    u64* part; float* lpart;                 // [rows][segments][K] ranks and [rows][segments][2] (offset, sum), where a row is split
     long long rows; int V, K; long long inner;
+    int segments, seglen;                    // a row's classes by segments of seglen (a multiple of the vector length)
 };
 
-// One workgroup per row.  Radix selection of the K-th largest key, eight bits at a time, then everything above it, and of its equals the
-// lowest classes; the row is re-read from the caches.
-template <int DT, int NT>
-__global__ __launch_bounds__(NT) void top_rows_kernel(const TopArgs a) {
-    typedef typename Elem<DT>::T T;
-    constexpr int E = 16 / sizeof(T);
-    __shared__ unsigned hist[256];
-    __shared__ unsigned sel[4];                                          // digit, rank left within it, its count, output cursor
-    __shared__ unsigned long long cand[KMAX];
-    __shared__ float shf[32];
-    const int t = threadIdx.x;
-    const long long r = blockIdx.x;
-    const T* z = static_cast<const T*>(a.z) + (size_t)r * a.ldz;
-    const float c = (float)(LOG2E_D / (double)a.T);
-    Run run;
-    sweep<DT, NT>(z, a.V, t, [&](int, const float* x, int) {
-        float m = x[0];
-#pragma unroll
-        for (int j = 1; j < E; ++j) m = fmaxf(m, x[j]);
-        if (m > run.m) run.raise(m, c);
-#pragma unroll
-        for (int j = 0; j < E; ++j) run.s += exp2_((x[j] - run.o) * c);
-    });
-    const Lse l = lse_block<NT>(run.lse(), c, shf);
-    if (t == 0) a.lse[r] = lse_value(l, a.T);
+// What NT threads that share a row need: a barrier, a histogram, the candidates.
+constexpr int CAND = 512;
+struct TopShared {
+    unsigned hist[256];
+    unsigned sel[4];                                                     // digit, rank left within it, its count, output cursor
+    float shf[32];
+    u64 cand[CAND];
+};
+template <int NT>
+__device__ inline void group_sync() {
+    if (NT == 64) { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier(); }
+    else __syncthreads();
+}
 
-    // picks the digit that holds the `left`-th largest of what matches so far
-    auto pick = [&](unsigned left) {
-        __syncthreads();
+// the K-th largest of N numbers per thread (item(i), all distinct but for 0, at least K of them not 0): radix selection, eight bits a round,
+// until a digit's numbers all belong
+template <int NT, int N, class F>
+__device__ inline u64 kth_largest(F item, int K, int t, TopShared& sh) {
+    u64 prefix = 0;
+    unsigned left = (unsigned)K;
+    for (int shift = 56;; shift -= 8) {
+        group_sync<NT>();
+        for (int i = t; i < 256; i += NT) sh.hist[i] = 0u;
+        group_sync<NT>();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const u64 k = item(i);
+            if (k && (shift == 56 || (k ^ prefix) >> (shift + 8) == 0)) atomicAdd(&sh.hist[(unsigned)(k >> shift) & 255u], 1u);
+        }
+        group_sync<NT>();
         if (t < 64) {                                                    // four digits per lane, from the highest down
             unsigned n[4], own = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { n[j] = hist[255 - (4 * t + j)]; own += n[j]; }
+            for (int j = 0; j < 4; ++j) { n[j] = sh.hist[255 - (4 * t + j)]; own += n[j]; }
             unsigned before = own;
             for (int d = 1; d < 64; d <<= 1) { const unsigned u = __shfl_up(before, d); if (t >= d) before += u; }
             before -= own;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (before < left && left <= before + n[j]) { sel[0] = 255 - (4 * t + j); sel[1] = left - before; sel[2] = n[j]; }
+                if (before < left && left <= before + n[j]) { sh.sel[0] = 255 - (4 * t + j); sh.sel[1] = left - before; sh.sel[2] = n[j]; }
                 before += n[j];
             }
         }
-        __syncthreads();
-    };
-    auto clear = [&]() { __syncthreads(); for (int i = t; i < 256; i += NT) hist[i] = 0u; __syncthreads(); };
-
-    unsigned prefix = 0, left = (unsigned)a.K, equal = 0;                // after the rounds: the K-th largest key, how many of its equals belong, how many there are
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        clear();
-        sweep<DT, NT>(z, a.V, t, [&](int, const float* x, int n) {
-#pragma unroll
-            for (int j = 0; j < E; ++j) {
-                const unsigned k = key_of(x[j]);
-                if (j < n && (shift == 24 || (k ^ prefix) >> (shift + 8) == 0)) atomicAdd(&hist[k >> shift & 255u], 1u);
-            }
-        });
-        pick(left);
-        prefix |= sel[0] << shift; left = sel[1]; equal = sel[2];
-    }
-    unsigned last = 0xFFFFFFFFu;                                         // of the equals, the classes up to this one
-    if (equal != left) {                                                 // the left-th LOWEST class among them: the same selection on the inverted class
-        unsigned p2 = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            clear();
-            sweep<DT, NT>(z, a.V, t, [&](int v, const float* x, int n) {
-#pragma unroll
-                for (int j = 0; j < E; ++j) {
-                    const unsigned k = ~(unsigned)(v + j);
-                    if (j < n && key_of(x[j]) == prefix && (shift == 24 || (k ^ p2) >> (shift + 8) == 0)) atomicAdd(&hist[k >> shift & 255u], 1u);
-                }
-            });
-            pick(left);
-            p2 |= sel[0] << shift; left = sel[1];
-        }
-        last = ~p2;
-    }
-    if (t == 0) sel[3] = 0u;
-    __syncthreads();
-    sweep<DT, NT>(z, a.V, t, [&](int v, const float* x, int n) {
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-            const unsigned k = key_of(x[j]);
-            if (j < n && (k > prefix || (k == prefix && (unsigned)(v + j) <= last))) cand[atomicAdd(&sel[3], 1u)] = (unsigned long long)k << 32 | ~(unsigned)(v + j);
-        }
-    });
-    __syncthreads();
-    for (int i = t; i < a.K; i += NT) {                                  // exactly K distinct candidates: a candidate's place is the number of those above it
-        const unsigned long long mine = cand[i];
-        int place = 0;
-        for (int j = 0; j < a.K; ++j) place += cand[j] > mine;
-        const unsigned v = ~(unsigned)mine;
-        a.idx[(size_t)r * a.K + place] = (int)v;
-        static_cast<T*>(a.val)[(size_t)r * a.K + place] = z[v];
+        group_sync<NT>();
+        prefix |= (u64)sh.sel[0] << shift; left = sh.sel[1];
+        if (sh.sel[2] == left || shift == 0) return prefix;
     }
 }
 
+// Of N numbers per thread the K largest, in order, to emit(place, number).  `low`: a lower bound of the K-th largest that keeps the candidates
+// few in the ordinary case; where more than CAND pass it (many equal logits), the K-th largest is selected exactly.  may(i): item(i) >= low,
+// cheaply.
+template <int NT, int N, class M, class F, class O>
+__device__ inline void take_largest(M may, F item, int K, int t, TopShared& sh, O emit) {
+    if (t == 0) sh.sel[3] = 0u;
+    group_sync<NT>();
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (may(i)) {
+            const u64 k = item(i);
+            if (k) { const unsigned at = atomicAdd(&sh.sel[3], 1u); if (at < CAND) sh.cand[at] = k; }
+        }
+    group_sync<NT>();
+    int C = (int)sh.sel[3];
+    if (C > CAND) {
+        const u64 least = kth_largest<NT, N>(item, K, t, sh);
+        group_sync<NT>();
+        if (t == 0) sh.sel[3] = 0u;
+        group_sync<NT>();
+#pragma unroll
+        for (int i = 0; i < N; ++i) { const u64 k = item(i); if (k && k >= least) sh.cand[atomicAdd(&sh.sel[3], 1u)] = k; }   // exactly K
+        group_sync<NT>();
+        C = K;
+    }
+    for (int i = t; i < C; i += NT) {                                    // a candidate's place is the number of those above it
+        const u64 mine = sh.cand[i];
+        int place = 0;
+        for (int j = 0; j < C; ++j) place += sh.cand[j] > mine;
+        if (place < K) emit(place, mine);
+    }
+}
+
+// wave-wide maximum, in every lane
+__device__ inline float wave_max(float x) {
+    for (int d = 32; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
+    return x;
+}
+// a lower bound of the K-th largest of the NT threads' numbers: every wave's r-th largest, r = K / waves rounded up, the smallest of these
+template <int NT>
+__device__ inline float kth_bound(float m, int K, float* sh) {
+    constexpr int W = NT / 64;
+    const int r = (K + W - 1) / W;
+    const float ninf = -__builtin_huge_valf();
+    if (r > 64) return ninf;
+    float w = ninf;
+    for (int i = 0; i < r; ++i) {
+        w = wave_max(m);
+        const u64 who = __ballot(m == w);
+        if (who == 0) return ninf;                                       // (not reached: the maximum is some lane's)
+        if ((int)(threadIdx.x & 63) == __ffsll((unsigned long long)who) - 1) m = ninf;
+    }
+    if (NT == 64) return w;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = w;
+    __syncthreads();
+    w = sh[0];
+    for (int i = 1; i < W; ++i) w = fminf(w, sh[i]);
+    return w;
+}
+
+// NT threads per row or segment of a row, which they hold in registers (NV vectors of 16 bytes each), read once.  Log-sum-exp, then a lower bound of
+// the K-th largest logit from the threads' own maxima, the few logits above it to LDS, and their order by counting.
+template <int DT, int NT, int NV>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void top_rows_kernel(const TopArgs a) {
+    typedef typename Elem<DT>::T T;
+    constexpr int E = 16 / sizeof(T), RPB = NT == 64 ? 4 : 1;
+    __shared__ TopShared shared[RPB];
+    const int sub = NT == 64 ? threadIdx.x >> 6 : 0, t = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
+    TopShared& sh = shared[sub];
+    const long long unit = (long long)blockIdx.x * RPB + sub;            // row and segment
+    if (unit >= a.rows * a.segments) return;                             // (whole waves only: NT == 64)
+    const long long r = unit / a.segments;
+    const int seg = (int)(unit - r * a.segments), v0 = seg * a.seglen, n = min(a.V - v0, a.seglen);
+    const T* z = static_cast<const T*>(a.z) + (size_t)r * a.ldz + v0;
+    const float c = (float)(LOG2E_D / (double)a.T), ninf = -__builtin_huge_valf();
+    typedef T TV __attribute__((ext_vector_type(E)));
+    TV x[NV];
+    float m = ninf;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int at = (i * NT + t) * E;
+        if (at + E <= n) __builtin_memcpy(&x[i], z + at, 16);            // (whatever the row's alignment)
+        else {
+#pragma unroll
+            for (int j = 0; j < E; ++j) x[i][j] = at + j < n ? z[at + j] : (T)ninf;
+        }
+    }
+    float vm[NV];                                                        // the vectors' largest
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        vm[i] = (float)x[i][0];
+#pragma unroll
+        for (int j = 1; j < E; ++j) vm[i] = fmaxf(vm[i], (float)x[i][j]);
+        m = fmaxf(m, vm[i]);
+    }
+    Lse l;
+    const float o = m == ninf || m != m ? 0.f : m;
+    l.o = m == m ? m : ninf; l.s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < E; ++j) l.s += exp2_(((float)x[i][j] - o) * c);
+    const bool odd = l.s != l.s || m != m;                               // a NaN or +inf here: every vector is looked at
+    l = lse_block<NT>(l, c, sh.shf);
+    const float low = kth_bound<NT>(m == m ? m : ninf, a.K, sh.shf);
+    if (a.segments == 1) { if (t == 0) a.lse[r] = lse_value(l, a.T); }
+    else if (t == 0) { a.lpart[2 * unit] = l.o; a.lpart[2 * unit + 1] = l.s; }
+    const auto item = [&](int i) -> u64 {
+        const int at = (i / E * NT + t) * E + i % E;
+        return at < n ? rank_of((float)x[i / E][i % E], (unsigned)(v0 + at)) : 0ull;
+    };
+    const auto may = [&](int i) { return (odd || vm[i / E] >= low) && !((float)x[i / E][i % E] < low); };
+    const int K = min(a.K, n);
+    if (a.segments == 1)
+        take_largest<NT, NV * E>(may, item, K, t, sh, [&](int place, u64 k) {
+            const unsigned v = ~(unsigned)k;
+            a.idx[(size_t)r * a.K + place] = (int)v;
+            static_cast<T*>(a.val)[(size_t)r * a.K + place] = z[v];
+        });
+    else {
+        take_largest<NT, NV * E>(may, item, K, t, sh, [&](int place, u64 k) { a.part[(size_t)unit * a.K + place] = k; });
+        for (int i = K + t; i < a.K; i += NT) a.part[(size_t)unit * a.K + i] = 0ull;
+    }
+}
+
+// joins a row's segments: N ranks per thread
+template <int DT, int N>
+__global__ __launch_bounds__(1024) void top_join_kernel(const TopArgs a) {
+    typedef typename Elem<DT>::T T;
+    __shared__ TopShared sh;
+    const int t = threadIdx.x;
+    const long long r = blockIdx.x;
+    const int total = a.segments * a.K;
+    const float c = (float)(LOG2E_D / (double)a.T), ninf = -__builtin_huge_valf();
+    u64 k[N];
+    float m = ninf;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int at = i * 1024 + t;
+        k[i] = at < total ? a.part[(size_t)r * total + at] : 0ull;
+    }
+    const auto value = [](u64 k) {                                       // key_of's inverse (NaN for NaN)
+        const unsigned u = (unsigned)(k >> 32);
+        return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
+    };
+#pragma unroll
+    for (int i = 0; i < N; ++i) if (k[i]) m = fmaxf(m, value(k[i]));
+    Lse l = {ninf, 0.f};
+    if (t < a.segments) l = {a.lpart[2 * (r * a.segments + t)], a.lpart[2 * (r * a.segments + t) + 1]};
+    l = lse_block<1024>(l, c, sh.shf);
+    if (t == 0) a.lse[r] = lse_value(l, a.T);
+    const float low = kth_bound<1024>(m, a.K, sh.shf);
+    const T* z = static_cast<const T*>(a.z) + (size_t)r * a.ldz;
+    take_largest<1024, N>([&](int i) { return k[i] && !(value(k[i]) < low); }, [&](int i) { return k[i]; }, a.K, t, sh, [&](int place, u64 q) {
+        const unsigned v = ~(unsigned)q;
+        a.idx[(size_t)r * a.K + place] = (int)v;
+        static_cast<T*>(a.val)[(size_t)r * a.K + place] = z[v];
+    });
+}
+
 // Classes in the middle, [outer][V][inner]: a lane per position keeps the KM largest of what it has seen, in order, in registers.  Classes come
-// in ascending order, so "strictly larger" keeps the lowest of equals in front.
+// in ascending order, so "strictly larger" keeps the lowest of equals in front.  Sixteen classes are requested ahead of their use.
 template <int DT, int KM>
 __global__ __launch_bounds__(256) void top_planes_kernel(const TopArgs a) {
     typedef typename Elem<DT>::T T;
+    constexpr int AHEAD = 16;
     const long long r = (long long)blockIdx.x * 256 + threadIdx.x;
     if (r >= a.rows) return;
     const long long ob = r / a.inner, at = r % a.inner;
     const T* z = static_cast<const T*>(a.z) + (size_t)ob * a.V * a.inner + at;
-    const float c = (float)(LOG2E_D / (double)a.T);
+    const float c = (float)(LOG2E_D / (double)a.T), ninf = -__builtin_huge_valf();
     unsigned key[KM];                                                    // 0 is below every key
     int cls[KM];
 #pragma unroll
     for (int i = 0; i < KM; ++i) { key[i] = 0u; cls[i] = 0; }
     Run run;
-#pragma unroll 4
-    for (int v = 0; v < a.V; ++v) {
-        const float x = (float)z[(size_t)v * a.inner];
-        if (x > run.m) run.raise(x, c);
-        run.s += exp2_((x - run.o) * c);
-        const unsigned k = key_of(x);
-        if (k > key[KM - 1]) {                                           // from the last place up: a place takes its upper neighbour if k goes above that, k if it goes here
+    T next[AHEAD];
 #pragma unroll
-            for (int i = KM - 1; i > 0; --i) {
-                cls[i] = k > key[i - 1] ? cls[i - 1] : k > key[i] ? v : cls[i];
-                key[i] = k > key[i - 1] ? key[i - 1] : k > key[i] ? k : key[i];
+    for (int j = 0; j < AHEAD; ++j) next[j] = z[(size_t)min(j, a.V - 1) * a.inner];
+    for (int v0 = 0; v0 < a.V; v0 += AHEAD) {
+        float x[AHEAD], m = ninf;
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            x[j] = v0 + j < a.V ? (float)next[j] : ninf;
+            m = fmaxf(m, x[j]);
+        }
+        if (v0 + AHEAD < a.V) {
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) next[j] = z[(size_t)min(v0 + AHEAD + j, a.V - 1) * a.inner];
+        }
+        if (m > run.m) run.raise(m, c);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            run.s += exp2_((x[j] - run.o) * c);
+            const unsigned k = key_of(x[j]);
+            const int v = v0 + j;
+            if (v < a.V && k > key[KM - 1]) {                            // from the last place up: a place takes its upper neighbour if k goes above that, k if it goes here
+#pragma unroll
+                for (int i = KM - 1; i > 0; --i) {
+                    cls[i] = k > key[i - 1] ? cls[i - 1] : k > key[i] ? v : cls[i];
+                    key[i] = k > key[i - 1] ? key[i - 1] : k > key[i] ? k : key[i];
+                }
+                cls[0] = k > key[0] ? v : cls[0];
+                key[0] = k > key[0] ? k : key[0];
             }
-            cls[0] = k > key[0] ? v : cls[0];
-            key[0] = k > key[0] ? k : key[0];
         }
     }
     const Lse l = run.lse();
@@ -646,18 +782,48 @@ __global__ __launch_bounds__(256) void top_planes_kernel(const TopArgs a) {
 
 constexpr int TOP_PLANES_KMAX = 16;
 
+// How rows are split: a workgroup of 512 threads holds 64 KB of a row; rows that are longer, or so few that they would leave most CUs idle,
+// are cut into up to 64 segments (at least 4 KB each) and joined by a second launch.
+int top_segments(long long rows, int V, int esize) {
+    const int most = 512 * 8 * 16 / esize, least = cnm_ceil_div(V, most);
+    if ((size_t)V * esize <= 8192 || rows >= 128) return least;
+    int want = (int)(256 / rows);
+    const int fit = (int)((size_t)V * esize / 4096);
+    want = want < fit ? want : fit;
+    want = want < 64 ? want : 64;
+    return want > least ? want : least;
+}
+
 template <int DT>
-int launch_top(const TopArgs& a, hipStream_t stream) {
+int launch_top(TopArgs a, hipStream_t stream) {
+    typedef typename Elem<DT>::T T;
+    constexpr int E = 16 / sizeof(T);
     if (a.inner > 1) {
         const unsigned blocks = (unsigned)cnm_ceil_div_ll(a.rows, 256);
         if (a.K <= 4) top_planes_kernel<DT, 4><<<blocks, 256, 0, stream>>>(a);
         else if (a.K <= 8) top_planes_kernel<DT, 8><<<blocks, 256, 0, stream>>>(a);
         else top_planes_kernel<DT, 16><<<blocks, 256, 0, stream>>>(a);
-    } else {
-        if (a.V <= 4096) top_rows_kernel<DT, 256><<<(unsigned)a.rows, 256, 0, stream>>>(a);
-        else top_rows_kernel<DT, 1024><<<(unsigned)a.rows, 1024, 0, stream>>>(a);
+        CNM_LAUNCH_CHECK();
+        return CNM_OK;
     }
+    a.segments = top_segments(a.rows, a.V, (int)sizeof(T));
+    a.seglen = cnm_ceil_div(cnm_ceil_div(a.V, a.segments), E) * E;
+    a.segments = cnm_ceil_div(a.V, a.seglen);
+    const int vecs = a.seglen / E;
+    const unsigned units = (unsigned)(a.rows * a.segments);
+    if (vecs <= 64) top_rows_kernel<DT, 64, 1><<<cnm_ceil_div((int)units, 4), 256, 0, stream>>>(a);
+    else if (vecs <= 256) top_rows_kernel<DT, 64, 4><<<cnm_ceil_div((int)units, 4), 256, 0, stream>>>(a);
+    else if (vecs <= 512) top_rows_kernel<DT, 512, 1><<<units, 512, 0, stream>>>(a);
+    else if (vecs <= 1024) top_rows_kernel<DT, 512, 2><<<units, 512, 0, stream>>>(a);
+    else if (vecs <= 2048) top_rows_kernel<DT, 512, 4><<<units, 512, 0, stream>>>(a);
+    else top_rows_kernel<DT, 512, 8><<<units, 512, 0, stream>>>(a);
     CNM_LAUNCH_CHECK();
+    if (a.segments > 1) {
+        const int total = a.segments * a.K;
+        if (total <= 2048) top_join_kernel<DT, 2><<<(unsigned)a.rows, 1024, 0, stream>>>(a);
+        else top_join_kernel<DT, 16><<<(unsigned)a.rows, 1024, 0, stream>>>(a);
+        CNM_LAUNCH_CHECK();
+    }
     return CNM_OK;
 }
 
@@ -668,12 +834,22 @@ extern "C" int cnm_distill_max_entries(void) { return KMAX; }
 extern "C" int cnm_distill_max_classes(void) { return VMAX; }
 extern "C" int cnm_distill_planes_ok(int classes, int entries) { return classes > 0 && entries > 0 && entries <= KMAX && classes <= VMAX && planes_lds(classes, entries) <= LDS_BYTES; }
 
-extern "C" int cnm_top_logits(const void* z, int dtype, long long ldz, float temperature, void* values, int* indices, float* lse,
+extern "C" size_t cnm_top_logits_workspace_bytes(int dtype, long long rows, int classes, int entries, long long inner) {
+    if (rows <= 0 || classes <= 0 || entries <= 0 || inner != 1 || dtype < CNM_F32 || dtype > CNM_BF16) return 0;
+    const int seg = top_segments(rows, classes, dtype == CNM_F32 ? 4 : 2);
+    return seg > 1 ? (size_t)rows * seg * ((size_t)entries * sizeof(u64) + 2 * sizeof(float)) : 0;
+}
+
+extern "C" int cnm_top_logits(const void* z, int dtype, long long ldz, float temperature, void* values, int* indices, float* lse, void* workspace, size_t workspace_bytes,
                               long long rows, int classes, int entries, long long inner, void* stream) {
     CNM_REQUIRE(z && values && indices && lse && rows > 0 && classes > 0 && inner > 0 && temperature > 0.f && temperature < __builtin_huge_valf(), CNM_ERR_BAD_ARG);
     CNM_REQUIRE(entries > 0 && entries <= classes && entries <= (inner > 1 ? TOP_PLANES_KMAX : KMAX) && rows % inner == 0 && (inner > 1 || ldz >= classes), CNM_ERR_BAD_ARG);
-    CNM_REQUIRE(rows < (1ll << 31) && classes <= (1 << 30), CNM_ERR_BAD_SHAPE);
-    const TopArgs a = {z, ldz, temperature, values, indices, lse, rows, classes, entries, inner};
+    CNM_REQUIRE(rows < (1ll << 30) / 64 * 64 && classes <= VMAX && (inner > 1 || rows * cnm_ceil_div(classes, 4096) < (1ll << 31)), CNM_ERR_BAD_SHAPE);
+    const size_t need = cnm_top_logits_workspace_bytes(dtype, rows, classes, entries, inner);
+    CNM_REQUIRE(!need || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 7) == 0), CNM_ERR_WORKSPACE);
+    u64* const part = static_cast<u64*>(workspace);
+    float* const lpart = need ? reinterpret_cast<float*>(part + (need - (size_t)2 * sizeof(float) * (need / ((size_t)entries * sizeof(u64) + 2 * sizeof(float)))) / sizeof(u64)) : nullptr;
+    const TopArgs a = {z, ldz, temperature, values, indices, lse, part, lpart, rows, classes, entries, inner, 1, 0};
     switch (dtype) {
         case CNM_F32: return launch_top<CNM_F32>(a, cnm_stream(stream));
         case CNM_F16: return launch_top<CNM_F16>(a, cnm_stream(stream));

@@ -941,9 +941,13 @@ def top_logits(logits, k, dim=-1, temperature=1.0):
     val = torch.empty(c.sized(k), device=dev, dtype=logits.dtype)
     idx = torch.empty(c.sized(k), device=dev, dtype=torch.int32)
     lse = torch.empty(c.row_shape, device=dev, dtype=torch.float32)
+    if c.V > lib.cnm_distill_max_classes():
+        raise _lib.EngineError("top_logits: %d classes (at most %d)" % (c.V, lib.cnm_distill_max_classes()))
     if c.rows:
+        n = lib.cnm_top_logits_workspace_bytes(DTYPES[logits.dtype], c.rows, c.V, k, c.inner)
+        ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
         with _on(dev):
-            _lib.check(lib.cnm_top_logits(_p(c.z), DTYPES[logits.dtype], c.ld, T, _p(val), _p(idx), _p(lse), c.rows, c.V, k, c.inner, _raw_stream(dev)))
+            _lib.check(lib.cnm_top_logits(_p(c.z), DTYPES[logits.dtype], c.ld, T, _p(val), _p(idx), _p(lse), _p(ws), n, c.rows, c.V, k, c.inner, _raw_stream(dev)))
     return c.back(val), c.back(idx), lse
 
 

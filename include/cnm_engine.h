@@ -887,8 +887,10 @@ int cnm_linear_fp8(const void* x, int dtype, long long ldx, const void* w, const
  *
  * cnm_top_logits: the `entries` largest logits per row in descending order (ties: the lower class first; NaN above everything, -0 equal to
  * +0), their classes, and lse = log sum exp(z / temperature).  entries <= classes, <= cnm_distill_max_entries() (inner = 1) or
- * cnm_top_logits_planes_max_entries() (inner > 1). */
-int cnm_top_logits(const void* z, int dtype, long long ldz, float temperature, void* values, int* indices, float* lse,
+ * cnm_top_logits_planes_max_entries() (inner > 1); classes <= cnm_distill_max_classes().  workspace: cnm_top_logits_workspace_bytes on 8 bytes
+ * (0 but for long or few rows, which several workgroups share), contents irrelevant. */
+size_t cnm_top_logits_workspace_bytes(int dtype, long long rows, int classes, int entries, long long inner);
+int cnm_top_logits(const void* z, int dtype, long long ldz, float temperature, void* values, int* indices, float* lse, void* workspace, size_t workspace_bytes,
                    long long rows, int classes, int entries, long long inner, void* stream);
 int cnm_top_logits_planes_max_entries(void);
 int cnm_distill_max_entries(void);

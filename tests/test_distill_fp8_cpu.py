@@ -64,7 +64,7 @@ def test_linear_entry_refuses():
 
 def test_top_and_distill_entries_refuse():
     lib = _lib.load()
-    top = [64, 0, 100, 1.0, 64, 64, 64, 4, 100, 8, 1, 0]
+    top = [64, 0, 100, 1.0, 64, 64, 64, 0, 0, 4, 100, 8, 1, 0]
     def t(**kw):
         a = list(top)
         for k, v in kw.items():
@@ -73,10 +73,13 @@ def test_top_and_distill_entries_refuse():
     for i in (0, 4, 5, 6):
         assert t(**{"_%d" % i: 0}) == -1
     assert t(_3=0.0) == -1 and t(_3=float("inf")) == -1 and t(_3=float("nan")) == -1
-    assert t(_9=101) == -1 and t(_9=0) == -1 and t(_8=1000, _2=1000, _9=257) == -1
-    assert t(_2=99) == -1 and t(_10=3) == -1                            # row stride; rows not a multiple of inner
-    assert t(_10=4, _9=17) == -1                                        # planes: at most 16
-    assert t(_1=5) == -1 and t(_7=1 << 31) == -2
+    assert t(_11=101) == -1 and t(_11=0) == -1 and t(_10=1000, _2=1000, _11=257) == -1
+    assert t(_2=99) == -1 and t(_12=3) == -1                            # row stride; rows not a multiple of inner
+    assert t(_12=4, _11=17) == -1                                        # planes: at most 16
+    assert t(_1=5) == -1 and t(_9=1 << 31) == -2 and t(_10=(1 << 20) + 1, _2=1 << 21) == -2
+    need = lib.cnm_top_logits_workspace_bytes(0, 2, 100000, 8, 1)          # two long rows: split
+    assert need > 0 and lib.cnm_top_logits_workspace_bytes(0, 4, 100, 8, 1) == 0
+    assert t(_9=2, _10=100000, _2=100000) == -5 and t(_9=2, _10=100000, _2=100000, _7=64, _8=need - 1) == -5
     n = lib.cnm_distill_workspace_doubles(4, 1)
     assert n >= 4 and lib.cnm_distill_workspace_doubles(5, 2) == 0
     dis = [64, 0, 100, 64, 0, 64, 0, None, 1.0, None, None, 0, 0, 1, 64, None, 64, n, 4, 100, 8, 1, 0]
