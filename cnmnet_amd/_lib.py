@@ -218,8 +218,8 @@ PROTOTYPES = {
     "cnm_distill_max_entries": (c_i, []),
     "cnm_distill_max_classes": (c_i, []),
     "cnm_distill_planes_ok": (c_i, [c_i, c_i]),
-    "cnm_distill_workspace_doubles": (c_sz, [c_ll, c_ll]),
-    "cnm_distill": (c_i, [c_fp, c_i, c_ll, c_fp, c_i, c_fp, c_i, c_fp, c_f, c_fp, c_fp, c_i, c_i, c_i, c_fp, c_fp, c_fp, c_sz, c_ll, c_i, c_i, c_ll, c_fp]),
+    "cnm_distill_workspace_doubles": (c_sz, [c_i, c_ll, c_i, c_ll]),
+    "cnm_distill": (c_i, [c_fp, c_i, c_ll, c_fp, c_i, c_fp, c_i, c_fp, c_f, c_fp, c_fp, c_i, c_i, c_i, c_fp, c_fp, c_fp, c_sz, c_i, c_ll, c_i, c_i, c_ll, c_fp]),
 }
 
 NET_DEPTH, NET_REFINE = 0, 1

@@ -781,21 +781,23 @@ class TopLogitsDistill(torch.autograd.Function):
     def forward(ctx, logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction):
         call = ops.DistillCall(logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction)
         ctx.dz = call.new_grad() if ctx.needs_input_grad[0] and call.reduction else None
+        loss = call.run(True, ctx.dz)
         if ctx.needs_input_grad[0]:
             ctx.save_for_backward(logits, top_idx, top_logits, top_lse, weight)
-            ctx.how = temperature, dim, reduction
-            ctx.captured = torch.cuda.is_current_stream_capturing()
-        return call.run(True, ctx.dz)
+            ctx.call, ctx.captured = call, torch.cuda.is_current_stream_capturing()
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, go):
-        call = ops.DistillCall(*ctx.saved_tensors, *ctx.how)
-        # the forward's gradient serves one backward pass (its buffer is given away), and not a captured one of an eager forward, which is replayed
-        dz = ctx.dz if ctx.captured == torch.cuda.is_current_stream_capturing() else None
-        ctx.dz = None
+        ctx.saved_tensors                                                # (raises if one of them has been changed in place, or the graph freed)
+        call = ctx.call
+        # the forward's gradient serves one backward pass (its buffer is given away); it and the forward's workspace do not serve a captured
+        # backward pass of an eager forward, which is replayed
+        same = ctx.captured == torch.cuda.is_current_stream_capturing()
+        dz, ctx.dz = ctx.dz if same else None, None
         skip = dz is not None
         if dz is None:
             dz = call.new_grad()
-        call.run(False, dz, go.contiguous().float(), skip)
+        call.run(False, dz, go.contiguous().float(), skip, call.ws if same else None)
         return call.c.back(dz), None, None, None, None, None, None, None

@@ -83,28 +83,30 @@ __device__ inline double max_block(double a, double* sh) {
     return a;
 }
 
-// f(first index, E values, how many of them count) over a row in units of 16 bytes where the row allows it: a head up to the first aligned
-// element, vectors, a tail; head and tail elements come one at a time, the rest of E being -inf
-template <int DT, int NT, class F>
-__device__ inline void sweep(const typename Elem<DT>::T* row, int V, int t, F f) {
+// sixteen bytes of a row as they are in memory, elements beyond the row -inf.  hold(): conversions done so far are forgotten (left alone, hipcc
+// keeps every converted element in a register of its own from one pass over the row to the next)
+template <int DT>
+struct Raw {
     typedef typename Elem<DT>::T T;
-    constexpr int E = 16 / sizeof(T);
-    const int mis = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-    const int head = min(V, mis ? E - mis : 0), nvec = (V - head) / E, tail = head + nvec * E;
-    typedef T TV __attribute__((ext_vector_type(E)));
-    const TV* rv = reinterpret_cast<const TV*>(row + head);
-    float x[E];
-    for (int i = t; i < nvec; i += NT) {
-        const TV v = rv[i];
+    static constexpr int E = 16 / sizeof(T);
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 w;
+    __device__ void load(const T* row, int at, int n) {
+        if (at + E <= n) __builtin_memcpy(&w, row + at, 16);             // (whatever the row's alignment)
+        else {
+            T v[E];
 #pragma unroll
-        for (int j = 0; j < E; ++j) x[j] = (float)v[j];
-        f(head + i * E, x, E);
+            for (int j = 0; j < E; ++j) v[j] = at + j < n ? row[at + j] : (T)-__builtin_huge_valf();
+            __builtin_memcpy(&w, v, 16);
+        }
     }
-#pragma unroll
-    for (int j = 1; j < E; ++j) x[j] = -__builtin_huge_valf();
-    if (t < head) { x[0] = (float)row[t]; f(t, x, 1); }
-    if (tail + t < V) { x[0] = (float)row[tail + t]; f(tail + t, x, 1); }   // fewer than E <= NT elements
-}
+    __device__ void hold() { asm volatile("" : "+v"(w)); }
+    __device__ float get(int j) const {
+        if constexpr (DT == CNM_F32) return __uint_as_float(w[j]);
+        else if constexpr (DT == CNM_BF16) return __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
+        else { const unsigned short h = (unsigned short)(j & 1 ? w[j / 2] >> 16 : w[j / 2]); return (float)__builtin_bit_cast(_Float16, h); }
+    }
+};
 
 // running largest value and sum of the exponentials 2^((x - o) c), o = the largest value (0 while there is none but -inf)
 struct Run {
@@ -135,10 +137,15 @@ struct DistillArgs {
     const float* go; int go_rows;            // upstream gradient: one value, or one per row; null: 1
     int skip_if_one;                         // *go == 1: the gradient is already there (written by the forward pass)
     float* loss;                             // [rows] or null
-    double* lpart;                           // per workgroup: sum of weight * loss, or null
+    double* lpart;                           // per row or per workgroup: weight * loss, or null
     void* dz;                                // as z but dense, or null
     long long rows; int V, K; long long inner;
+    struct DistillRow* rec; float* seg;      // rows cut into segments: what each amounts to, and [rows][segments][2] (offset, sum)
+    int segments, seglen;
 };
+
+// What a row amounts to: an unnamed class's gradient is A 2^((z - orest) c), a named one's B (2^((z - oall) c) inv - p); B = 0: nothing
+struct DistillRow { double L; float A, B, orest, oall, inv, pad; };
 
 // sum of up to 64 partial sums, in a fixed order, by a whole wave
 __device__ inline double wave_total(const double* part, int n) {
@@ -147,156 +154,268 @@ __device__ inline double wave_total(const double* part, int n) {
     return s;
 }
 
-// One row per NT threads.  LDS: one bit per class (named by an entry), the entries.  Two sweeps over the row: statistics of the unnamed
-// classes, then the gradient; the second one finds the row in the L2.
-template <int DT, int NT>
-__global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_rows_kernel(const DistillArgs a) {
-    typedef typename Elem<DT>::T T;
-    constexpr int RPB = NT == 64 ? 4 : 1, E = 16 / sizeof(T);
-    extern __shared__ unsigned lds_words[];
-    __shared__ double shd_[RPB][16];
-    __shared__ float shf_[RPB][32];
-    __shared__ int eidx_[RPB][KMAX];
-    __shared__ float ep_[RPB][KMAX];
-    const int sub = NT == 64 ? threadIdx.x >> 6 : 0, t = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
-    const int nw = a.V / 32 + 2;                                         // one word more than the bits need: eight bits are read from any of them on
-    unsigned* bits = lds_words + sub * nw;
-    double* shd = shd_[sub]; float* shf = shf_[sub]; int* eidx = eidx_[sub]; float* ep = ep_[sub];
-    float go = 1.f;
-    if (a.go && !a.go_rows) {
-        go = a.go[0];
-        if (a.skip_if_one && go == 1.f) return;
-    }
-    const long long row = (long long)blockIdx.x * RPB + sub;
-    const bool live = row < a.rows;
-    const long long r = live ? row : 0;
-    const T* z = static_cast<const T*>(a.z) + (size_t)r * a.ldz;
-    double norm = a.inv_norm;
-    if (a.wpart) { const double w = wave_total(a.wpart, a.nwpart); norm = w > 0.0 ? a.inv_norm / w : 0.0; }
-    if (a.go && a.go_rows) go = a.go[r];
-    const float wrow = a.weight ? a.weight[r] : 1.f;
-    const float c = (float)(LOG2E_D / (double)a.T);
-    auto sync = [&]() { if (NT == 64) { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier(); } else __syncthreads(); };
+// 2^x, relative error of a few 2^-24 whatever x's size
+__device__ inline float exp2_of(double x) {
+    if (!(x > -160.0)) return x != x ? (float)x : 0.f;
+    if (x > 130.0) return __builtin_huge_valf();
+    const double n = rint(x);
+    return ldexpf(exp2_((float)(x - n)), (int)n);
+}
 
-    for (int i = t; i < nw; i += NT) bits[i] = 0u;
-    sync();
-    double best = -__builtin_huge_val();
+// The entries of a row, shared by the NT threads that work on it.
+struct Entries {
+    double shd[16];
+    float shf[32];
+    int idx[KMAX];                                                       // -1: none
+    float z[KMAX], p[KMAX];                                              // the student's logit there; the teacher's logit, then the probability
+    int dup;                                                             // some class is named twice
+};
+template <int NT>
+__device__ inline void row_sync() {
+    if (NT == 64) { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); __builtin_amdgcn_wave_barrier(); }
+    else __syncthreads();
+}
+
+template <int DT, int NT>
+__device__ inline void load_entries(const DistillArgs& a, size_t r, const typename Elem<DT>::T* z, Entries& e, int t) {
+    if (t == 0) e.dup = 0;
+    for (int k = t; k < a.K; k += NT) {
+        const long long i = load_index(a.idx, a.wide, r * a.K + k);
+        const bool ok = i >= 0 && i < a.V;
+        e.idx[k] = ok ? (int)i : -1;
+        e.p[k] = ok ? load_any(a.val, a.vdt, r * a.K + k) : 0.f;
+        e.z[k] = ok ? (float)z[i] : 0.f;
+    }
+    row_sync<NT>();
+}
+// the named classes' bits among the n from v0 on; whether a class is named twice
+template <int NT>
+__device__ inline void mark_entries(Entries& e, int K, unsigned* bits, int v0, int n, int t) {
+    for (int k = t; k < K; k += NT) {
+        const int i = e.idx[k] - v0;
+        if (i >= 0 && i < n && e.idx[k] >= 0) atomicOr(&bits[i >> 5], 1u << (i & 31));
+    }
+    for (int q = t; q < K * K; q += NT) {
+        const int k = q / K, j = q - k * K;
+        if (j < k && e.idx[k] >= 0 && e.idx[j] == e.idx[k]) e.dup = 1;
+    }
+    row_sync<NT>();
+}
+template <int NT>
+__device__ inline double teacher_lse(const DistillArgs& a, size_t r, Entries& e, int t) {
+    if (a.lse) return (double)a.lse[r];
+    double best = -__builtin_huge_val(), s = 0.0;
+    for (int k = t; k < a.K; k += NT) if (e.idx[k] >= 0) best = fmax(best, (double)e.p[k]);
+    best = max_block<NT>(best, e.shd);
+    if (best == -__builtin_huge_val()) best = 0.0;
+    for (int k = t; k < a.K; k += NT) if (e.idx[k] >= 0) s += (double)exp2_of(((double)e.p[k] - best) * (LOG2E_D / (double)a.T));
+    s = sum_block<NT>(s, e.shd);
+    return best / (double)a.T + log(s);
+}
+__device__ inline double entry_log2p(const DistillArgs& a, const Entries& e, int k, double L) { return ((double)e.p[k] / (double)a.T - L) * LOG2E_D; }
+
+// a class that is named more than once: its first entry gets the sum, the others become none
+template <int NT>
+__device__ inline void join_entries(Entries& e, int K, int t) {
+    if (!e.dup) return;
+    float s[KMAX / 64];
+    bool first[KMAX / 64];
+#pragma unroll
+    for (int q = 0; q < (KMAX + NT - 1) / NT; ++q) {
+        const int k = q * NT + t;
+        first[q] = k < K && e.idx[k] >= 0; s[q] = 0.f;
+        if (first[q])
+            for (int j = 0; j < K; ++j) if (e.idx[j] == e.idx[k]) { if (j < k) first[q] = false; s[q] += e.p[j]; }
+    }
+    row_sync<NT>();
+#pragma unroll
+    for (int q = 0; q < (KMAX + NT - 1) / NT; ++q) {
+        const int k = q * NT + t;
+        if (k < K) { e.p[k] = s[q]; if (!first[q]) e.idx[k] = -1; }
+    }
+    row_sync<NT>();
+}
+
+// From the unnamed classes' statistics to the loss and the gradient's coefficients (for an upstream gradient of 1); e.p becomes the probabilities.
+template <int NT>
+__device__ inline DistillRow finish_row(const DistillArgs& a, size_t r, bool live, Lse rest, Entries& e, float c, int t) {
+    const float ninf = -__builtin_huge_valf();
+    Lse named = {ninf, 0.f};
     int have = 0;
     for (int k = t; k < a.K; k += NT) {
-        const long long i = load_index(a.idx, a.wide, (size_t)r * a.K + k);
-        const bool ok = i >= 0 && i < a.V;
-        eidx[k] = ok ? (int)i : -1;
-        if (ok) {
-            atomicOr(&bits[i >> 5], 1u << (i & 31));
-            have = 1;
-            best = fmax(best, (double)load_any(a.val, a.vdt, (size_t)r * a.K + k) / (double)a.T);
-        }
-    }
-    sync();
-    have = (int)max_block<NT>((double)have, shd);
-    double L;
-    if (a.lse) L = (double)a.lse[r];
-    else {
-        best = max_block<NT>(best, shd);
-        if (best == -__builtin_huge_val()) best = 0.0;
-        double s = 0.0;
-        for (int k = t; k < a.K; k += NT)
-            if (eidx[k] >= 0) s += (double)exp2_((float)(((double)load_any(a.val, a.vdt, (size_t)r * a.K + k) / (double)a.T - best) * LOG2E_D));
-        s = sum_block<NT>(s, shd);
-        L = best + log(s);
-    }
-    // statistics of the unnamed classes
-    Run run;
-    sweep<DT, NT>(z, a.V, t, [&](int v, const float* x, int) {
-        const unsigned mask = (unsigned)(((unsigned long long)bits[(v >> 5) + 1] << 32 | bits[v >> 5]) >> (v & 31));
-        float m = -__builtin_huge_valf();
-#pragma unroll
-        for (int j = 0; j < E; ++j) m = fmaxf(m, mask >> j & 1u ? -__builtin_huge_valf() : x[j]);
-        if (m > run.m) run.raise(m, c);
-#pragma unroll
-        for (int j = 0; j < E; ++j) run.s += mask >> j & 1u ? 0.f : exp2_((x[j] - run.o) * c);
-    });
-    Lse rest = run.lse();
-    rest = lse_block<NT>(rest, c, shf);
-    // the named classes, each once: its first entry stands for it
-    Lse named = {-__builtin_huge_valf(), 0.f};
-    for (int k = t; k < a.K; k += NT) {
-        const int i = eidx[k];
+        const int i = e.idx[k];
         bool first = i >= 0;
-        for (int j = 0; j < k && first; ++j) first = eidx[j] != i;
+        have |= first;
+        if (e.dup) for (int j = 0; j < k && first; ++j) first = e.idx[j] != i;
         if (first) {
-            const float x = (float)z[i];
-            named = lse_join(named, Lse{x, x == -__builtin_huge_valf() ? 0.f : x == x ? 1.f : x}, c);
+            const float x = e.z[k];
+            named = lse_join(named, Lse{x, x == ninf ? 0.f : x == x ? 1.f : x}, c);
         }
     }
-    named = lse_block<NT>(named, c, shf);
+    DistillRow w;
+    w.L = teacher_lse<NT>(a, r, e, t);
+    named = lse_block<NT>(named, c, e.shf);
     const Lse all = lse_join(rest, named, c);
-    const float oall = all.o == -__builtin_huge_valf() ? 0.f : all.o, orest = rest.o == -__builtin_huge_valf() ? 0.f : rest.o;
+    w.oall = all.o == ninf ? 0.f : all.o; w.orest = rest.o == ninf ? 0.f : rest.o;
     const double lq0 = -log2((double)all.s);                             // log2 q_v = (z_v - oall) c + lq0
-    // entries
-    double P = 0.0, loss = 0.0;
+    double P = 0.0, Q = 0.0, loss = 0.0;
     for (int k = t; k < a.K; k += NT) {
-        const int i = eidx[k];
         float p = 0.f;
-        if (i >= 0) {
-            const double lp = ((double)load_any(a.val, a.vdt, (size_t)r * a.K + k) / (double)a.T - L) * LOG2E_D;
-            p = exp2_((float)lp);
-            if (p > 0.f) loss += (double)p * LN2_D * (lp - (((double)(float)z[i] - (double)oall) * (double)c + lq0));
+        if (e.idx[k] >= 0) {
+            const double lp = entry_log2p(a, e, k, w.L), lq = ((double)e.z[k] - (double)w.oall) * (double)c + lq0;
+            p = exp2_of(lp);
+            if (p > 0.f) loss += (double)p * LN2_D * (lp - lq);
             P += (double)p;
         }
-        ep[k] = p;
+        e.p[k] = p;
     }
-    P = sum_block<NT>(P, shd);
-    loss = sum_block<NT>(loss, shd);
+    if (a.lse) {                                                         // the named classes' probability, each once
+        P = sum_block<NT>(P, e.shd);
+        Q = (double)named.s * (double)exp2_of(((double)named.o - (double)w.oall) * (double)c + lq0);
+        if (named.o == ninf) Q = 0.0;
+    }
+    loss = sum_block<NT>(loss, e.shd);
+    have = (int)max_block<NT>((double)have, e.shd);
     double ratio = 0.0;                                                  // p_r / (sum of the unnamed exponentials)
     if (a.lse && rest.s > 0.f) {
         const double pr = 1.0 - P;
         if (pr > 0.0) {
-            const double lqr = ((double)orest - (double)oall) * (double)c + log2((double)rest.s) + lq0;
-            loss += pr * (log(pr) - lqr * LN2_D);
+            // q_r from the smaller side: 1 - Q keeps its digits where the named classes hold little
+            const double lqr = Q < 0.5 ? log1p(-Q) : (((double)w.orest - (double)w.oall) * (double)c + log2((double)rest.s) + lq0) * LN2_D;
+            loss += pr * (log1p(-P) - lqr);
             ratio = pr / (double)rest.s;
         }
     }
     loss *= (double)a.T * (double)a.T;
     if (!have) loss = 0.0;
+    const float wrow = a.weight ? a.weight[r] : 1.f;
     if (t == 0 && live) {
         if (a.loss) a.loss[r] = (float)loss;
-        if (a.lpart) a.lpart[r] = (wrow != 0.f ? (double)wrow * loss : 0.0);
+        if (a.lpart) a.lpart[r] = wrow != 0.f ? (double)wrow * loss : 0.0;
     }
-    if (!a.dz || !live) return;
-    T* dz = static_cast<T*>(a.dz) + (size_t)r * a.V;
-    const double scale = have && wrow != 0.f ? (double)a.T * (double)go * (double)wrow * norm : 0.0;
-    const bool zero = scale == 0.0;                                      // rows that count for nothing: zeros, whatever the logits hold
-    const double inv = (double)exp2_((orest - oall) * c) / (double)all.s;
-    const float A = (float)(scale * (inv - ratio)), Bp = (float)scale;
-    sync();
-    auto grad = [&](int v, float x) -> float {
-        if (zero) return 0.f;
-        const float e = exp2_((x - orest) * c);
-        if (!(bits[v >> 5] >> (v & 31) & 1u)) return A * e;
-        float p = 0.f;
-        for (int k = 0; k < a.K; ++k) p += eidx[k] == v ? ep[k] : 0.f;
-        // a named class may lie far above the unnamed ones: its own exponent against the whole row's
-        return Bp * (exp2_((x - oall) * c) / all.s - p);
-    };
-    const int mis = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
-    if (((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0) {
-        typedef T TV __attribute__((ext_vector_type(E)));
-        const int head = min(a.V, mis ? E - mis : 0), nvec = (a.V - head) / E, tail = head + nvec * E;
-        if (t < head) dz[t] = (T)grad(t, (float)z[t]);
-        const TV* zv = reinterpret_cast<const TV*>(z + head);
-        TV* dv = reinterpret_cast<TV*>(dz + head);
-        for (int i = t; i < nvec; i += NT) {
-            const TV x = zv[i];
-            TV g;
+    double norm = a.inv_norm;
+    if (a.wpart) { const double s = wave_total(a.wpart, a.nwpart); norm = s > 0.0 ? a.inv_norm / s : 0.0; }
+    const double scale = have && wrow != 0.f ? (double)a.T * (double)wrow * norm : 0.0;
+    w.inv = 1.f / all.s;
+    w.A = rest.s == 0.f ? 0.f : (float)(scale * ((double)exp2_((w.orest - w.oall) * c) / (double)all.s - ratio));   // (no mass outside the entries: nothing to scale)
+    w.B = (float)scale;
+    return w;
+}
+
+// NT threads per row (MODE ROW) or segment of a row, which they hold in registers (NV vectors of 16 bytes each): z is read once, the gradient
+// written once.  LDS: one bit per class (named by an entry), the entries.
+// A row that no workgroup can hold, or one of few, is cut into segments: statistics of each (SEG_STATS), the row's numbers (distill_join_kernel),
+// gradients of each (SEG_GRAD), the second reading from the caches.
+enum { ROW, SEG_STATS, SEG_GRAD };
+template <int DT, int NT, int NV, int MODE>
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_rows_kernel(const DistillArgs a) {
+    typedef typename Elem<DT>::T T;
+    constexpr int RPB = NT == 64 ? 4 : 1, E = 16 / sizeof(T);
+    extern __shared__ unsigned lds_words[];
+    __shared__ Entries entries[RPB];
+    const int sub = NT == 64 ? threadIdx.x >> 6 : 0, t = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
+    const int nw = (a.seglen + 31) / 32;
+    unsigned* const bits = lds_words + sub * nw;
+    Entries& e = entries[sub];
+    float go = 1.f;
+    if (a.go && !a.go_rows) {
+        go = a.go[0];
+        if (a.skip_if_one && go == 1.f) return;
+    }
+    const long long unit = (long long)blockIdx.x * RPB + sub;
+    if (unit >= a.rows * a.segments) return;                             // (whole waves only: NT == 64)
+    const size_t r = (size_t)(unit / a.segments);
+    const int seg = (int)(unit - (long long)r * a.segments), v0 = seg * a.seglen, n = min(a.V - v0, a.seglen);
+    const T* const zrow = static_cast<const T*>(a.z) + r * a.ldz;
+    const T* const z = zrow + v0;
+    if (a.go && a.go_rows) go = a.go[r];
+    const float c = (float)(LOG2E_D / (double)a.T), ninf = -__builtin_huge_valf();
+    Raw<DT> x[NV];
 #pragma unroll
-            for (int j = 0; j < E; ++j) g[j] = (T)grad(head + i * E + j, (float)x[j]);
-            dv[i] = g;
+    for (int i = 0; i < NV; ++i) x[i].load(z, (i * NT + t) * E, n);
+    for (int i = t; i < nw; i += NT) bits[i] = 0u;
+    load_entries<DT, NT>(a, r, zrow, e, t);
+    mark_entries<NT>(e, a.K, bits, v0, n, t);
+    const auto mask = [&](int i) { const int at = (i * NT + t) * E; return at < n ? bits[at >> 5] >> (at & 31) : 0u; };
+    DistillRow w;
+    if constexpr (MODE != SEG_GRAD) {                                    // statistics of the unnamed classes
+        float m = ninf;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            x[i].hold();
+            const unsigned b = mask(i);
+#pragma unroll
+            for (int j = 0; j < E; ++j) m = fmaxf(m, b >> j & 1u ? ninf : x[i].get(j));
         }
-        if (tail + t < a.V) dz[tail + t] = (T)grad(tail + t, (float)z[tail + t]);
+        const float o = m == ninf ? 0.f : m;
+        Lse rest = {m, 0.f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            x[i].hold();
+            const unsigned b = mask(i);
+#pragma unroll
+            for (int j = 0; j < E; ++j) rest.s += b >> j & 1u ? 0.f : exp2_((x[i].get(j) - o) * c);
+        }
+        rest = lse_block<NT>(rest, c, e.shf);
+        if constexpr (MODE == SEG_STATS) {
+            if (t == 0) { a.seg[2 * unit] = rest.o; a.seg[2 * unit + 1] = rest.s; }
+            return;
+        }
+        w = finish_row<NT>(a, r, true, rest, e, c, t);
     } else {
-        for (int v = t; v < a.V; v += NT) dz[v] = (T)grad(v, (float)z[v]);
+        w = a.rec[r];
+        for (int k = t; k < a.K; k += NT) e.p[k] = e.idx[k] >= 0 ? exp2_of(entry_log2p(a, e, k, w.L)) : 0.f;
     }
+    if (!a.dz) return;
+    row_sync<NT>();
+    join_entries<NT>(e, a.K, t);
+    const float A = w.A * go, B = w.B * go;
+    const bool zero = B == 0.f;                                          // rows that count for nothing: zeros, whatever the logits hold
+    T* const dz = static_cast<T*>(a.dz) + r * a.V + v0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int at = (i * NT + t) * E;
+        if (at < n) {
+            x[i].hold();
+            const unsigned b = mask(i) & ((1u << E) - 1);
+            T g[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j) g[j] = (T)(zero ? 0.f : A * exp2_((x[i].get(j) - w.orest) * c));
+            if (b && !zero) {
+                for (int k = 0; k < a.K; ++k) {                          // few classes are named: look up whose
+                    const int j = e.idx[k] - v0 - at;
+                    if (e.idx[k] >= 0 && j >= 0 && j < E) {
+                        // a named class may lie far above the unnamed ones: its own exponent against the whole row's
+                        const T q = (T)(B * (exp2_((e.z[k] - w.oall) * c) * w.inv - e.p[k]));
+#pragma unroll
+                        for (int jj = 0; jj < E; ++jj) g[jj] = jj == j ? q : g[jj];
+                    }
+                }
+            }
+            if (at + E <= n) __builtin_memcpy(dz + at, g, 16);
+            else {
+#pragma unroll
+                for (int j = 0; j < E; ++j) if (at + j < n) dz[at + j] = g[j];
+            }
+        }
+    }
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void distill_join_kernel(const DistillArgs a) {
+    typedef typename Elem<DT>::T T;
+    __shared__ Entries e;
+    const int t = threadIdx.x;
+    if (a.skip_if_one && a.go && a.go[0] == 1.f) return;
+    const size_t r = blockIdx.x;
+    const float c = (float)(LOG2E_D / (double)a.T);
+    load_entries<DT, 256>(a, r, static_cast<const T*>(a.z) + r * a.ldz, e, t);
+    mark_entries<256>(e, a.K, nullptr, 0, 0, t);
+    Lse rest = {-__builtin_huge_valf(), 0.f};
+    if (t < a.segments) rest = {a.seg[2 * (r * a.segments + t)], a.seg[2 * (r * a.segments + t) + 1]};
+    rest = lse_block<256>(rest, c, e.shf);
+    const DistillRow w = finish_row<256>(a, r, true, rest, e, c, t);
+    if (t == 0) a.rec[r] = w;
 }
 
 // The same with the classes in the middle: [outer][V][inner], a workgroup takes 64 neighbouring positions ("pixels"), one per lane; its four
@@ -395,7 +514,7 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
         float p = 0.f;
         if (i >= 0) {
             const double lp = ((double)ep[k * 64 + px] / (double)a.T - L) * LOG2E_D;
-            p = exp2_((float)lp);
+            p = exp2_of(lp);
             if (p > 0.f) loss += (double)p * LN2_D * (lp - (((double)tile[i * 64 + px] - (double)oall) * (double)c + lq0));
             P += (double)p;
         }
@@ -409,8 +528,9 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
     if (a.lse && rest.s > 0.f) {
         const double pr = 1.0 - P;
         if (pr > 0.0) {
-            const double lqr = ((double)orest - (double)oall) * (double)c + log2((double)rest.s) + lq0;
-            loss += pr * (log(pr) - lqr * LN2_D);
+            const double Q = named.o == ninf ? 0.0 : (double)named.s * (double)exp2_of(((double)named.o - (double)oall) * (double)c + lq0);
+            const double lqr = Q < 0.5 ? log1p(-Q) : (((double)orest - (double)oall) * (double)c + log2((double)rest.s) + lq0) * LN2_D;
+            loss += pr * (log1p(-P) - lqr);
             ratio = pr / (double)rest.s;
         }
     }
@@ -427,7 +547,7 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
     if (!a.dz) return;
     const double scale = have && wrow != 0.f ? (double)a.T * (double)go * (double)wrow * norm : 0.0;
     const bool zero = scale == 0.0;
-    const float inv = 1.f / all.s, A = (float)(scale * ((double)exp2_((orest - oall) * c) / (double)all.s - ratio)), Bp = (float)scale;
+    const float inv = 1.f / all.s, A = rest.s == 0.f ? 0.f : (float)(scale * ((double)exp2_((orest - oall) * c) / (double)all.s - ratio)), Bp = (float)scale;
     for (int v = w; v < V; v += 4) {
         const float x = tile[v * 64 + px];
         const bool in = bits[(v >> 5) * 64 + px] >> (v & 31) & 1u;
@@ -475,19 +595,63 @@ __global__ __launch_bounds__(1024) void loss_total_kernel(const double* __restri
     if (threadIdx.x == 0) out[0] = norm != 0.0 ? (float)(s * norm) : 0.f;
 }
 
+// How rows are split: 1024 threads hold 256 KB of a row in registers; longer rows, and long ones of fewer than 128, are cut into segments.
+int distill_segments(long long rows, int V, int esize) {
+    const size_t bytes = (size_t)V * esize;
+    int want = (int)((bytes + (256 << 10) - 1) / (256 << 10));
+    if (rows < 128 && bytes > (16 << 10)) {
+        const int fit = (int)(bytes / (8 << 10)), fill = (int)(256 / rows);
+        const int more = fit < fill ? fit : fill;
+        want = more > want ? more : want;
+    }
+    return want;
+}
+
+template <int DT, int MODE>
+void launch_rows(const DistillArgs& a, hipStream_t stream) {
+    constexpr int E = 16 / (int)sizeof(typename Elem<DT>::T);
+    const int vecs = a.seglen / E;
+    const unsigned units = (unsigned)(a.rows * a.segments);
+    const size_t lds = (size_t)((a.seglen + 31) / 32) * 4;
+    if (vecs <= 64) distill_rows_kernel<DT, 64, 1, MODE><<<(units + 3) / 4, 256, 4 * lds, stream>>>(a);
+    else if (vecs <= 256) distill_rows_kernel<DT, 64, 4, MODE><<<(units + 3) / 4, 256, 4 * lds, stream>>>(a);
+    else if (vecs <= 512) distill_rows_kernel<DT, 256, 2, MODE><<<units, 256, lds, stream>>>(a);
+    else if (vecs <= 1024) distill_rows_kernel<DT, 256, 4, MODE><<<units, 256, lds, stream>>>(a);
+    else if (vecs <= 2048) distill_rows_kernel<DT, 512, 4, MODE><<<units, 512, lds, stream>>>(a);
+    else if (vecs <= 4096) distill_rows_kernel<DT, 512, 8, MODE><<<units, 512, lds, stream>>>(a);
+    else if (vecs <= 8192) distill_rows_kernel<DT, 1024, 8, MODE><<<units, 1024, lds, stream>>>(a);
+    else distill_rows_kernel<DT, 1024, 16, MODE><<<units, 1024, lds, stream>>>(a);
+}
+
+// ready: the workspace is as a call with the same arguments but for dz and the upstream gradient has left it
 template <int DT>
-int launch_distill(const DistillArgs& a, hipStream_t stream) {
+int launch_distill(DistillArgs a, bool ready, hipStream_t stream) {
+    constexpr int E = 16 / (int)sizeof(typename Elem<DT>::T);
     if (a.inner > 1) {
         const int tiles = (int)cnm_ceil_div_ll(a.inner, 64);
         const long long blocks = (a.rows / a.inner) * tiles;
         distill_planes_kernel<DT><<<(unsigned)blocks, 256, planes_lds(a.V, a.K), stream>>>(a, tiles);
-    } else {
-        const size_t words = ((size_t)a.V / 32 + 2) * 4;
-        if (a.V <= 1024) distill_rows_kernel<DT, 64><<<(unsigned)cnm_ceil_div_ll(a.rows, 4), 256, 4 * words, stream>>>(a);
-        else if (a.V <= 8192) distill_rows_kernel<DT, 256><<<(unsigned)a.rows, 256, words, stream>>>(a);
-        else distill_rows_kernel<DT, 1024><<<(unsigned)a.rows, 1024, words, stream>>>(a);
+        CNM_LAUNCH_CHECK();
+        return CNM_OK;
     }
-    CNM_LAUNCH_CHECK();
+    a.seglen = cnm_ceil_div(cnm_ceil_div(a.V, a.segments), E) * E;
+    const int cut = a.segments > 1;
+    a.segments = cnm_ceil_div(a.V, a.seglen);
+    if (!cut) {
+        launch_rows<DT, ROW>(a, stream);
+        CNM_LAUNCH_CHECK();
+        return CNM_OK;
+    }
+    if (!ready) {
+        launch_rows<DT, SEG_STATS>(a, stream);
+        CNM_LAUNCH_CHECK();
+        distill_join_kernel<DT><<<(unsigned)a.rows, 256, 0, stream>>>(a);
+        CNM_LAUNCH_CHECK();
+    }
+    if (a.dz) {
+        launch_rows<DT, SEG_GRAD>(a, stream);
+        CNM_LAUNCH_CHECK();
+    }
     return CNM_OK;
 }
 
@@ -528,15 +692,14 @@ __device__ inline void group_sync() {
 
 // the K-th largest of N numbers per thread (item(i), all distinct but for 0, at least K of them not 0): radix selection, eight bits a round,
 // until a digit's numbers all belong
-template <int NT, int N, class F>
-__device__ inline u64 kth_largest(F item, int K, int t, TopShared& sh) {
+template <int NT, class F>
+__device__ __noinline__ u64 kth_largest(F item, int N, int K, int t, TopShared& sh) {
     u64 prefix = 0;
     unsigned left = (unsigned)K;
     for (int shift = 56;; shift -= 8) {
         group_sync<NT>();
         for (int i = t; i < 256; i += NT) sh.hist[i] = 0u;
         group_sync<NT>();
-#pragma unroll
         for (int i = 0; i < N; ++i) {
             const u64 k = item(i);
             if (k && (shift == 56 || (k ^ prefix) >> (shift + 8) == 0)) atomicAdd(&sh.hist[(unsigned)(k >> shift) & 255u], 1u);
@@ -562,26 +725,20 @@ __device__ inline u64 kth_largest(F item, int K, int t, TopShared& sh) {
 }
 
 // Of N numbers per thread the K largest, in order, to emit(place, number).  `low`: a lower bound of the K-th largest that keeps the candidates
-// few in the ordinary case; where more than CAND pass it (many equal logits), the K-th largest is selected exactly.  may(i): item(i) >= low,
-// cheaply.
-template <int NT, int N, class M, class F, class O>
-__device__ inline void take_largest(M may, F item, int K, int t, TopShared& sh, O emit) {
+// few in the ordinary case; where more than CAND pass it (many equal logits), the K-th largest is selected exactly.  pass(put): calls put(number)
+// for the thread's numbers that are not below the bound; item(i), i < N: the thread's numbers again, from memory.
+template <int NT, class P, class F, class O>
+__device__ inline void take_largest(P pass, F item, int N, int K, int t, TopShared& sh, O emit) {
     if (t == 0) sh.sel[3] = 0u;
     group_sync<NT>();
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (may(i)) {
-            const u64 k = item(i);
-            if (k) { const unsigned at = atomicAdd(&sh.sel[3], 1u); if (at < CAND) sh.cand[at] = k; }
-        }
+    pass([&](u64 k) { const unsigned at = atomicAdd(&sh.sel[3], 1u); if (at < CAND) sh.cand[at] = k; });
     group_sync<NT>();
     int C = (int)sh.sel[3];
     if (C > CAND) {
-        const u64 least = kth_largest<NT, N>(item, K, t, sh);
+        const u64 least = kth_largest<NT>(item, N, K, t, sh);
         group_sync<NT>();
         if (t == 0) sh.sel[3] = 0u;
         group_sync<NT>();
-#pragma unroll
         for (int i = 0; i < N; ++i) { const u64 k = item(i); if (k && k >= least) sh.cand[atomicAdd(&sh.sel[3], 1u)] = k; }   // exactly K
         group_sync<NT>();
         C = K;
@@ -606,13 +763,20 @@ __device__ inline float kth_bound(float m, int K, float* sh) {
     const int r = (K + W - 1) / W;
     const float ninf = -__builtin_huge_valf();
     if (r > 64) return ninf;
-    float w = ninf;
-    for (int i = 0; i < r; ++i) {
-        w = wave_max(m);
-        const u64 who = __ballot(m == w);
-        if (who == 0) return ninf;                                       // (not reached: the maximum is some lane's)
-        if ((int)(threadIdx.x & 63) == __ffsll((unsigned long long)who) - 1) m = ninf;
+    const int lane = threadIdx.x & 63;
+    // the wave's numbers in order (bitonic, descending: 21 exchanges), or for the first of them six exchanges
+    if (r == 1) m = wave_max(m);
+    else {
+#pragma unroll
+        for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+            for (int d = size >> 1; d; d >>= 1) {
+                const float other = __shfl_xor(m, d);
+                const bool upper = (lane & d) == 0, down = (lane & size) == 0;   // the lane that keeps the larger one
+                m = upper == down ? fmaxf(m, other) : fminf(m, other);
+            }
     }
+    float w = __shfl(m, r - 1);
     if (NT == 64) return w;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = w;
@@ -637,52 +801,55 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void top_rows_kernel(const Top
     const int seg = (int)(unit - r * a.segments), v0 = seg * a.seglen, n = min(a.V - v0, a.seglen);
     const T* z = static_cast<const T*>(a.z) + (size_t)r * a.ldz + v0;
     const float c = (float)(LOG2E_D / (double)a.T), ninf = -__builtin_huge_valf();
-    typedef T TV __attribute__((ext_vector_type(E)));
-    TV x[NV];
+    Raw<DT> x[NV];
     float m = ninf;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int at = (i * NT + t) * E;
-        if (at + E <= n) __builtin_memcpy(&x[i], z + at, 16);            // (whatever the row's alignment)
-        else {
-#pragma unroll
-            for (int j = 0; j < E; ++j) x[i][j] = at + j < n ? z[at + j] : (T)ninf;
-        }
-    }
+    for (int i = 0; i < NV; ++i) x[i].load(z, (i * NT + t) * E, n);
     float vm[NV];                                                        // the vectors' largest
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        vm[i] = (float)x[i][0];
+        x[i].hold();
+        vm[i] = x[i].get(0);
 #pragma unroll
-        for (int j = 1; j < E; ++j) vm[i] = fmaxf(vm[i], (float)x[i][j]);
+        for (int j = 1; j < E; ++j) vm[i] = fmaxf(vm[i], x[i].get(j));
         m = fmaxf(m, vm[i]);
     }
-    Lse l;
-    const float o = m == ninf || m != m ? 0.f : m;
-    l.o = m == m ? m : ninf; l.s = 0.f;
+    const float o = m == ninf ? 0.f : m;
+    Lse l = {m, 0.f};
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+        x[i].hold();
 #pragma unroll
-        for (int j = 0; j < E; ++j) l.s += exp2_(((float)x[i][j] - o) * c);
-    const bool odd = l.s != l.s || m != m;                               // a NaN or +inf here: every vector is looked at
+        for (int j = 0; j < E; ++j) l.s += exp2_((x[i].get(j) - o) * c);
+    }
+    const bool odd = l.s != l.s;                                         // a NaN or +inf here: every vector is looked at
     l = lse_block<NT>(l, c, sh.shf);
-    const float low = kth_bound<NT>(m == m ? m : ninf, a.K, sh.shf);
+    const float low = kth_bound<NT>(m, a.K, sh.shf);
     if (a.segments == 1) { if (t == 0) a.lse[r] = lse_value(l, a.T); }
     else if (t == 0) { a.lpart[2 * unit] = l.o; a.lpart[2 * unit + 1] = l.s; }
-    const auto item = [&](int i) -> u64 {
-        const int at = (i / E * NT + t) * E + i % E;
-        return at < n ? rank_of((float)x[i / E][i % E], (unsigned)(v0 + at)) : 0ull;
+    const auto pass = [&](auto put) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (odd || vm[i] >= low) {
+                x[i].hold();
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    const float y = x[i].get(j);
+                    const int at = (i * NT + t) * E + j;
+                    if (!(y < low) && at < n) put(rank_of(y, (unsigned)(v0 + at)));
+                }
+            }
     };
-    const auto may = [&](int i) { return (odd || vm[i / E] >= low) && !((float)x[i / E][i % E] < low); };
-    const int K = min(a.K, n);
+    const auto item = [=](int i) -> u64 { const int at = i * NT + t; return at < n ? rank_of((float)z[at], (unsigned)(v0 + at)) : 0ull; };
+    const int K = min(a.K, n), N = (n + NT - 1) / NT;
     if (a.segments == 1)
-        take_largest<NT, NV * E>(may, item, K, t, sh, [&](int place, u64 k) {
+        take_largest<NT>(pass, item, N, K, t, sh, [&](int place, u64 k) {
             const unsigned v = ~(unsigned)k;
             a.idx[(size_t)r * a.K + place] = (int)v;
             static_cast<T*>(a.val)[(size_t)r * a.K + place] = z[v];
         });
     else {
-        take_largest<NT, NV * E>(may, item, K, t, sh, [&](int place, u64 k) { a.part[(size_t)unit * a.K + place] = k; });
+        take_largest<NT>(pass, item, N, K, t, sh, [&](int place, u64 k) { a.part[(size_t)unit * a.K + place] = k; });
         for (int i = K + t; i < a.K; i += NT) a.part[(size_t)unit * a.K + i] = 0ull;
     }
 }
@@ -715,7 +882,11 @@ __global__ __launch_bounds__(1024) void top_join_kernel(const TopArgs a) {
     if (t == 0) a.lse[r] = lse_value(l, a.T);
     const float low = kth_bound<1024>(m, a.K, sh.shf);
     const T* z = static_cast<const T*>(a.z) + (size_t)r * a.ldz;
-    take_largest<1024, N>([&](int i) { return k[i] && !(value(k[i]) < low); }, [&](int i) { return k[i]; }, a.K, t, sh, [&](int place, u64 q) {
+    const u64* const part = a.part + (size_t)r * total;
+    take_largest<1024>([&](auto put) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) if (k[i] && !(value(k[i]) < low)) put(k[i]);
+    }, [=](int i) -> u64 { return i * 1024 + t < total ? part[i * 1024 + t] : 0ull; }, (total + 1023) / 1024, a.K, t, sh, [&](int place, u64 q) {
         const unsigned v = ~(unsigned)q;
         a.idx[(size_t)r * a.K + place] = (int)v;
         static_cast<T*>(a.val)[(size_t)r * a.K + place] = z[v];
@@ -858,39 +1029,47 @@ extern "C" int cnm_top_logits(const void* z, int dtype, long long ldz, float tem
     return CNM_ERR_BAD_ARG;
 }
 
-extern "C" size_t cnm_distill_workspace_doubles(long long rows, long long inner) {
-    if (rows <= 0 || inner <= 0 || rows % inner) return 0;
-    return (size_t)WPARTS + (inner > 1 ? (size_t)(rows / inner) * (size_t)cnm_ceil_div_ll(inner, 64) : (size_t)rows);
+// workspace: the weights' partial sums, the losses', and for rows cut into segments the rows' numbers and the segments'
+extern "C" size_t cnm_distill_workspace_doubles(int dtype, long long rows, int classes, long long inner) {
+    if (rows <= 0 || classes <= 0 || inner <= 0 || rows % inner || dtype < CNM_F32 || dtype > CNM_BF16) return 0;
+    if (inner > 1) return (size_t)WPARTS + (size_t)(rows / inner) * (size_t)cnm_ceil_div_ll(inner, 64);
+    const int seg = distill_segments(rows, classes, dtype == CNM_F32 ? 4 : 2);
+    return (size_t)WPARTS + (size_t)rows + (seg > 1 ? (size_t)rows * (sizeof(DistillRow) / sizeof(double) + (size_t)seg) : 0);
 }
 
 extern "C" int cnm_distill(const void* z, int dtype, long long ldz, const void* indices, int wide_indices, const void* entry_logits, int entry_dtype,
                            const float* teacher_lse, float temperature, const float* weight, const float* grad_out, int grad_out_rows, int skip_if_one,
-                           int reduction, float* loss, void* dz, double* workspace, size_t workspace_doubles,
+                           int reduction, float* loss, void* dz, double* workspace, size_t workspace_doubles, int workspace_ready,
                            long long rows, int classes, int entries, long long inner, void* stream) {
     CNM_REQUIRE(z && indices && entry_logits && rows > 0 && classes > 0 && entries > 0 && inner > 0 && (loss || dz), CNM_ERR_BAD_ARG);
     CNM_REQUIRE(temperature > 0.f && temperature < __builtin_huge_valf() && reduction >= 0 && reduction <= 2 && entries <= KMAX, CNM_ERR_BAD_ARG);
-    CNM_REQUIRE(rows % inner == 0 && (inner > 1 || ldz >= classes) && entry_dtype >= CNM_F32 && entry_dtype <= CNM_BF16, CNM_ERR_BAD_ARG);
+    CNM_REQUIRE(rows % inner == 0 && (inner > 1 || ldz >= classes) && dtype >= CNM_F32 && dtype <= CNM_BF16 && entry_dtype >= CNM_F32 && entry_dtype <= CNM_BF16, CNM_ERR_BAD_ARG);
     CNM_REQUIRE(!grad_out_rows || (grad_out && reduction == 0), CNM_ERR_BAD_ARG);
+    CNM_REQUIRE(!workspace_ready || !loss, CNM_ERR_BAD_ARG);
     CNM_REQUIRE(rows < (1ll << 31) && classes <= VMAX && (inner == 1 || cnm_distill_planes_ok(classes, entries)), CNM_ERR_BAD_SHAPE);
-    CNM_REQUIRE(reduction == 0 || (workspace && workspace_doubles >= cnm_distill_workspace_doubles(rows, inner)), CNM_ERR_WORKSPACE);
+    const int seg = inner > 1 ? 1 : distill_segments(rows, classes, dtype == CNM_F32 ? 4 : 2);
+    CNM_REQUIRE(rows * seg < (1ll << 31), CNM_ERR_BAD_SHAPE);
+    CNM_REQUIRE(workspace && workspace_doubles >= cnm_distill_workspace_doubles(dtype, rows, classes, inner), CNM_ERR_WORKSPACE);
     const hipStream_t st = cnm_stream(stream);
     const bool mean = reduction == 1;
     double* const wpart = workspace;
-    double* const lpart = workspace ? workspace + WPARTS : nullptr;
+    double* const lpart = workspace + WPARTS;
+    const long long parts = inner > 1 ? (rows / inner) * cnm_ceil_div_ll(inner, 64) : rows;
+    DistillRow* const rec = seg > 1 ? reinterpret_cast<DistillRow*>(lpart + parts) : nullptr;
+    float* const segs = seg > 1 ? reinterpret_cast<float*>(rec + rows) : nullptr;
     const int nw = mean && weight ? (int)(cnm_ceil_div_ll(rows, 4096) < WPARTS ? cnm_ceil_div_ll(rows, 4096) : WPARTS) : 0;
-    if (nw) { weight_parts_kernel<<<nw, 1024, 0, st>>>(weight, rows, wpart); CNM_LAUNCH_CHECK(); }
+    if (nw && !workspace_ready) { weight_parts_kernel<<<nw, 1024, 0, st>>>(weight, rows, wpart); CNM_LAUNCH_CHECK(); }
     const double inv_norm = mean && !weight ? 1.0 / (double)rows : 1.0;
     const bool total = reduction != 0 && loss;
     const DistillArgs a = {z, ldz, indices, wide_indices, entry_logits, entry_dtype, teacher_lse, temperature, weight, nw ? wpart : nullptr, nw, inv_norm,
-                           grad_out, grad_out_rows, skip_if_one, total ? nullptr : loss, total ? lpart : nullptr, dz, rows, classes, entries, inner};
+                           grad_out, grad_out_rows, skip_if_one, total ? nullptr : loss, total ? lpart : nullptr, dz, rows, classes, entries, inner, rec, segs, seg, 0};
     int rc = CNM_ERR_BAD_ARG;
     switch (dtype) {
-        case CNM_F32: rc = launch_distill<CNM_F32>(a, st); break;
-        case CNM_F16: rc = launch_distill<CNM_F16>(a, st); break;
-        case CNM_BF16: rc = launch_distill<CNM_BF16>(a, st); break;
+        case CNM_F32: rc = launch_distill<CNM_F32>(a, workspace_ready != 0, st); break;
+        case CNM_F16: rc = launch_distill<CNM_F16>(a, workspace_ready != 0, st); break;
+        case CNM_BF16: rc = launch_distill<CNM_BF16>(a, workspace_ready != 0, st); break;
     }
     if (rc != CNM_OK || !total) return rc;
-    const long long parts = inner > 1 ? (rows / inner) * cnm_ceil_div_ll(inner, 64) : rows;
     loss_total_kernel<<<1, 1024, 0, st>>>(lpart, parts, nw ? wpart : nullptr, nw, inv_norm, loss);
     CNM_LAUNCH_CHECK();
     return CNM_OK;

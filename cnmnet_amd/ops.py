@@ -986,18 +986,21 @@ class DistillCall:
     def new_grad(self):
         return torch.empty(self.c.sized(self.c.V), device=self.dev, dtype=self.dtype)
 
-    def run(self, need_loss, dz, grad_out=None, skip_if_one=False):
-        """Launches; returns the loss (or None).  dz: a new_grad() buffer to fill, or None."""
+    def run(self, need_loss, dz, grad_out=None, skip_if_one=False, ready=None):
+        """Launches; returns the loss (or None).  dz: a new_grad() buffer to fill, or None.  self.ws: the workspace, which a later call for the
+        gradient alone may pass on as `ready`."""
         c = self.c
         loss = torch.empty(c.row_shape if self.reduction == 0 else (), device=self.dev, dtype=torch.float32) if need_loss else None
+        self.ws = ready
         if c.rows == 0:
             return loss.zero_() if need_loss else None
-        n = self.lib.cnm_distill_workspace_doubles(c.rows, c.inner) if self.reduction else 0
-        ws = torch.empty(n, device=self.dev, dtype=torch.float64) if n else None
+        n = self.lib.cnm_distill_workspace_doubles(DTYPES[self.dtype], c.rows, c.V, c.inner)
+        if ready is None:
+            self.ws = torch.empty(n, device=self.dev, dtype=torch.float64)
         with _on(self.dev):
             _lib.check(self.lib.cnm_distill(_p(c.z), DTYPES[self.dtype], c.ld, _p(self.idx), int(self.idx.dtype == torch.int64), _p(self.val), DTYPES[self.val.dtype],
                                             _p(self.lse), self.T, _p(self.weight), _p(grad_out), int(grad_out is not None and self.reduction == 0), int(skip_if_one),
-                                            self.reduction, _p(loss), _p(dz), _p(ws), n, c.rows, c.V, self.K, c.inner, _raw_stream(self.dev)))
+                                            self.reduction, _p(loss), _p(dz), _p(self.ws), n, int(ready is not None), c.rows, c.V, self.K, c.inner, _raw_stream(self.dev)))
         return loss
 
 

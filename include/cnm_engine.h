@@ -905,12 +905,13 @@ int cnm_distill_planes_ok(int classes, int entries);
  * reduction 0: loss [rows]; 1: loss [1] = sum weight loss / sum weight (0 if the weights sum to 0); 2: loss [1] = sum weight loss.
  * weight [rows] or NULL (1).  dz (dense, z's dtype) = the gradient of what `loss` is (reduction 0: of sum weight loss), times grad_out[0], or
  * grad_out[row] with grad_out_rows (reduction 0 only), or 1 (NULL).  skip_if_one: if grad_out[0] == 1 the launch leaves dz as it is.
- * loss or dz may be NULL, not both.  workspace: cnm_distill_workspace_doubles(rows, inner) doubles, needed for reduction 1 and 2, contents
- * irrelevant.  Every sum has a fixed order: results repeat bit by bit. */
-size_t cnm_distill_workspace_doubles(long long rows, long long inner);
+ * loss or dz may be NULL, not both.  workspace: cnm_distill_workspace_doubles doubles, contents irrelevant; with workspace_ready (loss NULL) it
+ * is as an earlier call with the same arguments but for loss, dz and grad_out has left it.  Every sum has a fixed order: results repeat bit
+ * by bit. */
+size_t cnm_distill_workspace_doubles(int dtype, long long rows, int classes, long long inner);
 int cnm_distill(const void* z, int dtype, long long ldz, const void* indices, int wide_indices, const void* entry_logits, int entry_dtype,
                 const float* teacher_lse, float temperature, const float* weight, const float* grad_out, int grad_out_rows, int skip_if_one,
-                int reduction, float* loss, void* dz, double* workspace, size_t workspace_doubles,
+                int reduction, float* loss, void* dz, double* workspace, size_t workspace_doubles, int workspace_ready,
                 long long rows, int classes, int entries, long long inner, void* stream);
 
 #ifdef __cplusplus

@@ -80,9 +80,9 @@ def test_top_and_distill_entries_refuse():
     need = lib.cnm_top_logits_workspace_bytes(0, 2, 100000, 8, 1)          # two long rows: split
     assert need > 0 and lib.cnm_top_logits_workspace_bytes(0, 4, 100, 8, 1) == 0
     assert t(_9=2, _10=100000, _2=100000) == -5 and t(_9=2, _10=100000, _2=100000, _7=64, _8=need - 1) == -5
-    n = lib.cnm_distill_workspace_doubles(4, 1)
-    assert n >= 4 and lib.cnm_distill_workspace_doubles(5, 2) == 0
-    dis = [64, 0, 100, 64, 0, 64, 0, None, 1.0, None, None, 0, 0, 1, 64, None, 64, n, 4, 100, 8, 1, 0]
+    n = lib.cnm_distill_workspace_doubles(0, 4, 100, 1)
+    assert n >= 4 and lib.cnm_distill_workspace_doubles(0, 5, 100, 2) == 0 and lib.cnm_distill_workspace_doubles(0, 4, 100000, 1) > n
+    dis = [64, 0, 100, 64, 0, 64, 0, None, 1.0, None, None, 0, 0, 1, 64, None, 64, n, 0, 4, 100, 8, 1, 0]
     def d(**kw):
         a = list(dis)
         for k, v in kw.items():
@@ -91,13 +91,14 @@ def test_top_and_distill_entries_refuse():
     for i in (0, 3, 5):
         assert d(**{"_%d" % i: 0}) == -1
     assert d(_14=0) == -1                                               # nothing to compute
-    assert d(_8=-1.0) == -1 and d(_13=3) == -1 and d(_20=257) == -1 and d(_20=0) == -1
+    assert d(_8=-1.0) == -1 and d(_13=3) == -1 and d(_21=257) == -1 and d(_21=0) == -1
     assert d(_2=99) == -1 and d(_6=4) == -1 and d(_1=-1) == -1
     assert d(_11=1) == -1                                               # per-row upstream gradient without one / with a reduction
     assert d(_10=64, _11=1) == -1
     assert d(_16=0) == -5 and d(_17=n - 1) == -5
-    assert d(_19=(1 << 20) + 1, _2=1 << 21) == -2
-    assert d(_21=2, _19=100000) == -2                                   # planes that do not fit LDS
+    assert d(_20=(1 << 20) + 1, _2=1 << 21) == -2
+    assert d(_18=1) == -1                                               # a loss needs its own pass
+    assert d(_22=2, _20=100000) == -2                                   # planes that do not fit LDS
     assert lib.cnm_distill_planes_ok(64, 8) == 1 and lib.cnm_distill_planes_ok(100000, 8) == 0 and lib.cnm_distill_planes_ok(64, 0) == 0
 
 

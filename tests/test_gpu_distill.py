@@ -227,6 +227,10 @@ def test_distill_masked_classes():
     z = torch.where(keep, z, -inf)
     loss, dz = check_distill(z, idx, val, lse, w, 1.0, "mean")
     assert bool(torch.isfinite(loss)) and bool((dz.cpu()[~keep] == 0).all())
+    loss, dz = check_distill(z - 300.0, idx, val, lse, w, 1.0, "mean")   # far from zero as well
+    assert bool(torch.isfinite(loss)) and bool((dz.cpu()[~keep] == 0).all())
+    view = ((lambda t, c: t.view(1, 4, -1).permute(0, 2, 1).contiguous() if c else t.view(1, 4)), (lambda t: t.permute(0, 2, 1).reshape(4, 30)))
+    check_distill(z - 300.0, idx, val, lse, w, 1.0, "mean", view=view, dim=1)
 
 
 def test_distill_rows_that_count_for_nothing():
