@@ -71,18 +71,6 @@ __device__ inline double sum_block(double a, double* sh) {
     for (int d = 32; d; d >>= 1) a += __shfl_xor(a, d);
     return a;
 }
-template <int NT>
-__device__ inline double max_block(double a, double* sh) {
-    for (int d = 32; d; d >>= 1) a = fmax(a, __shfl_xor(a, d));
-    if (NT == 64) return a;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
-    __syncthreads();
-    a = (threadIdx.x & 63) < NT / 64 ? sh[threadIdx.x & 63] : -__builtin_huge_val();
-    for (int d = 32; d; d >>= 1) a = fmax(a, __shfl_xor(a, d));
-    return a;
-}
-
 // sixteen bytes of a row as they are in memory, elements beyond the row -inf.  hold(): conversions done so far are forgotten (left alone, hipcc
 // keeps every converted element in a register of its own from one pass over the row to the next)
 template <int DT>
@@ -162,13 +150,13 @@ __device__ inline float exp2_of(double x) {
     return ldexpf(exp2_((float)(x - n)), (int)n);
 }
 
-// The entries of a row, shared by the NT threads that work on it.
+// The entries of a row, shared by the threads that work on it.
 struct Entries {
-    double shd[16];
-    float shf[32];
     int idx[KMAX];                                                       // -1: none
     float z[KMAX], p[KMAX];                                              // the student's logit there; the teacher's logit, then the probability
     int dup;                                                             // some class is named twice
+    Lse rest[16];                                                        // the waves' statistics of the unnamed classes
+    DistillRow row;
 };
 template <int NT>
 __device__ inline void row_sync() {
@@ -178,7 +166,6 @@ __device__ inline void row_sync() {
 
 template <int DT, int NT>
 __device__ inline void load_entries(const DistillArgs& a, size_t r, const typename Elem<DT>::T* z, Entries& e, int t) {
-    if (t == 0) e.dup = 0;
     for (int k = t; k < a.K; k += NT) {
         const long long i = load_index(a.idx, a.wide, r * a.K + k);
         const bool ok = i >= 0 && i < a.V;
@@ -186,120 +173,122 @@ __device__ inline void load_entries(const DistillArgs& a, size_t r, const typena
         e.p[k] = ok ? load_any(a.val, a.vdt, r * a.K + k) : 0.f;
         e.z[k] = ok ? (float)z[i] : 0.f;
     }
-    row_sync<NT>();
 }
-// the named classes' bits among the n from v0 on; whether a class is named twice
+// the named classes' bits among the n from v0 on; a bit that is there already: a class named twice
 template <int NT>
 __device__ inline void mark_entries(Entries& e, int K, unsigned* bits, int v0, int n, int t) {
     for (int k = t; k < K; k += NT) {
         const int i = e.idx[k] - v0;
-        if (i >= 0 && i < n && e.idx[k] >= 0) atomicOr(&bits[i >> 5], 1u << (i & 31));
+        if (e.idx[k] >= 0 && i >= 0 && i < n && (atomicOr(&bits[i >> 5], 1u << (i & 31)) >> (i & 31) & 1u)) e.dup = 1;
     }
-    for (int q = t; q < K * K; q += NT) {
-        const int k = q / K, j = q - k * K;
-        if (j < k && e.idx[k] >= 0 && e.idx[j] == e.idx[k]) e.dup = 1;
-    }
-    row_sync<NT>();
 }
-template <int NT>
-__device__ inline double teacher_lse(const DistillArgs& a, size_t r, Entries& e, int t) {
-    if (a.lse) return (double)a.lse[r];
-    double best = -__builtin_huge_val(), s = 0.0;
-    for (int k = t; k < a.K; k += NT) if (e.idx[k] >= 0) best = fmax(best, (double)e.p[k]);
-    best = max_block<NT>(best, e.shd);
-    if (best == -__builtin_huge_val()) best = 0.0;
-    for (int k = t; k < a.K; k += NT) if (e.idx[k] >= 0) s += (double)exp2_of(((double)e.p[k] - best) * (LOG2E_D / (double)a.T));
-    s = sum_block<NT>(s, e.shd);
-    return best / (double)a.T + log(s);
-}
-__device__ inline double entry_log2p(const DistillArgs& a, const Entries& e, int k, double L) { return ((double)e.p[k] / (double)a.T - L) * LOG2E_D; }
+__device__ inline double entry_log2p(const DistillArgs& a, float logit, double L) { return ((double)logit / (double)a.T - L) * LOG2E_D; }
 
-// a class that is named more than once: its first entry gets the sum, the others become none
-template <int NT>
-__device__ inline void join_entries(Entries& e, int K, int t) {
+// a class that is named more than once: its first entry gets the sum, the others become none (one wave)
+__device__ inline void join_entries(Entries& e, int K, int lane) {
     if (!e.dup) return;
     float s[KMAX / 64];
     bool first[KMAX / 64];
 #pragma unroll
-    for (int q = 0; q < (KMAX + NT - 1) / NT; ++q) {
-        const int k = q * NT + t;
+    for (int q = 0; q < KMAX / 64; ++q) {
+        const int k = q * 64 + lane;
         first[q] = k < K && e.idx[k] >= 0; s[q] = 0.f;
         if (first[q])
             for (int j = 0; j < K; ++j) if (e.idx[j] == e.idx[k]) { if (j < k) first[q] = false; s[q] += e.p[j]; }
     }
-    row_sync<NT>();
+    row_sync<64>();
 #pragma unroll
-    for (int q = 0; q < (KMAX + NT - 1) / NT; ++q) {
-        const int k = q * NT + t;
+    for (int q = 0; q < KMAX / 64; ++q) {
+        const int k = q * 64 + lane;
         if (k < K) { e.p[k] = s[q]; if (!first[q]) e.idx[k] = -1; }
     }
-    row_sync<NT>();
+    row_sync<64>();
 }
 
-// From the unnamed classes' statistics to the loss and the gradient's coefficients (for an upstream gradient of 1); e.p becomes the probabilities.
-template <int NT>
-__device__ inline DistillRow finish_row(const DistillArgs& a, size_t r, bool live, Lse rest, Entries& e, float c, int t) {
+// A row's numbers, by one wave while the others go over the classes: the fp64 logarithms are hundreds of instructions, too many for every wave.
+// First what the entries alone say (e.p becomes the probabilities), then, with the unnamed classes' statistics, the loss and the gradient's
+// coefficients for an upstream gradient of 1.
+struct Teacher { double L, P, lp; Lse named; int have; };                // lp: sum p log2 p
+__device__ inline double sum_wave(double a) { for (int d = 32; d; d >>= 1) a += __shfl_xor(a, d); return a; }
+__device__ inline double max_wave(double a) { for (int d = 32; d; d >>= 1) a = fmax(a, __shfl_xor(a, d)); return a; }
+
+__device__ inline Teacher entry_numbers(const DistillArgs& a, size_t r, Entries& e, float c, int lane) {
     const float ninf = -__builtin_huge_valf();
-    Lse named = {ninf, 0.f};
-    int have = 0;
-    for (int k = t; k < a.K; k += NT) {
+    Teacher w;
+    w.named = {ninf, 0.f};
+    double best = -__builtin_huge_val();
+    bool have = false;
+    for (int k = lane; k < a.K; k += 64) {
         const int i = e.idx[k];
         bool first = i >= 0;
-        have |= first;
+        if (first) { have = true; best = fmax(best, (double)e.p[k]); }
         if (e.dup) for (int j = 0; j < k && first; ++j) first = e.idx[j] != i;
         if (first) {
             const float x = e.z[k];
-            named = lse_join(named, Lse{x, x == ninf ? 0.f : x == x ? 1.f : x}, c);
+            w.named = lse_join(w.named, Lse{x, x == ninf ? 0.f : x == x ? 1.f : x}, c);
         }
     }
-    DistillRow w;
-    w.L = teacher_lse<NT>(a, r, e, t);
-    named = lse_block<NT>(named, c, e.shf);
-    const Lse all = lse_join(rest, named, c);
-    w.oall = all.o == ninf ? 0.f : all.o; w.orest = rest.o == ninf ? 0.f : rest.o;
-    const double lq0 = -log2((double)all.s);                             // log2 q_v = (z_v - oall) c + lq0
-    double P = 0.0, Q = 0.0, loss = 0.0;
-    for (int k = t; k < a.K; k += NT) {
+    w.have = __any(have);
+    w.named = lse_wave(w.named, c);
+    if (a.lse) w.L = (double)a.lse[r];
+    else {
+        best = max_wave(best);
+        if (best == -__builtin_huge_val()) best = 0.0;
+        double s = 0.0;
+        for (int k = lane; k < a.K; k += 64) if (e.idx[k] >= 0) s += (double)exp2_of(((double)e.p[k] - best) * (LOG2E_D / (double)a.T));
+        w.L = best / (double)a.T + log(sum_wave(s));
+    }
+    double P = 0.0, lp = 0.0;
+    for (int k = lane; k < a.K; k += 64) {
         float p = 0.f;
         if (e.idx[k] >= 0) {
-            const double lp = entry_log2p(a, e, k, w.L), lq = ((double)e.z[k] - (double)w.oall) * (double)c + lq0;
-            p = exp2_of(lp);
-            if (p > 0.f) loss += (double)p * LN2_D * (lp - lq);
+            const double l = entry_log2p(a, e.p[k], w.L);
+            p = exp2_of(l);
+            if (p > 0.f) lp += (double)p * l;
             P += (double)p;
         }
         e.p[k] = p;
     }
-    if (a.lse) {                                                         // the named classes' probability, each once
-        P = sum_block<NT>(P, e.shd);
-        Q = (double)named.s * (double)exp2_of(((double)named.o - (double)w.oall) * (double)c + lq0);
-        if (named.o == ninf) Q = 0.0;
-    }
-    loss = sum_block<NT>(loss, e.shd);
-    have = (int)max_block<NT>((double)have, e.shd);
+    w.P = sum_wave(P); w.lp = lp;
+    return w;
+}
+__device__ inline DistillRow finish_row(const DistillArgs& a, size_t r, Lse rest, const Teacher& w, Entries& e, float c, int lane) {
+    const float ninf = -__builtin_huge_valf();
+    const Lse all = lse_join(rest, w.named, c);
+    DistillRow row;
+    row.L = w.L;
+    row.oall = all.o == ninf ? 0.f : all.o; row.orest = rest.o == ninf ? 0.f : rest.o;
+    const double lq0 = -log2((double)all.s);                             // log2 q_v = (z_v - oall) c + lq0
+    double loss = w.lp;
+    for (int k = lane; k < a.K; k += 64)
+        if (e.p[k] > 0.f) loss -= (double)e.p[k] * (((double)e.z[k] - (double)row.oall) * (double)c + lq0);
+    loss = sum_wave(loss) * LN2_D;
     double ratio = 0.0;                                                  // p_r / (sum of the unnamed exponentials)
     if (a.lse && rest.s > 0.f) {
-        const double pr = 1.0 - P;
+        const double pr = 1.0 - w.P;
         if (pr > 0.0) {
             // q_r from the smaller side: 1 - Q keeps its digits where the named classes hold little
-            const double lqr = Q < 0.5 ? log1p(-Q) : (((double)w.orest - (double)w.oall) * (double)c + log2((double)rest.s) + lq0) * LN2_D;
-            loss += pr * (log1p(-P) - lqr);
+            const double Q = w.named.o == ninf ? 0.0 : (double)w.named.s * (double)exp2_of(((double)w.named.o - (double)row.oall) * (double)c + lq0);
+            const double lqr = Q < 0.5 ? log1p(-Q) : (((double)row.orest - (double)row.oall) * (double)c + log2((double)rest.s) + lq0) * LN2_D;
+            loss += pr * (log1p(-w.P) - lqr);
             ratio = pr / (double)rest.s;
         }
     }
     loss *= (double)a.T * (double)a.T;
-    if (!have) loss = 0.0;
+    if (!w.have) loss = 0.0;
     const float wrow = a.weight ? a.weight[r] : 1.f;
-    if (t == 0 && live) {
+    if (lane == 0) {
         if (a.loss) a.loss[r] = (float)loss;
         if (a.lpart) a.lpart[r] = wrow != 0.f ? (double)wrow * loss : 0.0;
     }
     double norm = a.inv_norm;
     if (a.wpart) { const double s = wave_total(a.wpart, a.nwpart); norm = s > 0.0 ? a.inv_norm / s : 0.0; }
-    const double scale = have && wrow != 0.f ? (double)a.T * (double)wrow * norm : 0.0;
-    w.inv = 1.f / all.s;
-    w.A = rest.s == 0.f ? 0.f : (float)(scale * ((double)exp2_((w.orest - w.oall) * c) / (double)all.s - ratio));   // (no mass outside the entries: nothing to scale)
-    w.B = (float)scale;
-    return w;
+    const double scale = w.have && wrow != 0.f ? (double)a.T * (double)wrow * norm : 0.0;
+    row.inv = 1.f / all.s;
+    row.A = rest.s == 0.f ? 0.f : (float)(scale * ((double)exp2_((row.orest - row.oall) * c) / (double)all.s - ratio));   // (no mass outside the entries: nothing to scale)
+    row.B = (float)scale;
+    row.pad = 0.f;
+    return row;
 }
 
 // NT threads per row (MODE ROW) or segment of a row, which they hold in registers (NV vectors of 16 bytes each): z is read once, the gradient
@@ -334,12 +323,17 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_rows_kernel(const
 #pragma unroll
     for (int i = 0; i < NV; ++i) x[i].load(z, (i * NT + t) * E, n);
     for (int i = t; i < nw; i += NT) bits[i] = 0u;
+    if (t == 0) e.dup = 0;
     load_entries<DT, NT>(a, r, zrow, e, t);
+    row_sync<NT>();
     mark_entries<NT>(e, a.K, bits, v0, n, t);
+    row_sync<NT>();
+    const int lane = threadIdx.x & 63;
     const auto mask = [&](int i) { const int at = (i * NT + t) * E; return at < n ? bits[at >> 5] >> (at & 31) : 0u; };
-    DistillRow w;
-    if constexpr (MODE != SEG_GRAD) {                                    // statistics of the unnamed classes
-        float m = ninf;
+    if constexpr (MODE != SEG_GRAD) {
+        Teacher teach;
+        if (MODE == ROW && t < 64) teach = entry_numbers(a, r, e, c, lane);
+        float m = ninf;                                                  // statistics of the unnamed classes
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             x[i].hold();
@@ -356,19 +350,30 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_rows_kernel(const
 #pragma unroll
             for (int j = 0; j < E; ++j) rest.s += b >> j & 1u ? 0.f : exp2_((x[i].get(j) - o) * c);
         }
-        rest = lse_block<NT>(rest, c, e.shf);
+        rest = lse_wave(rest, c);
+        if (NT > 64) {
+            if (lane == 0) e.rest[t >> 6] = rest;
+            __syncthreads();
+            if (t < 64) rest = lse_wave(lane < NT / 64 ? e.rest[lane] : Lse{ninf, 0.f}, c);
+        }
         if constexpr (MODE == SEG_STATS) {
             if (t == 0) { a.seg[2 * unit] = rest.o; a.seg[2 * unit + 1] = rest.s; }
             return;
         }
-        w = finish_row<NT>(a, r, true, rest, e, c, t);
+        if (t < 64) {
+            const DistillRow row = finish_row(a, r, rest, teach, e, c, lane);
+            if (lane == 0) e.row = row;
+        }
     } else {
-        w = a.rec[r];
-        for (int k = t; k < a.K; k += NT) e.p[k] = e.idx[k] >= 0 ? exp2_of(entry_log2p(a, e, k, w.L)) : 0.f;
+        if (t == 0) e.row = a.rec[r];
+        const double L = a.rec[r].L;
+        for (int k = t; k < a.K; k += NT) e.p[k] = e.idx[k] >= 0 ? exp2_of(entry_log2p(a, e.p[k], L)) : 0.f;
+        row_sync<NT>();
     }
     if (!a.dz) return;
+    if (t < 64) join_entries(e, a.K, lane);
     row_sync<NT>();
-    join_entries<NT>(e, a.K, t);
+    const DistillRow w = e.row;
     const float A = w.A * go, B = w.B * go;
     const bool zero = B == 0.f;                                          // rows that count for nothing: zeros, whatever the logits hold
     T* const dz = static_cast<T*>(a.dz) + r * a.V + v0;
@@ -402,36 +407,38 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_rows_kernel(const
 }
 
 template <int DT>
-__global__ __launch_bounds__(256) void distill_join_kernel(const DistillArgs a) {
+__global__ __launch_bounds__(64) void distill_join_kernel(const DistillArgs a) {
     typedef typename Elem<DT>::T T;
     __shared__ Entries e;
     const int t = threadIdx.x;
     if (a.skip_if_one && a.go && a.go[0] == 1.f) return;
     const size_t r = blockIdx.x;
     const float c = (float)(LOG2E_D / (double)a.T);
-    load_entries<DT, 256>(a, r, static_cast<const T*>(a.z) + r * a.ldz, e, t);
-    mark_entries<256>(e, a.K, nullptr, 0, 0, t);
+    if (t == 0) e.dup = 1;                                               // (no bits here to tell: looked up)
+    load_entries<DT, 64>(a, r, static_cast<const T*>(a.z) + r * a.ldz, e, t);
+    row_sync<64>();
+    const Teacher teach = entry_numbers(a, r, e, c, t);
     Lse rest = {-__builtin_huge_valf(), 0.f};
-    if (t < a.segments) rest = {a.seg[2 * (r * a.segments + t)], a.seg[2 * (r * a.segments + t) + 1]};
-    rest = lse_block<256>(rest, c, e.shf);
-    const DistillRow w = finish_row<256>(a, r, true, rest, e, c, t);
-    if (t == 0) a.rec[r] = w;
+    for (int i = t; i < a.segments; i += 64) rest = lse_join(rest, Lse{a.seg[2 * (r * a.segments + i)], a.seg[2 * (r * a.segments + i) + 1]}, c);
+    const DistillRow row = finish_row(a, r, lse_wave(rest, c), teach, e, c, t);
+    if (t == 0) a.rec[r] = row;
 }
 
-// The same with the classes in the middle: [outer][V][inner], a workgroup takes 64 neighbouring positions ("pixels"), one per lane; its four
-// waves share the classes and the entries.  The tile is read once, into LDS, and the gradient leaves from there: the entries' threads correct
-// the named classes in place.  LDS: 64 floats per class, one bit per class and pixel, the entries.
+// The same with the classes in the middle: [outer][V][inner], a workgroup takes 64 neighbouring positions ("pixels"), one per lane.  The tile is
+// read once, into LDS, and the gradient leaves from there.  Wave 0 takes the named classes out of the tile (-inf in their place) and works out
+// the pixels' numbers -- it alone, for its fp64 logarithms --, the other three share the statistics of the rest; the gradient is everybody's.
+// LDS: 64 floats per class, one bit per class and pixel, the entries.
 template <int DT>
 __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a, int tiles) {
     typedef typename Elem<DT>::T T;
     extern __shared__ unsigned lds_words[];
     const int V = a.V, K = a.K, nw = (V + 31) / 32;
-    float* tile = reinterpret_cast<float*>(lds_words);                   // [V][64]
-    unsigned* bits = lds_words + V * 64;                                 // [nw][64]
-    int* eidx = reinterpret_cast<int*>(bits + nw * 64);                  // [K][64]
-    float* ep = reinterpret_cast<float*>(eidx + K * 64);                 // [K][64]: the entry's logit, then its p
-    double* shd = reinterpret_cast<double*>(ep + K * 64);                // [4][64]
-    double* shd2 = shd + 256;                                            // [4][64]
+    float* const tile = reinterpret_cast<float*>(lds_words);             // [V][64]
+    unsigned* const bits = lds_words + V * 64;                           // [nw][64]
+    int* const eidx = reinterpret_cast<int*>(bits + nw * 64);            // [K][64]: -1: none, or named by an earlier entry (then that class is -2 - eidx)
+    float* const ep = reinterpret_cast<float*>(eidx + K * 64);           // [K][64]: the entry's logit, then its p
+    float* const ez = ep + K * 64;                                       // [K][64]: the student's logit there
+    float* const sh = ez + K * 64;                                       // [3][64][2]: the waves' statistics; then [4][64]: the pixels' numbers
     float go = 1.f;
     if (a.go && !a.go_rows) {
         go = a.go[0];
@@ -442,136 +449,138 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
     const long long p0 = (long long)(blockIdx.x % tiles) * 64;
     const bool live = p0 + px < a.inner;
     const size_t at = live ? p0 + px : 0;                                // position in a plane
-    const T* z = static_cast<const T*>(a.z) + (size_t)ob * V * a.inner + at;
+    const T* const z = static_cast<const T*>(a.z) + (size_t)ob * V * a.inner + at;
     const size_t ebase = (size_t)ob * K * a.inner + at, r = (size_t)ob * a.inner + at;
-    double norm = a.inv_norm;
-    if (a.wpart) { const double s = wave_total(a.wpart, a.nwpart); norm = s > 0.0 ? a.inv_norm / s : 0.0; }
-    if (a.go && a.go_rows) go = a.go[r];
-    const float wrow = live ? (a.weight ? a.weight[r] : 1.f) : 0.f;
-    const float c = (float)(LOG2E_D / (double)a.T);
-    const float ninf = -__builtin_huge_valf();
+    const float c = (float)(LOG2E_D / (double)a.T), ninf = -__builtin_huge_valf();
 
     for (int i = w; i < nw; i += 4) bits[i * 64 + px] = 0u;
-    for (int v = w; v < V; v += 4) tile[v * 64 + px] = live ? (float)z[(size_t)v * a.inner] : 0.f;
-    __syncthreads();
     for (int k = w; k < K; k += 4) {
         const long long i = live ? load_index(a.idx, a.wide, ebase + (size_t)k * a.inner) : -1;
         const bool ok = i >= 0 && i < V;
         eidx[k * 64 + px] = ok ? (int)i : -1;
         ep[k * 64 + px] = ok ? load_any(a.val, a.vdt, ebase + (size_t)k * a.inner) : 0.f;
-        if (ok) atomicOr(&bits[(int)(i >> 5) * 64 + px], 1u << (i & 31));
+    }
+#pragma unroll 8
+    for (int v = w; v < V; v += 4) tile[v * 64 + px] = live ? (float)z[(size_t)v * a.inner] : 0.f;
+    __syncthreads();
+    Lse named = {ninf, 0.f};
+    bool have = false, dup = false;
+    if (w == 0) {
+        for (int k = 0; k < K; ++k) {
+            const int i = eidx[k * 64 + px];
+            if (i >= 0) {
+                have = true;
+                unsigned* const b = bits + (i >> 5) * 64 + px;
+                if (*b >> (i & 31) & 1u) {                               // named before: the logit from that entry
+                    dup = true;
+                    for (int j = 0; j < k; ++j) if (eidx[j * 64 + px] == i) ez[k * 64 + px] = ez[j * 64 + px];
+                    eidx[k * 64 + px] = -2 - i;
+                } else {
+                    *b |= 1u << (i & 31);
+                    const float x = tile[i * 64 + px];
+                    ez[k * 64 + px] = x;
+                    tile[i * 64 + px] = ninf;
+                    named = lse_join(named, Lse{x, x == ninf ? 0.f : x == x ? 1.f : x}, c);
+                }
+            }
+        }
     }
     __syncthreads();
-    // statistics: this wave's share of the unnamed classes and of the named ones (each once: its first entry stands for it)
-    Run run;
-    for (int v = w; v < V; v += 4)
-        if (!(bits[(v >> 5) * 64 + px] >> (v & 31) & 1u)) {
-            const float x = tile[v * 64 + px];
-            if (x > run.m) run.raise(x, c);
-            run.s += exp2_((x - run.o) * c);
-        }
-    Lse rest = run.lse(), named = {ninf, 0.f};
-    for (int k = w; k < K; k += 4) {
-        const int i = eidx[k * 64 + px];
-        bool first = i >= 0;
-        for (int j = 0; j < k; ++j) first = first && eidx[j * 64 + px] != i;
-        if (first) {
-            const float x = tile[i * 64 + px];
-            named = lse_join(named, Lse{x, x == ninf ? 0.f : x == x ? 1.f : x}, c);
-        }
-    }
-    float* shf = reinterpret_cast<float*>(shd);
-    float* shf2 = reinterpret_cast<float*>(shd2);
-    shf[w * 64 + px] = rest.o; shf[256 + w * 64 + px] = rest.s;
-    shf2[w * 64 + px] = named.o; shf2[256 + w * 64 + px] = named.s;
-    __syncthreads();
-    rest = Lse{shf[px], shf[256 + px]}; named = Lse{shf2[px], shf2[256 + px]};
-    for (int i = 1; i < 4; ++i) {
-        rest = lse_join(rest, Lse{shf[i * 64 + px], shf[256 + i * 64 + px]}, c);
-        named = lse_join(named, Lse{shf2[i * 64 + px], shf2[256 + i * 64 + px]}, c);
-    }
-    const Lse all = lse_join(rest, named, c);
-    const float oall = all.o == ninf ? 0.f : all.o, orest = rest.o == ninf ? 0.f : rest.o;
-    const double lq0 = -log2((double)all.s);
-    // the teacher's log-sum-exp: given, or over the entries
-    double L;
-    bool have = false;
-    {
-        float best = ninf;
-        for (int k = 0; k < K; ++k) if (eidx[k * 64 + px] >= 0) { have = true; best = fmaxf(best, ep[k * 64 + px]); }
+    double L = 0.0, P = 0.0, loss = 0.0;
+    if (w == 0) {                                                        // what the entries alone say
         if (a.lse) L = (double)a.lse[r];
         else {
+            float best = ninf;
+            for (int k = 0; k < K; ++k) if (eidx[k * 64 + px] != -1) best = fmaxf(best, ep[k * 64 + px]);
             if (best == ninf) best = 0.f;
             double s = 0.0;
-            for (int k = 0; k < K; ++k) if (eidx[k * 64 + px] >= 0) s += (double)exp2_((float)(((double)ep[k * 64 + px] - (double)best) * (LOG2E_D / (double)a.T)));
+            for (int k = 0; k < K; ++k) if (eidx[k * 64 + px] != -1) s += (double)exp2_of(((double)ep[k * 64 + px] - (double)best) * (LOG2E_D / (double)a.T));
             L = (double)best / (double)a.T + log(s);
         }
-    }
-    __syncthreads();                                                     // every wave has read the entries' logits and the partial sums
-    double P = 0.0, loss = 0.0;
-    for (int k = w; k < K; k += 4) {
-        const int i = eidx[k * 64 + px];
-        float p = 0.f;
-        if (i >= 0) {
-            const double lp = ((double)ep[k * 64 + px] / (double)a.T - L) * LOG2E_D;
-            p = exp2_of(lp);
-            if (p > 0.f) loss += (double)p * LN2_D * (lp - (((double)tile[i * 64 + px] - (double)oall) * (double)c + lq0));
-            P += (double)p;
+        for (int k = 0; k < K; ++k) {
+            float p = 0.f;
+            if (eidx[k * 64 + px] != -1) {
+                const double l = entry_log2p(a, ep[k * 64 + px], L);
+                p = exp2_of(l);
+                if (p > 0.f) loss += (double)p * l;
+                P += (double)p;
+            }
+            ep[k * 64 + px] = p;
         }
-        ep[k * 64 + px] = p;
+    } else {
+        float m = ninf, s = 0.f;
+        for (int v = w - 1; v < V; v += 3) m = fmaxf(m, tile[v * 64 + px]);
+        const float o = m == ninf ? 0.f : m;
+        for (int v = w - 1; v < V; v += 3) s += exp2_((tile[v * 64 + px] - o) * c);
+        sh[((w - 1) * 64 + px) * 2] = m; sh[((w - 1) * 64 + px) * 2 + 1] = s;
     }
-    shd[w * 64 + px] = P; shd2[w * 64 + px] = loss;
     __syncthreads();
-    P = (shd[px] + shd[64 + px]) + (shd[128 + px] + shd[192 + px]);
-    loss = (shd2[px] + shd2[64 + px]) + (shd2[128 + px] + shd2[192 + px]);
-    double ratio = 0.0;
-    if (a.lse && rest.s > 0.f) {
-        const double pr = 1.0 - P;
-        if (pr > 0.0) {
-            const double Q = named.o == ninf ? 0.0 : (double)named.s * (double)exp2_of(((double)named.o - (double)oall) * (double)c + lq0);
-            const double lqr = Q < 0.5 ? log1p(-Q) : (((double)orest - (double)oall) * (double)c + log2((double)rest.s) + lq0) * LN2_D;
-            loss += pr * (log1p(-P) - lqr);
-            ratio = pr / (double)rest.s;
-        }
-    }
-    loss *= (double)a.T * (double)a.T;
-    if (!have) loss = 0.0;
     if (w == 0) {
+        Lse rest = {sh[px * 2], sh[px * 2 + 1]};
+        for (int i = 1; i < 3; ++i) rest = lse_join(rest, Lse{sh[(i * 64 + px) * 2], sh[(i * 64 + px) * 2 + 1]}, c);
+        const Lse all = lse_join(rest, named, c);
+        const float oall = all.o == ninf ? 0.f : all.o, orest = rest.o == ninf ? 0.f : rest.o;
+        const double lq0 = -log2((double)all.s);
+        for (int k = 0; k < K; ++k)
+            if (ep[k * 64 + px] > 0.f) loss -= (double)ep[k * 64 + px] * (((double)ez[k * 64 + px] - (double)oall) * (double)c + lq0);
+        loss *= LN2_D;
+        double ratio = 0.0;
+        if (a.lse && rest.s > 0.f) {
+            const double pr = 1.0 - P;
+            if (pr > 0.0) {
+                const double Q = named.o == ninf ? 0.0 : (double)named.s * (double)exp2_of(((double)named.o - (double)oall) * (double)c + lq0);
+                const double lqr = Q < 0.5 ? log1p(-Q) : (((double)orest - (double)oall) * (double)c + log2((double)rest.s) + lq0) * LN2_D;
+                loss += pr * (log1p(-P) - lqr);
+                ratio = pr / (double)rest.s;
+            }
+        }
+        loss *= (double)a.T * (double)a.T;
+        if (!have) loss = 0.0;
+        const float wrow = live ? (a.weight ? a.weight[r] : 1.f) : 0.f;
         if (a.loss && live) a.loss[r] = (float)loss;
         if (a.lpart) {
-            double l = wrow != 0.f ? (double)wrow * loss : 0.0;
-            for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+            const double l = sum_wave(wrow != 0.f ? (double)wrow * loss : 0.0);
             if (px == 0) a.lpart[blockIdx.x] = l;
+        }
+        if (a.dz) {
+            double norm = a.inv_norm;
+            if (a.wpart) { const double s = wave_total(a.wpart, a.nwpart); norm = s > 0.0 ? a.inv_norm / s : 0.0; }
+            if (a.go && a.go_rows) go = a.go[r];
+            const float B = (float)(have && wrow != 0.f ? (double)a.T * (double)go * (double)wrow * norm : 0.0);
+            const float A = rest.s == 0.f ? 0.f : (float)((double)B * ((double)exp2_((orest - oall) * c) / (double)all.s - ratio));
+            const float inv = 1.f / all.s;
+            for (int k = 0; k < K; ++k) {                                // the named classes' gradients into their places
+                const int i = eidx[k * 64 + px];
+                if (i >= 0) {
+                    float p = ep[k * 64 + px];
+                    if (dup) for (int j = k + 1; j < K; ++j) if (eidx[j * 64 + px] == -2 - i) p += ep[j * 64 + px];
+                    tile[i * 64 + px] = B == 0.f ? 0.f : B * (exp2_((ez[k * 64 + px] - oall) * c) * inv - p);
+                }
+            }
+            sh[px] = A; sh[64 + px] = orest; sh[128 + px] = B;
         }
     }
     if (!a.dz) return;
-    const double scale = have && wrow != 0.f ? (double)a.T * (double)go * (double)wrow * norm : 0.0;
-    const bool zero = scale == 0.0;
-    const float inv = 1.f / all.s, A = rest.s == 0.f ? 0.f : (float)(scale * ((double)exp2_((orest - oall) * c) / (double)all.s - ratio)), Bp = (float)scale;
-    for (int v = w; v < V; v += 4) {
-        const float x = tile[v * 64 + px];
-        const bool in = bits[(v >> 5) * 64 + px] >> (v & 31) & 1u;
-        const float e = exp2_((x - (in ? oall : orest)) * c);
-        tile[v * 64 + px] = zero ? 0.f : in ? e * inv : A * e;           // a named class: q, until its first entry has passed
-    }
-    __syncthreads();
-    for (int k = w; k < K; k += 4) {
-        const int i = eidx[k * 64 + px];
-        bool first = i >= 0 && !zero;
-        for (int j = 0; j < k; ++j) first = first && eidx[j * 64 + px] != i;
-        if (first) {
-            float p = ep[k * 64 + px];
-            for (int j = k + 1; j < K; ++j) p += eidx[j * 64 + px] == i ? ep[j * 64 + px] : 0.f;
-            tile[i * 64 + px] = Bp * (tile[i * 64 + px] - p);
-        }
-    }
     __syncthreads();
     if (!live) return;
-    T* dz = static_cast<T*>(a.dz) + (size_t)ob * V * a.inner + at;
-    for (int v = w; v < V; v += 4) dz[(size_t)v * a.inner] = (T)tile[v * 64 + px];
+    const float A = sh[px], o = sh[64 + px];
+    const bool zero = sh[128 + px] == 0.f;                               // pixels that count for nothing: zeros, whatever the logits hold
+    T* const dz = static_cast<T*>(a.dz) + (size_t)ob * V * a.inner + at;
+    for (int v0 = 0; v0 < V; v0 += 32) {
+        const unsigned b = bits[(v0 >> 5) * 64 + px] >> w;
+        T* const d = dz + (size_t)(v0 + w) * a.inner;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int v = v0 + w + 4 * j;
+            if (v < V) {
+                const float x = tile[v * 64 + px];
+                d[(size_t)(4 * j) * a.inner] = (T)(b >> (4 * j) & 1u ? x : zero ? 0.f : A * exp2_((x - o) * c));
+            }
+        }
+    }
 }
 
-size_t planes_lds(int V, int K) { return (size_t)64 * 4 * ((size_t)V + (V + 31) / 32 + 2 * (size_t)K) + 2 * 256 * sizeof(double); }
+size_t planes_lds(int V, int K) { return (size_t)64 * 4 * ((size_t)V + (V + 31) / 32 + 3 * (size_t)K + 6); }
 
 // partial sums of the weights, one per workgroup, each in a fixed order
 constexpr int WPARTS = 64;
@@ -645,7 +654,7 @@ int launch_distill(DistillArgs a, bool ready, hipStream_t stream) {
     if (!ready) {
         launch_rows<DT, SEG_STATS>(a, stream);
         CNM_LAUNCH_CHECK();
-        distill_join_kernel<DT><<<(unsigned)a.rows, 256, 0, stream>>>(a);
+        distill_join_kernel<DT><<<(unsigned)a.rows, 64, 0, stream>>>(a);
         CNM_LAUNCH_CHECK();
     }
     if (a.dz) {
@@ -954,14 +963,14 @@ __global__ __launch_bounds__(256) void top_planes_kernel(const TopArgs a) {
 constexpr int TOP_PLANES_KMAX = 16;
 
 // How rows are split: a workgroup of 512 threads holds 64 KB of a row; rows that are longer, or so few that they would leave most CUs idle,
-// are cut into up to 64 segments (at least 4 KB each) and joined by a second launch.
-int top_segments(long long rows, int V, int esize) {
+// are cut into segments (at least 4 KB each) and joined by a second launch.
+int top_segments(long long rows, int V, int K, int esize) {
     const int most = 512 * 8 * 16 / esize, least = cnm_ceil_div(V, most);
     if ((size_t)V * esize <= 8192 || rows >= 128) return least;
     int want = (int)(256 / rows);
-    const int fit = (int)((size_t)V * esize / 4096);
+    const int fit = (int)((size_t)V * esize / 4096), few = 2048 / K;     // (few: what is left to join is one number or two per thread)
     want = want < fit ? want : fit;
-    want = want < 64 ? want : 64;
+    want = want < few ? want : few;
     return want > least ? want : least;
 }
 
@@ -977,13 +986,13 @@ int launch_top(TopArgs a, hipStream_t stream) {
         CNM_LAUNCH_CHECK();
         return CNM_OK;
     }
-    a.segments = top_segments(a.rows, a.V, (int)sizeof(T));
+    a.segments = top_segments(a.rows, a.V, a.K, (int)sizeof(T));
     a.seglen = cnm_ceil_div(cnm_ceil_div(a.V, a.segments), E) * E;
     a.segments = cnm_ceil_div(a.V, a.seglen);
     const int vecs = a.seglen / E;
     const unsigned units = (unsigned)(a.rows * a.segments);
     if (vecs <= 64) top_rows_kernel<DT, 64, 1><<<cnm_ceil_div((int)units, 4), 256, 0, stream>>>(a);
-    else if (vecs <= 256) top_rows_kernel<DT, 64, 4><<<cnm_ceil_div((int)units, 4), 256, 0, stream>>>(a);
+    else if (vecs <= 256) top_rows_kernel<DT, 256, 1><<<units, 256, 0, stream>>>(a);
     else if (vecs <= 512) top_rows_kernel<DT, 512, 1><<<units, 512, 0, stream>>>(a);
     else if (vecs <= 1024) top_rows_kernel<DT, 512, 2><<<units, 512, 0, stream>>>(a);
     else if (vecs <= 2048) top_rows_kernel<DT, 512, 4><<<units, 512, 0, stream>>>(a);
@@ -1007,7 +1016,7 @@ extern "C" int cnm_distill_planes_ok(int classes, int entries) { return classes 
 
 extern "C" size_t cnm_top_logits_workspace_bytes(int dtype, long long rows, int classes, int entries, long long inner) {
     if (rows <= 0 || classes <= 0 || entries <= 0 || inner != 1 || dtype < CNM_F32 || dtype > CNM_BF16) return 0;
-    const int seg = top_segments(rows, classes, dtype == CNM_F32 ? 4 : 2);
+    const int seg = top_segments(rows, classes, entries, dtype == CNM_F32 ? 4 : 2);
     return seg > 1 ? (size_t)rows * seg * ((size_t)entries * sizeof(u64) + 2 * sizeof(float)) : 0;
 }
 
