@@ -89,6 +89,19 @@ struct Raw {
         }
     }
     __device__ void hold() { asm volatile("" : "+v"(w)); }
+    __device__ void drop(unsigned b) {                                   // the elements whose bit is set become -inf
+        if constexpr (DT == CNM_F32) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = b >> j & 1u ? 0xFF800000u : w[j];
+        } else {
+            constexpr unsigned none = DT == CNM_BF16 ? 0xFF80u : 0xFC00u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = b >> (2 * j) & 1u ? (w[j] & 0xFFFF0000u) | none : w[j];
+                w[j] = b >> (2 * j + 1) & 1u ? (w[j] & 0xFFFFu) | none << 16 : w[j];
+            }
+        }
+    }
     __device__ float get(int j) const {
         if constexpr (DT == CNM_F32) return __uint_as_float(w[j]);
         else if constexpr (DT == CNM_BF16) return __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
@@ -150,11 +163,15 @@ __device__ inline float exp2_of(double x) {
     return ldexpf(exp2_((float)(x - n)), (int)n);
 }
 
+// What a row's entries say by themselves: the teacher's log-sum-exp, sum p, sum p log2 p, the named classes' exponentials.
+struct Teacher { double L, P, lp; Lse named; int have; };
+
 // The entries of a row, shared by the threads that work on it.
 struct Entries {
     int idx[KMAX];                                                       // -1: none
     float z[KMAX], p[KMAX];                                              // the student's logit there; the teacher's logit, then the probability
     int dup;                                                             // some class is named twice
+    Teacher teach;
     Lse rest[16];                                                        // the waves' statistics of the unnamed classes
     DistillRow row;
 };
@@ -208,7 +225,6 @@ __device__ inline void join_entries(Entries& e, int K, int lane) {
 // A row's numbers, by one wave while the others go over the classes: the fp64 logarithms are hundreds of instructions, too many for every wave.
 // First what the entries alone say (e.p becomes the probabilities), then, with the unnamed classes' statistics, the loss and the gradient's
 // coefficients for an upstream gradient of 1.
-struct Teacher { double L, P, lp; Lse named; int have; };                // lp: sum p log2 p
 __device__ inline double sum_wave(double a) { for (int d = 32; d; d >>= 1) a += __shfl_xor(a, d); return a; }
 __device__ inline double max_wave(double a) { for (int d = 32; d; d >>= 1) a = fmax(a, __shfl_xor(a, d)); return a; }
 
@@ -249,7 +265,7 @@ __device__ inline Teacher entry_numbers(const DistillArgs& a, size_t r, Entries&
         }
         e.p[k] = p;
     }
-    w.P = sum_wave(P); w.lp = lp;
+    w.P = sum_wave(P); w.lp = sum_wave(lp);
     return w;
 }
 __device__ inline DistillRow finish_row(const DistillArgs& a, size_t r, Lse rest, const Teacher& w, Entries& e, float c, int lane) {
@@ -259,10 +275,10 @@ __device__ inline DistillRow finish_row(const DistillArgs& a, size_t r, Lse rest
     row.L = w.L;
     row.oall = all.o == ninf ? 0.f : all.o; row.orest = rest.o == ninf ? 0.f : rest.o;
     const double lq0 = -log2((double)all.s);                             // log2 q_v = (z_v - oall) c + lq0
-    double loss = w.lp;
+    double loss = 0.0;
     for (int k = lane; k < a.K; k += 64)
         if (e.p[k] > 0.f) loss -= (double)e.p[k] * (((double)e.z[k] - (double)row.oall) * (double)c + lq0);
-    loss = sum_wave(loss) * LN2_D;
+    loss = (w.lp + sum_wave(loss)) * LN2_D;
     double ratio = 0.0;                                                  // p_r / (sum of the unnamed exponentials)
     if (a.lse && rest.s > 0.f) {
         const double pr = 1.0 - w.P;
@@ -297,7 +313,7 @@ __device__ inline DistillRow finish_row(const DistillArgs& a, size_t r, Lse rest
 // gradients of each (SEG_GRAD), the second reading from the caches.
 enum { ROW, SEG_STATS, SEG_GRAD };
 template <int DT, int NT, int NV, int MODE>
-__global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_rows_kernel(const DistillArgs a) {
+__global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 512 && NV == 8 ? 6 : 1) void distill_rows_kernel(const DistillArgs a) {
     typedef typename Elem<DT>::T T;
     constexpr int RPB = NT == 64 ? 4 : 1, E = 16 / sizeof(T);
     extern __shared__ unsigned lds_words[];
@@ -329,26 +345,30 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_rows_kernel(const
     mark_entries<NT>(e, a.K, bits, v0, n, t);
     row_sync<NT>();
     const int lane = threadIdx.x & 63;
-    const auto mask = [&](int i) { const int at = (i * NT + t) * E; return at < n ? bits[at >> 5] >> (at & 31) : 0u; };
+    // named classes leave the row: their places are -inf from here on
+    unsigned b[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int at = (i * NT + t) * E;
+        b[i] = at < n ? bits[at >> 5] >> (at & 31) & ((1u << E) - 1) : 0u;
+        if (b[i]) x[i].drop(b[i]);
+    }
     if constexpr (MODE != SEG_GRAD) {
-        Teacher teach;
-        if (MODE == ROW && t < 64) teach = entry_numbers(a, r, e, c, lane);
+        if (MODE == ROW && t < 64) { const Teacher teach = entry_numbers(a, r, e, c, lane); if (lane == 0) e.teach = teach; }
         float m = ninf;                                                  // statistics of the unnamed classes
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             x[i].hold();
-            const unsigned b = mask(i);
 #pragma unroll
-            for (int j = 0; j < E; ++j) m = fmaxf(m, b >> j & 1u ? ninf : x[i].get(j));
+            for (int j = 0; j < E; ++j) m = fmaxf(m, x[i].get(j));
         }
         const float o = m == ninf ? 0.f : m;
         Lse rest = {m, 0.f};
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             x[i].hold();
-            const unsigned b = mask(i);
 #pragma unroll
-            for (int j = 0; j < E; ++j) rest.s += b >> j & 1u ? 0.f : exp2_((x[i].get(j) - o) * c);
+            for (int j = 0; j < E; ++j) rest.s += exp2_((x[i].get(j) - o) * c);
         }
         rest = lse_wave(rest, c);
         if (NT > 64) {
@@ -361,7 +381,8 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_rows_kernel(const
             return;
         }
         if (t < 64) {
-            const DistillRow row = finish_row(a, r, rest, teach, e, c, lane);
+            row_sync<64>();
+            const DistillRow row = finish_row(a, r, rest, e.teach, e, c, lane);
             if (lane == 0) e.row = row;
         }
     } else {
@@ -382,11 +403,10 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_rows_kernel(const
         const int at = (i * NT + t) * E;
         if (at < n) {
             x[i].hold();
-            const unsigned b = mask(i) & ((1u << E) - 1);
             T g[E];
 #pragma unroll
             for (int j = 0; j < E; ++j) g[j] = (T)(zero ? 0.f : A * exp2_((x[i].get(j) - w.orest) * c));
-            if (b && !zero) {
+            if (b[i] && !zero) {
                 for (int k = 0; k < a.K; ++k) {                          // few classes are named: look up whose
                     const int j = e.idx[k] - v0 - at;
                     if (e.idx[k] >= 0 && j >= 0 && j < E) {
@@ -798,7 +818,7 @@ __device__ inline float kth_bound(float m, int K, float* sh) {
 // NT threads per row or segment of a row, which they hold in registers (NV vectors of 16 bytes each), read once.  Log-sum-exp, then a lower bound of
 // the K-th largest logit from the threads' own maxima, the few logits above it to LDS, and their order by counting.
 template <int DT, int NT, int NV>
-__global__ __launch_bounds__(NT == 64 ? 256 : NT) void top_rows_kernel(const TopArgs a) {
+__global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 512 && NV == 8 ? 6 : 1) void top_rows_kernel(const TopArgs a) {
     typedef typename Elem<DT>::T T;
     constexpr int E = 16 / sizeof(T), RPB = NT == 64 ? 4 : 1;
     __shared__ TopShared shared[RPB];
