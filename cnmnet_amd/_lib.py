@@ -212,6 +212,10 @@ PROTOTYPES = {
     "cnm_matmul_fp8": (c_i, [c_fp, c_fp, c_fp, c_fp, c_i, c_fp, c_i, c_ll, c_ll, c_ll, c_ll, c_fp]),
     "cnm_linear_fp8_workspace_bytes": (c_sz, [c_ll, c_ll, c_ll]),
     "cnm_linear_fp8": (c_i, [c_fp, c_i, c_ll, c_fp, c_fp, c_fp, c_ll, c_ll, c_ll, c_ll, c_fp, c_sz, c_fp]),
+    "cnm_linear_fp8_keep_bytes": (c_sz, [c_ll, c_ll, c_ll, c_i, c_i]),
+    "cnm_linear_fp8_train_workspace_bytes": (c_sz, [c_ll, c_ll, c_ll]),
+    "cnm_linear_fp8_forward": (c_i, [c_fp, c_i, c_ll, c_fp, c_i, c_ll, c_fp, c_ll, c_ll, c_ll, c_i, c_i, c_fp, c_sz, c_fp, c_sz, c_fp]),
+    "cnm_linear_fp8_backward": (c_i, [c_fp, c_i, c_ll, c_fp, c_sz, c_fp, c_i, c_fp, c_i, c_ll, c_ll, c_ll, c_i, c_i, c_fp, c_sz, c_fp]),
     "cnm_top_logits_workspace_bytes": (c_sz, [c_i, c_ll, c_i, c_i, c_ll]),
     "cnm_top_logits": (c_i, [c_fp, c_i, c_ll, c_f, c_fp, c_fp, c_fp, c_fp, c_sz, c_ll, c_i, c_i, c_ll, c_fp]),
     "cnm_top_logits_planes_max_entries": (c_i, []),

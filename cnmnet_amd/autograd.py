@@ -739,31 +739,44 @@ class LinearFP8(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight):
-        if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:
+        if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1] or weight.shape[0] == 0:
             raise _lib.EngineError("linear_fp8: x %s against weight %s" % (tuple(x.shape), tuple(weight.shape)))
-        ops._dev_any(x, weight)
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        wq = ops.quantize_fp8(weight, 128, transposed=need_x)
-        xq = ops.quantize_fp8(x, 1, transposed=need_w)
-        ctx.save_for_backward(*(wq[2:] if need_x else (None, None)), *(xq[2:] if need_w else (None, None)))
-        ctx.info = x.shape, x.dtype, weight.shape, weight.dtype
-        return ops.matmul_fp8(xq[0], xq[1], wq[0], wq[1], x.dtype).view(*x.shape[:-1], weight.shape[0])
+        dev = ops._dev_any(x, weight)
+        need_x, need_w = ctx.needs_input_grad
+        x2, ldx = ops._rows2d(x, "linear_fp8")
+        w2, ldw = ops._rows2d(weight, "linear_fp8")
+        (M, K), N = x2.shape, w2.shape[0]
+        y = torch.empty(x.shape[:-1] + (N,), device=dev, dtype=x.dtype)
+        ctx.info = x.shape, x.dtype, weight.dtype, M, N, K, need_x, need_w
+        if M == 0:
+            return y
+        lib = _lib.load()
+        nk, nw = lib.cnm_linear_fp8_keep_bytes(M, N, K, need_x, need_w), lib.cnm_linear_fp8_train_workspace_bytes(M, N, K)
+        keep = torch.empty(nk, device=dev, dtype=torch.uint8) if nk else None
+        ws = torch.empty(nw, device=dev, dtype=torch.uint8)
+        with ops._on(dev):
+            _lib.check(lib.cnm_linear_fp8_forward(x2.data_ptr(), ops.DTYPES[x.dtype], ldx, w2.data_ptr(), ops.DTYPES[weight.dtype], ldw, y.data_ptr(), M, N, K, need_x, need_w,
+                                                  ops._p(keep), nk, ws.data_ptr(), nw, ops._raw_stream(dev)))
+        ctx.save_for_backward(keep)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        wt, wts, xt, xts = ctx.saved_tensors
-        x_shape, x_dtype, w_shape, w_dtype = ctx.info
-        need_x, need_w = wt is not None, xt is not None
-        dx = dw = None
-        if dy.numel() == 0:                                              # no rows
-            return (torch.zeros(x_shape, device=dy.device, dtype=x_dtype) if need_x else None,
-                    torch.zeros(w_shape, device=dy.device, dtype=w_dtype) if need_w else None)
-        q = ops.quantize_fp8(dy, 1, transposed=need_w)
-        if need_x:
-            dx = ops.matmul_fp8(q[0], q[1], wt, wts, x_dtype).view(x_shape)
-        if need_w:
-            dw = ops.matmul_fp8(q[2], q[3], xt, xts, w_dtype)
+        x_shape, x_dtype, w_dtype, M, N, K, need_x, need_w = ctx.info
+        dev = dy.device
+        dx = torch.empty(x_shape, device=dev, dtype=x_dtype) if need_x else None
+        if M == 0:
+            return dx, torch.zeros(N, K, device=dev, dtype=w_dtype) if need_w else None
+        keep, = ctx.saved_tensors
+        dw = torch.empty(N, K, device=dev, dtype=w_dtype) if need_w else None
+        d2, ld = ops._rows2d(dy, "linear_fp8")
+        lib = _lib.load()
+        nw = lib.cnm_linear_fp8_train_workspace_bytes(M, N, K)
+        ws = torch.empty(nw, device=dev, dtype=torch.uint8)
+        with ops._on(dev):
+            _lib.check(lib.cnm_linear_fp8_backward(d2.data_ptr(), ops.DTYPES[dy.dtype], ld, keep.data_ptr(), keep.numel(), ops._p(dx), ops.DTYPES[x_dtype],
+                                                   ops._p(dw), ops.DTYPES[w_dtype], M, N, K, need_x, need_w, ws.data_ptr(), nw, ops._raw_stream(dev)))
         return dx, dw
 
 

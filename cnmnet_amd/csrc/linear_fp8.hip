@@ -48,16 +48,10 @@ __device__ inline float inv_scale(int byte) { return __uint_as_float((unsigned)(
 
 __device__ inline float finite_abs(float v) { const float a = fabsf(v); return a < __builtin_huge_valf() ? a : 0.f; }   // (NaN compares false)
 
-// four values -> four e4m3 bytes; |v| <= 448 but for non-finite inputs
+// four values -> four e4m3 bytes; |v| <= 448 but for non-finite inputs, which the instruction turns into NaN (its overflow mode is off)
 __device__ inline unsigned pack4(float a, float b, float c, float d) {
     int p = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-    p = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, p, true);
-    unsigned u = (unsigned)p;
-    if (!(fabsf(a) < __builtin_huge_valf())) u = (u & ~0x000000FFu) | 0x0000007Fu;
-    if (!(fabsf(b) < __builtin_huge_valf())) u = (u & ~0x0000FF00u) | 0x00007F00u;
-    if (!(fabsf(c) < __builtin_huge_valf())) u = (u & ~0x00FF0000u) | 0x007F0000u;
-    if (!(fabsf(d) < __builtin_huge_valf())) u = (u & ~0xFF000000u) | 0x7F000000u;
-    return u;
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, p, true);
 }
 
 // eight consecutive values of a row, zero beyond `have` (16-byte loads whatever the row's alignment: global memory takes them)
@@ -75,29 +69,30 @@ __device__ inline void load8(const typename Elem<DT>::T* p, int have, float v[8]
     }
 }
 
-// One workgroup quantises a 128 x 128 tile, read once: 16 lanes per row (8 values each), a thread's eight rows consecutive, so that the
-// transposed copy leaves as 8-byte columns through LDS.  Row form: q [R][Cp], s [R][Cp/128] (BLK = false) or s [R/128][Cp/128] (BLK = true).
+// One workgroup quantises a 128 x 128 tile, read once: 16 lanes per row (8 values each), a thread's four rows consecutive, so that the
+// transposed copy leaves as 4-byte columns through LDS.  Row form: q [R][Cp], s [R][Cp/128] (BLK = false) or s [R/128][Cp/128] (BLK = true).
 // Transposed form (optional): qt [C][Rp], blocked along R: st [C][Rp/128], or the same 128 x 128 block's byte at st [C/128][Rp/128].
 template <int DT, bool BLK>
-__global__ __launch_bounds__(256) void quantize_kernel(const typename Elem<DT>::T* __restrict__ x, long long ldx, int R, int C, int Cb, int Rb,
+__global__ __launch_bounds__(512) void quantize_kernel(const typename Elem<DT>::T* __restrict__ x, long long ldx, int R, int C, int Cb, int Rb,
                                                        unsigned char* __restrict__ q, unsigned char* __restrict__ s,
                                                        unsigned char* __restrict__ qt, unsigned char* __restrict__ st) {
-    __shared__ float cmax[16][QB];
-    __shared__ unsigned char tile[QB][QB + 8];
-    __shared__ float bmax[4];
+    constexpr int NR = 4;                                                // rows per thread
+    __shared__ float cmax[8][QB];
+    __shared__ __attribute__((aligned(16))) unsigned char tile[QB][QB + 16];
+    __shared__ float bmax[8];
     const int tid = threadIdx.x, lc = tid & 15, lr = tid >> 4;
     const int cb = blockIdx.x % Cb, rb = blockIdx.x / Cb;
-    const int c0 = cb * QB + lc * 8, r0 = rb * QB + lr * 8;
-    float v[8][8];
+    const int c0 = cb * QB + lc * 8, r0 = rb * QB + lr * NR;
+    float v[NR][8];
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
+    for (int p = 0; p < NR; ++p) {
         const int r = r0 + p;
         load8<DT>(x + (size_t)(r < R ? r : 0) * ldx + (c0 < C ? c0 : 0), r < R ? C - c0 : 0, v[p]);
     }
-    int byte[8];
-    float am[8];
+    int byte[NR];
+    float am[NR];
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
+    for (int p = 0; p < NR; ++p) {
         float m = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(v[p][j]));
@@ -107,27 +102,29 @@ __global__ __launch_bounds__(256) void quantize_kernel(const typename Elem<DT>::
     if (BLK) {
         float m = 0.f;
 #pragma unroll
-        for (int p = 0; p < 8; ++p) m = fmaxf(m, am[p]);
+        for (int p = 0; p < NR; ++p) m = fmaxf(m, am[p]);
         m = fmaxf(m, __shfl_xor(m, 16)); m = fmaxf(m, __shfl_xor(m, 32));
         if ((tid & 63) == 0) bmax[tid >> 6] = m;
         __syncthreads();
-        m = fmaxf(fmaxf(bmax[0], bmax[1]), fmaxf(bmax[2], bmax[3]));
+        m = bmax[0];
 #pragma unroll
-        for (int p = 0; p < 8; ++p) byte[p] = scale_byte(m);
+        for (int i = 1; i < 8; ++i) m = fmaxf(m, bmax[i]);
+#pragma unroll
+        for (int p = 0; p < NR; ++p) byte[p] = scale_byte(m);
         if (tid == 0) {
             if (s) s[(size_t)rb * Cb + cb] = (unsigned char)byte[0];
             if (st) st[(size_t)cb * Rb + rb] = (unsigned char)byte[0];
         }
     } else {
 #pragma unroll
-        for (int p = 0; p < 8; ++p) {
+        for (int p = 0; p < NR; ++p) {
             byte[p] = scale_byte(am[p]);
             if (s && lc == 0 && r0 + p < R) s[(size_t)(r0 + p) * Cb + cb] = (unsigned char)byte[p];
         }
     }
     if (q) {
 #pragma unroll
-        for (int p = 0; p < 8; ++p) {
+        for (int p = 0; p < NR; ++p) {
             if (r0 + p < R) {
                 const float k = inv_scale(byte[p]);
                 uint2 u;
@@ -144,14 +141,16 @@ __global__ __launch_bounds__(256) void quantize_kernel(const typename Elem<DT>::
         for (int j = 0; j < 8; ++j) {
             float m = 0.f;
 #pragma unroll
-            for (int p = 0; p < 8; ++p) m = fmaxf(m, finite_abs(v[p][j]));
-            cmax[lr][lc * 8 + j] = m;
+            for (int p = 0; p < NR; ++p) m = fmaxf(m, finite_abs(v[p][j]));
+            m = fmaxf(m, __shfl_xor(m, 16)); m = fmaxf(m, __shfl_xor(m, 32));
+            if ((tid & 63) < 16) cmax[tid >> 6][lc * 8 + j] = m;
         }
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            float m = 0.f;
-            for (int g = 0; g < 16; ++g) m = fmaxf(m, cmax[g][lc * 8 + j]);
+            float m = cmax[0][lc * 8 + j];
+#pragma unroll
+            for (int g = 1; g < 8; ++g) m = fmaxf(m, cmax[g][lc * 8 + j]);
             const int b = scale_byte(m);
             k8[j] = inv_scale(b);
             if (lr == 0 && c0 + j < C) st[(size_t)(c0 + j) * Rb + rb] = (unsigned char)b;
@@ -161,18 +160,14 @@ __global__ __launch_bounds__(256) void quantize_kernel(const typename Elem<DT>::
         for (int j = 0; j < 8; ++j) k8[j] = inv_scale(byte[0]);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        uint2 u;
-        u.x = pack4(v[0][j] * k8[j], v[1][j] * k8[j], v[2][j] * k8[j], v[3][j] * k8[j]);
-        u.y = pack4(v[4][j] * k8[j], v[5][j] * k8[j], v[6][j] * k8[j], v[7][j] * k8[j]);
-        *reinterpret_cast<uint2*>(&tile[lc * 8 + j][lr * 8]) = u;
-    }
+    for (int j = 0; j < 8; ++j)
+        *reinterpret_cast<unsigned*>(&tile[lc * 8 + j][lr * NR]) = pack4(v[0][j] * k8[j], v[1][j] * k8[j], v[2][j] * k8[j], v[3][j] * k8[j]);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {                                        // 16 lanes x 8 bytes = one transposed row of the tile
-        const int c = i * 16 + lr;
+    for (int i = 0; i < 2; ++i) {                                        // 8 lanes x 16 bytes = one transposed row of the tile
+        const int c = i * 64 + (tid >> 3), l = tid & 7;
         if (cb * QB + c < C)
-            *reinterpret_cast<uint2*>(qt + (size_t)(cb * QB + c) * ((size_t)Rb * QB) + (size_t)rb * QB + lc * 8) = *reinterpret_cast<const uint2*>(&tile[c][lc * 8]);
+            *reinterpret_cast<uint4*>(qt + (size_t)(cb * QB + c) * ((size_t)Rb * QB) + (size_t)rb * QB + l * 16) = *reinterpret_cast<const uint4*>(&tile[c][l * 16]);
     }
 }
 
@@ -183,7 +178,7 @@ int launch_quantize(const void* x, long long ldx, int R, int C, void* q, void* s
     auto* xp = static_cast<const T*>(x);
     auto* qp = static_cast<unsigned char*>(q); auto* sp = static_cast<unsigned char*>(s);
     auto* qtp = static_cast<unsigned char*>(qt); auto* stp = static_cast<unsigned char*>(st);
-    quantize_kernel<DT, BLK><<<Cb * Rb, 256, 0, stream>>>(xp, ldx, R, C, Cb, Rb, qp, sp, qtp, stp);
+    quantize_kernel<DT, BLK><<<Cb * Rb, 512, 0, stream>>>(xp, ldx, R, C, Cb, Rb, qp, sp, qtp, stp);
     CNM_LAUNCH_CHECK();
     return CNM_OK;
 }
@@ -660,6 +655,70 @@ extern "C" int cnm_matmul_fp8(const void* a, const void* a_scale, const void* b,
     return CNM_ERR_BAD_ARG;
 }
 
+// ---- one training step of the layer.  A matrix in 8 bits, values then scales, in a byte buffer of fp8_bytes
+static size_t fp8_bytes(long long rows, long long cols, bool blocks) {
+    const size_t kb = (size_t)cnm_ceil_div_ll(cols, QB), n = (size_t)rows * kb * QB + (size_t)(blocks ? cnm_ceil_div_ll(rows, QB) : rows) * kb;
+    return (n + 15) / 16 * 16;
+}
+struct Fp8 { unsigned char *q = nullptr, *s = nullptr; };
+static Fp8 fp8_take(unsigned char*& at, long long rows, long long cols, bool blocks) {
+    Fp8 m;
+    m.q = at; m.s = at + (size_t)rows * cnm_ceil_div_ll(cols, QB) * QB;
+    at += fp8_bytes(rows, cols, blocks);
+    return m;
+}
+static bool dtype_ok(int d) { return d >= CNM_F32 && d <= CNM_BF16; }
+static bool train_shape_ok(long long M, long long N, long long K) {
+    const long long most = 1ll << 23;                                    // each of them is a reduced axis of some product
+    return M <= most - QB && N <= most - QB && K <= most - QB;
+}
+
+extern "C" size_t cnm_linear_fp8_keep_bytes(long long M, long long N, long long K, int need_dx, int need_dw) {
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    return (need_dx ? fp8_bytes(K, N, true) : 0) + (need_dw ? fp8_bytes(K, M, false) : 0);
+}
+extern "C" size_t cnm_linear_fp8_train_workspace_bytes(long long M, long long N, long long K) {
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    const size_t fwd = fp8_bytes(M, K, false) + fp8_bytes(N, K, true), bwd = fp8_bytes(M, N, false) + fp8_bytes(N, M, false);
+    return fwd > bwd ? fwd : bwd;
+}
+
+extern "C" int cnm_linear_fp8_forward(const void* x, int x_dtype, long long ldx, const void* w, int w_dtype, long long ldw, void* y,
+                                      long long M, long long N, long long K, int need_dx, int need_dw, void* keep, size_t keep_bytes,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+    CNM_REQUIRE(x && w && y && M > 0 && N > 0 && K > 0 && ldx >= K && ldw >= K && dtype_ok(x_dtype) && dtype_ok(w_dtype), CNM_ERR_BAD_ARG);   // (everything before the first launch)
+    CNM_REQUIRE(train_shape_ok(M, N, K), CNM_ERR_BAD_SHAPE);
+    CNM_REQUIRE(workspace && workspace_bytes >= cnm_linear_fp8_train_workspace_bytes(M, N, K) && keep_bytes >= cnm_linear_fp8_keep_bytes(M, N, K, need_dx, need_dw)
+                && (keep || !(need_dx || need_dw)) && ((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(keep)) & 15) == 0, CNM_ERR_WORKSPACE);
+    unsigned char *ws = static_cast<unsigned char*>(workspace), *kp = static_cast<unsigned char*>(keep);
+    const Fp8 xq = fp8_take(ws, M, K, false), wq = fp8_take(ws, N, K, true);
+    Fp8 wt, xt;
+    if (need_dx) wt = fp8_take(kp, K, N, true);
+    if (need_dw) xt = fp8_take(kp, K, M, false);
+    int rc = cnm_quantize_fp8(w, w_dtype, ldw, N, K, QB, wq.q, wq.s, wt.q, wt.s, stream);
+    if (rc == CNM_OK) rc = cnm_quantize_fp8(x, x_dtype, ldx, M, K, 1, xq.q, xq.s, xt.q, xt.s, stream);
+    return rc != CNM_OK ? rc : cnm_matmul_fp8(xq.q, xq.s, wq.q, wq.s, QB, y, x_dtype, N, M, N, cnm_ceil_div_ll(K, QB) * QB, stream);
+}
+
+extern "C" int cnm_linear_fp8_backward(const void* dy, int dy_dtype, long long lddy, const void* keep, size_t keep_bytes, void* dx, int dx_dtype, void* dw, int dw_dtype,
+                                       long long M, long long N, long long K, int kept_dx, int kept_dw, void* workspace, size_t workspace_bytes, void* stream) {
+    CNM_REQUIRE(dy && keep && (dx || dw) && M > 0 && N > 0 && K > 0 && lddy >= N && (!dx || kept_dx) && (!dw || kept_dw), CNM_ERR_BAD_ARG);
+    CNM_REQUIRE(dtype_ok(dy_dtype) && (!dx || dtype_ok(dx_dtype)) && (!dw || dtype_ok(dw_dtype)), CNM_ERR_BAD_ARG);
+    CNM_REQUIRE(train_shape_ok(M, N, K), CNM_ERR_BAD_SHAPE);
+    CNM_REQUIRE(workspace && workspace_bytes >= cnm_linear_fp8_train_workspace_bytes(M, N, K) && keep_bytes >= cnm_linear_fp8_keep_bytes(M, N, K, kept_dx, kept_dw)
+                && ((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(keep)) & 15) == 0, CNM_ERR_WORKSPACE);
+    unsigned char *ws = static_cast<unsigned char*>(workspace), *kp = static_cast<unsigned char*>(const_cast<void*>(keep));
+    Fp8 wt, xt, dyq, dyt;
+    if (kept_dx) wt = fp8_take(kp, K, N, true);
+    if (kept_dw) xt = fp8_take(kp, K, M, false);
+    if (dx) dyq = fp8_take(ws, M, N, false);
+    if (dw) dyt = fp8_take(ws, N, M, false);
+    int rc = cnm_quantize_fp8(dy, dy_dtype, lddy, M, N, 1, dyq.q, dyq.s, dyt.q, dyt.s, stream);
+    if (rc == CNM_OK && dx) rc = cnm_matmul_fp8(dyq.q, dyq.s, wt.q, wt.s, QB, dx, dx_dtype, K, M, K, cnm_ceil_div_ll(N, QB) * QB, stream);
+    if (rc == CNM_OK && dw) rc = cnm_matmul_fp8(dyt.q, dyt.s, xt.q, xt.s, 1, dw, dw_dtype, K, N, K, cnm_ceil_div_ll(M, QB) * QB, stream);
+    return rc;
+}
+
 extern "C" size_t cnm_linear_fp8_workspace_bytes(long long M, long long N, long long K) {
     if (M <= 0 || N <= 0 || K <= 0 || M <= 16 || N <= FEW_COLS) return 0;
     const size_t kb = (size_t)cnm_ceil_div_ll(K, QB);
@@ -669,7 +728,7 @@ extern "C" size_t cnm_linear_fp8_workspace_bytes(long long M, long long N, long 
 extern "C" int cnm_linear_fp8(const void* x, int dtype, long long ldx, const void* w, const void* w_scale, void* y, long long ldy,
                               long long M, long long N, long long K, void* workspace, size_t workspace_bytes, void* stream) {
     CNM_REQUIRE(x && w && w_scale && y && M > 0 && N > 0 && K > 0 && ldx >= K && ldy >= N, CNM_ERR_BAD_ARG);
-    CNM_REQUIRE((reinterpret_cast<uintptr_t>(w) & 15) == 0 && dtype >= CNM_F32 && dtype <= CNM_BF16, CNM_ERR_BAD_ARG);
+    CNM_REQUIRE((reinterpret_cast<uintptr_t>(w) & 15) == 0 && dtype_ok(dtype), CNM_ERR_BAD_ARG);
     CNM_REQUIRE(M < (1ll << 31) - 256 && N < (1ll << 31) - 256 && K <= (1ll << 23) && cnm_ceil_div_ll(M, 16) * cnm_ceil_div_ll(N, 16) < (1ll << 31), CNM_ERR_BAD_SHAPE);
     const size_t need = cnm_linear_fp8_workspace_bytes(M, N, K);
     const long long kb = cnm_ceil_div_ll(K, QB);

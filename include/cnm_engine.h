@@ -878,6 +878,17 @@ int cnm_matmul_fp8(const void* a, const void* a_scale, const void* b, const void
 size_t cnm_linear_fp8_workspace_bytes(long long M, long long N, long long K);
 int cnm_linear_fp8(const void* x, int dtype, long long ldx, const void* w, const void* w_scale, void* y, long long ldy,
                    long long M, long long N, long long K, void* workspace, size_t workspace_bytes, void* stream);
+/* A training step of the layer: forward y [M][N] = Q(x) Q(w)^T with x [M][ldx], w [N][ldw] each of its own dtype (y of x's), and, for the gradients
+ * that are needed, the transposed 8-bit forms in `keep` (cnm_linear_fp8_keep_bytes); backward dx [M][K] = Q(dy) Q(w), dw [N][K] = Q(dy^T) Q(x^T)^T,
+ * either may be NULL.  kept_dx / kept_dw: need_dx / need_dw of the forward call.  workspace: cnm_linear_fp8_train_workspace_bytes for each
+ * call, contents irrelevant; both buffers on 16 bytes.  M, N, K below 2^23 - 128. */
+size_t cnm_linear_fp8_keep_bytes(long long M, long long N, long long K, int need_dx, int need_dw);
+size_t cnm_linear_fp8_train_workspace_bytes(long long M, long long N, long long K);
+int cnm_linear_fp8_forward(const void* x, int x_dtype, long long ldx, const void* w, int w_dtype, long long ldw, void* y,
+                           long long M, long long N, long long K, int need_dx, int need_dw, void* keep, size_t keep_bytes,
+                           void* workspace, size_t workspace_bytes, void* stream);
+int cnm_linear_fp8_backward(const void* dy, int dy_dtype, long long lddy, const void* keep, size_t keep_bytes, void* dx, int dx_dtype, void* dw, int dw_dtype,
+                            long long M, long long N, long long K, int kept_dx, int kept_dw, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------ distillation from a teacher's top logits
  * Beside the reference's losses (depthnet/losses.py), which compare maps: these compare distributions over classes (depth planes, tokens).

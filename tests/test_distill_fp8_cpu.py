@@ -62,6 +62,33 @@ def test_linear_entry_refuses():
     assert with_(_9=(1 << 23) + 1, _2=1 << 24) == -2
 
 
+def test_linear_training_entries_refuse():
+    lib = _lib.load()
+    M, N, K = 100, 300, 200
+    nk, nw = lib.cnm_linear_fp8_keep_bytes(M, N, K, 1, 1), lib.cnm_linear_fp8_train_workspace_bytes(M, N, K)
+    assert nk >= K * 384 + 6 + K * 128 + K and lib.cnm_linear_fp8_keep_bytes(M, N, K, 0, 0) == 0 and nk % 16 == 0 and nw % 16 == 0
+    fwd = [64, 0, 200, 64, 2, 200, 64, M, N, K, 1, 1, 4096, nk, 4096, nw, 0]
+    bwd = [64, 0, 300, 4096, nk, 64, 0, 64, 0, M, N, K, 1, 1, 4096, nw, 0]
+
+    def call(f, ok, **kw):
+        a = list(ok)
+        for k, v in kw.items():
+            a[int(k[1:])] = v
+        return f(*a)
+    f = lib.cnm_linear_fp8_forward
+    for i in (0, 3, 6, 7, 8, 9):
+        assert call(f, fwd, **{"_%d" % i: 0}) == -1
+    assert call(f, fwd, _2=199) == -1 and call(f, fwd, _5=199) == -1 and call(f, fwd, _1=4) == -1 and call(f, fwd, _4=3) == -1
+    assert call(f, fwd, _12=0) == -5 and call(f, fwd, _13=nk - 1) == -5 and call(f, fwd, _14=0) == -5 and call(f, fwd, _15=nw - 1) == -5 and call(f, fwd, _12=4104) == -5
+    assert call(f, fwd, _7=1 << 23) == -2
+    f = lib.cnm_linear_fp8_backward
+    for i in (0, 3, 9, 10, 11):
+        assert call(f, bwd, **{"_%d" % i: 0}) == -1
+    assert call(f, bwd, _5=0, _7=0) == -1 and call(f, bwd, _2=299) == -1 and call(f, bwd, _12=0) == -1 and call(f, bwd, _13=0) == -1 and call(f, bwd, _1=9) == -1
+    assert call(f, bwd, _6=3) == -1 and call(f, bwd, _8=-1) == -1
+    assert call(f, bwd, _4=nk - 1) == -5 and call(f, bwd, _14=0) == -5 and call(f, bwd, _15=nw - 1) == -5
+
+
 def test_top_and_distill_entries_refuse():
     lib = _lib.load()
     top = [64, 0, 100, 1.0, 64, 64, 64, 0, 0, 4, 100, 8, 1, 0]
