@@ -405,8 +405,11 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 512 && NV == 8 ? 6 : 1) 
             x[i].hold();
             T g[E];
 #pragma unroll
-            for (int j = 0; j < E; ++j) g[j] = (T)(zero ? 0.f : A * exp2_((x[i].get(j) - w.orest) * c));
-            if (b[i] && !zero) {
+            for (int j = 0; j < E; ++j) g[j] = (T)(A * exp2_((x[i].get(j) - w.orest) * c));
+            if (zero) {
+#pragma unroll
+                for (int j = 0; j < E; ++j) g[j] = (T)0.f;
+            } else if (b[i]) {
                 for (int k = 0; k < a.K; ++k) {                          // few classes are named: look up whose
                     const int j = e.idx[k] - v0 - at;
                     if (e.idx[k] >= 0 && j >= 0 && j < E) {
@@ -818,7 +821,7 @@ __device__ inline float kth_bound(float m, int K, float* sh) {
 // NT threads per row or segment of a row, which they hold in registers (NV vectors of 16 bytes each), read once.  Log-sum-exp, then a lower bound of
 // the K-th largest logit from the threads' own maxima, the few logits above it to LDS, and their order by counting.
 template <int DT, int NT, int NV>
-__global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 512 && NV == 8 ? 6 : 1) void top_rows_kernel(const TopArgs a) {
+__global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 256 && NV == 16 ? 4 : 1) void top_rows_kernel(const TopArgs a) {
     typedef typename Elem<DT>::T T;
     constexpr int E = 16 / sizeof(T), RPB = NT == 64 ? 4 : 1;
     __shared__ TopShared shared[RPB];
@@ -1016,7 +1019,7 @@ int launch_top(TopArgs a, hipStream_t stream) {
     else if (vecs <= 512) top_rows_kernel<DT, 512, 1><<<units, 512, 0, stream>>>(a);
     else if (vecs <= 1024) top_rows_kernel<DT, 512, 2><<<units, 512, 0, stream>>>(a);
     else if (vecs <= 2048) top_rows_kernel<DT, 512, 4><<<units, 512, 0, stream>>>(a);
-    else top_rows_kernel<DT, 512, 8><<<units, 512, 0, stream>>>(a);
+    else top_rows_kernel<DT, 256, 16><<<units, 256, 0, stream>>>(a);
     CNM_LAUNCH_CHECK();
     if (a.segments > 1) {
         const int total = a.segments * a.K;
