@@ -477,14 +477,19 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
     const float c = (float)(LOG2E_D / (double)a.T), ninf = -__builtin_huge_valf();
 
     for (int i = w; i < nw; i += 4) bits[i * 64 + px] = 0u;
+    T first[16];                                                         // sixteen of the wave's classes are requested before anything waits
+#pragma unroll
+    for (int j = 0; j < 16; ++j) first[j] = z[(size_t)min(w + 4 * j, V - 1) * a.inner];
     for (int k = w; k < K; k += 4) {
         const long long i = live ? load_index(a.idx, a.wide, ebase + (size_t)k * a.inner) : -1;
         const bool ok = i >= 0 && i < V;
         eidx[k * 64 + px] = ok ? (int)i : -1;
         ep[k * 64 + px] = ok ? load_any(a.val, a.vdt, ebase + (size_t)k * a.inner) : 0.f;
     }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) if (w + 4 * j < V) tile[(w + 4 * j) * 64 + px] = live ? (float)first[j] : 0.f;
 #pragma unroll 8
-    for (int v = w; v < V; v += 4) tile[v * 64 + px] = live ? (float)z[(size_t)v * a.inner] : 0.f;
+    for (int v = w + 64; v < V; v += 4) tile[v * 64 + px] = live ? (float)z[(size_t)v * a.inner] : 0.f;
     __syncthreads();
     Lse named = {ninf, 0.f};
     bool have = false, dup = false;

@@ -448,10 +448,11 @@ struct StreamArgs {
     int M, N, K, Kb, bshift;                 // K: columns of x that exist (QUANT)
 };
 
+constexpr int stream_waves(int ks) { return ks > 1 ? ks : 4; }            // per workgroup: small ones where nothing is shared, so that all fit the CUs at once
 template <int DT, bool QUANT, int MT, int NT_, int KS, int PF>
-__global__ __launch_bounds__(512) void stream_kernel(const StreamArgs g) {
+__global__ __launch_bounds__(stream_waves(KS) * 64) void stream_kernel(const StreamArgs g) {
     typedef typename Elem<DT>::T T;
-    constexpr int MG = 8 / KS;                                           // row groups per workgroup
+    constexpr int MG = stream_waves(KS) / KS;                                           // row groups per workgroup
     __shared__ float part[KS > 1 ? KS : 1][KS > 1 ? NT_ * 16 : 1][KS > 1 ? MT * 16 + 1 : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ks = wave % KS, mg = wave / KS, fr = lane & 15, fg = lane >> 4;
@@ -473,75 +474,93 @@ __global__ __launch_bounds__(512) void stream_kernel(const StreamArgs g) {
         else { qp[i] = static_cast<const unsigned char*>(g.x) + (size_t)m * g.Kb * QB + fg * 32; sxp[i] = g.sx + (size_t)m * g.Kb; }
     }
     f32x4 acc[MT][NT_] = {};
-    for (int g0 = ks; g0 < g.Kb; g0 += KS * PF) {
-        i32x8 fw[PF][NT_], fx[PF][QUANT ? 1 : MT];
-        int bw[PF][NT_], bx[PF][MT];
-        T raw[PF][QUANT ? MT : 1][32];
+    i32x8 fw[PF][NT_], fa[PF][MT];
+    int bw[PF][NT_], ba[PF][MT];
+    T raw[PF][QUANT ? MT : 1][32];
+    const auto request_x = [&](int p, int kb) {
+        if (kb >= g.Kb) return;
 #pragma unroll
-        for (int p = 0; p < PF; ++p) {
-            const int kb = g0 + p * KS;
-            if (kb < g.Kb) {
+        for (int i = 0; i < MT; ++i) {
+            if constexpr (QUANT) {
+                const T* const src = xp[i] + (size_t)kb * QB;
+                const int have = g.K - kb * QB - fg * 32;
+                if (have >= 32) __builtin_memcpy(raw[p][i], src, 32 * sizeof(T));
+                else {
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    if constexpr (QUANT) {
-                        const T* const src = xp[i] + (size_t)kb * QB;
-                        const int have = g.K - kb * QB - fg * 32;
-                        if (have >= 32) __builtin_memcpy(raw[p][i], src, 32 * sizeof(T));
-                        else {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) raw[p][i][e] = e < have ? src[e] : (T)0.f;
-                        }
-                    } else {
-                        __builtin_memcpy(&fx[p][i], qp[i] + (size_t)kb * QB, 32);
-                        bx[p][i] = sxp[i][kb];
-                    }
+                    for (int e = 0; e < 32; ++e) raw[p][i][e] = e < have ? src[e] : (T)0.f;
                 }
-#pragma unroll
-                for (int j = 0; j < NT_; ++j) {
-                    __builtin_memcpy(&fw[p][j], wp[j] + (size_t)kb * QB, 32);
-                    bw[p][j] = swp[j][kb];
-                }
+            } else {
+                __builtin_memcpy(&fa[p][i], qp[i] + (size_t)kb * QB, 32);
+                ba[p][i] = sxp[i][kb];
             }
         }
+    };
+    const auto request_w = [&](int p, int kb) {
+        if (kb >= g.Kb) return;
 #pragma unroll
-        for (int p = 0; p < PF; ++p) {
-            if (g0 + p * KS < g.Kb) {
+        for (int j = 0; j < NT_; ++j) {
+            __builtin_memcpy(&fw[p][j], wp[j] + (size_t)kb * QB, 32);
+            bw[p][j] = swp[j][kb];
+        }
+    };
+    const auto quantize_x = [&](int p, int kb) {
+        if (kb >= g.Kb) return;
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    i32x8 fa;
-                    int ba;
-                    if constexpr (QUANT) {
-                        float v[32], m = 0.f;
+        for (int i = 0; i < MT; ++i) {
+            float v[32], m = 0.f;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) { v[e] = Elem<DT>::up(raw[p][i][e]); m = fmaxf(m, fabsf(v[e])); }
-                        m = fmaxf(m, __shfl_xor(m, 16)); m = fmaxf(m, __shfl_xor(m, 32));
-                        if (__any(m == __builtin_huge_valf())) {         // an infinity in some row's block: it does not take part in the maximum
-                            m = 0.f;
+            for (int e = 0; e < 32; ++e) { v[e] = Elem<DT>::up(raw[p][QUANT ? i : 0][e]); m = fmaxf(m, fabsf(v[e])); }
+            m = fmaxf(m, __shfl_xor(m, 16)); m = fmaxf(m, __shfl_xor(m, 32));
+            if (__any(m == __builtin_huge_valf())) {                     // an infinity in some row's block: it does not take part in the maximum
+                m = 0.f;
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) m = fmaxf(m, finite_abs(v[e]));
-                            m = fmaxf(m, __shfl_xor(m, 16)); m = fmaxf(m, __shfl_xor(m, 32));
-                        }
-                        ba = scale_byte(m);
-                        const float k = inv_scale(ba);
+                for (int e = 0; e < 32; ++e) m = fmaxf(m, finite_abs(v[e]));
+                m = fmaxf(m, __shfl_xor(m, 16)); m = fmaxf(m, __shfl_xor(m, 32));
+            }
+            ba[p][i] = scale_byte(m);
+            const float k = inv_scale(ba[p][i]);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) fa[e] = (int)pack4(v[4 * e] * k, v[4 * e + 1] * k, v[4 * e + 2] * k, v[4 * e + 3] * k);
-                    } else {
-                        fa = fx[p][i]; ba = bx[p][i];
-                    }
-                    if constexpr (DT == CNM_F32) {
+            for (int e = 0; e < 8; ++e) fa[p][i][e] = (int)pack4(v[4 * e] * k, v[4 * e + 1] * k, v[4 * e + 2] * k, v[4 * e + 3] * k);
+        }
+    };
+    const auto multiply = [&](int p, int kb) {
+        if (kb >= g.Kb) return;
 #pragma unroll
-                        for (int h = 0; h < 4; ++h) {
-                            const bf16x8 xa = widen(fa[2 * h], fa[2 * h + 1], scale_float((unsigned)ba, 0));
+        for (int i = 0; i < MT; ++i) {
+            if constexpr (DT == CNM_F32) {
 #pragma unroll
-                            for (int j = 0; j < NT_; ++j)
-                                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(fw[p][j][2 * h], fw[p][j][2 * h + 1], scale_float((unsigned)bw[p][j], 0)), xa, acc[i][j], 0, 0, 0);
-                        }
-                    } else {
+                for (int h = 0; h < 4; ++h) {
+                    const bf16x8 xa = widen(fa[p][i][2 * h], fa[p][i][2 * h + 1], scale_float((unsigned)ba[p][i], 0));
 #pragma unroll
-                        for (int j = 0; j < NT_; ++j)
-                            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[p][j], fa, acc[i][j], 0, 0, 0, bw[p][j], 0, ba);
-                    }
+                    for (int j = 0; j < NT_; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(fw[p][j][2 * h], fw[p][j][2 * h + 1], scale_float((unsigned)bw[p][j], 0)), xa, acc[i][j], 0, 0, 0);
                 }
+            } else {
+#pragma unroll
+                for (int j = 0; j < NT_; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[p][j], fa[p][i], acc[i][j], 0, 0, 0, bw[p][j], 0, ba[p][i]);
+            }
+        }
+    };
+    if constexpr (KS == 1) {
+        // x is what streams: the next block is requested once this one's registers are free, behind this one's w (loads return in order: w
+        // from the caches must not wait for x)
+        static_assert(PF == 1, "one block ahead");
+        request_x(0, 0);
+        for (int kb = 0; kb < g.Kb; ++kb) {
+            request_w(0, kb);
+            quantize_x(0, kb);
+            request_x(0, kb + 1);
+            multiply(0, kb);
+        }
+    } else {                                                             // w is what streams
+        for (int g0 = ks; g0 < g.Kb; g0 += KS * PF) {
+#pragma unroll
+            for (int p = 0; p < PF; ++p) { request_x(p, g0 + p * KS); request_w(p, g0 + p * KS); }   // (x first: loads return in order, and x has to be quantised)
+#pragma unroll
+            for (int p = 0; p < PF; ++p) {
+                if constexpr (QUANT) quantize_x(p, g0 + p * KS);
+                multiply(p, g0 + p * KS);
             }
         }
     }
@@ -558,7 +577,7 @@ __global__ __launch_bounds__(512) void stream_kernel(const StreamArgs g) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) part[ks][j * 16 + 4 * fg + e][i * 16 + fr] = acc[i][j][e];
         __syncthreads();
-        for (int o = threadIdx.x; o < MT * 16 * NT_ * 16; o += 512) {
+        for (int o = threadIdx.x; o < MT * 16 * NT_ * 16; o += stream_waves(KS) * 64) {
             const int n = o % (NT_ * 16), m = o / (NT_ * 16);
             float s = part[0][n][m];
 #pragma unroll
@@ -589,8 +608,8 @@ __global__ __launch_bounds__(512) void stream_kernel(const StreamArgs g) {
 
 template <int DT, bool QUANT, int MT, int NT_, int KS, int PF>
 int launch_stream(const StreamArgs& g, hipStream_t stream) {
-    const long long blocks = (long long)cnm_ceil_div(g.N, NT_ * 16) * cnm_ceil_div(g.M, 8 / KS * MT * 16);
-    stream_kernel<DT, QUANT, MT, NT_, KS, PF><<<(unsigned)blocks, 512, 0, stream>>>(g);
+    const long long blocks = (long long)cnm_ceil_div(g.N, NT_ * 16) * cnm_ceil_div(g.M, stream_waves(KS) / KS * MT * 16);
+    stream_kernel<DT, QUANT, MT, NT_, KS, PF><<<(unsigned)blocks, stream_waves(KS) * 64, 0, stream>>>(g);
     CNM_LAUNCH_CHECK();
     return CNM_OK;
 }
@@ -599,9 +618,9 @@ int launch_stream(const StreamArgs& g, hipStream_t stream) {
 template <int DT>
 int launch_few_rows(const StreamArgs& g, hipStream_t stream) {
     if (g.M <= 16) return launch_stream<DT, false, 1, 1, 8, 4>(g, stream);
-    if (g.M <= 32) return launch_stream<DT, false, 2, 1, 8, 4>(g, stream);
-    if (g.M <= 48) return launch_stream<DT, false, 3, 1, 8, 4>(g, stream);
-    return launch_stream<DT, false, 4, 1, 8, 4>(g, stream);
+    if (g.M <= 32) return launch_stream<DT, false, 2, 1, 8, 2>(g, stream);
+    if (g.M <= 48) return launch_stream<DT, false, 3, 1, 8, 2>(g, stream);
+    return launch_stream<DT, false, 4, 1, 8, 2>(g, stream);
 }
 
 // x as it is: few columns, or at most 16 rows
