@@ -209,7 +209,8 @@ PROTOTYPES = {
     "cnm_refinenet_forward_multi_cpu": (c_i, [C.POINTER(LayerWeights), c_f, c_fp, c_fp, c_i, c_fp, c_fp, c_fp,
                                               c_fp, c_sz, c_i, c_i, c_i]),
     "cnm_quantize_fp8": (c_i, [c_fp, c_i, c_ll, c_ll, c_ll, c_i, c_fp, c_fp, c_fp, c_fp, c_fp]),
-    "cnm_matmul_fp8": (c_i, [c_fp, c_fp, c_fp, c_fp, c_i, c_fp, c_i, c_ll, c_ll, c_ll, c_ll, c_fp]),
+    "cnm_matmul_fp8_workspace_bytes": (c_sz, [c_i, c_ll, c_ll, c_ll]),
+    "cnm_matmul_fp8": (c_i, [c_fp, c_fp, c_fp, c_fp, c_i, c_fp, c_i, c_ll, c_ll, c_ll, c_ll, c_fp, c_sz, c_fp]),
     "cnm_linear_fp8_workspace_bytes": (c_sz, [c_ll, c_ll, c_ll]),
     "cnm_linear_fp8": (c_i, [c_fp, c_i, c_ll, c_fp, c_fp, c_fp, c_ll, c_ll, c_ll, c_ll, c_fp, c_sz, c_fp]),
     "cnm_linear_fp8_keep_bytes": (c_sz, [c_ll, c_ll, c_ll, c_i, c_i]),

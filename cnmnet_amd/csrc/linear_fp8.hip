@@ -198,6 +198,7 @@ struct MatArgs {
     int M, N, Kb, bshift;
     long long ldc;
     int tiles_m, tiles_n;
+    int splits, chunk;                       // SPLIT: ranges of `chunk` blocks (a multiple of four) along the reduced axis, c = [splits][M][N] fp32
 };
 
 // Tiles in an order that keeps neighbours on one XCD near each other: workgroups are dealt to XCDs in contiguous ranges (xcd_remap), and a
@@ -237,7 +238,7 @@ struct Mat {
     static_assert(TM % (16 * NW) == 0 && TN % (16 * NW) == 0 && LDS <= 160 * 1024 && (!BLK || (TN % QB == 0 && TN / WN <= QB)), "tile");
 };
 
-template <int TM, int TN, int WM, int WN, int DT, bool BLK>
+template <int TM, int TN, int WM, int WN, int DT, bool BLK, bool SPLIT>
 __global__ __launch_bounds__(WM * WN * 64) void matmul_fp8_kernel(const MatArgs g) {
     typedef Mat<TM, TN, WM, WN, DT, BLK> C;
     constexpr int IM = C::IM, IN = C::IN;
@@ -247,11 +248,12 @@ __global__ __launch_bounds__(WM * WN * 64) void matmul_fp8_kernel(const MatArgs 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN;
     int tm, tn;
-    tile_of(xcd_remap(blockIdx.x, gridDim.x), g, tm, tn);
+    const int id = xcd_remap(blockIdx.x, gridDim.x), split = SPLIT ? id / (g.tiles_m * g.tiles_n) : 0;
+    tile_of(SPLIT ? id - split * g.tiles_m * g.tiles_n : id, g, tm, tn);
     const int m0 = tm * TM, n0 = tn * TN, Kb = g.Kb, K = Kb * QB;
     // buffer ranges that end with the operands' last rows: beyond them the DMA writes zeros
     const unsigned bytes_a = (unsigned)min(g.M - m0, TM) * (unsigned)K, bytes_b = (unsigned)min(g.N - n0, TN) * (unsigned)K;
-    const int S = 2 * Kb;
+    const int kb0 = SPLIT ? split * g.chunk : 0, kb1 = SPLIT ? min(Kb, kb0 + g.chunk) : Kb, S = 2 * kb1;
     const unsigned chunk = (unsigned)((lane & 3) ^ ((lane >> 4) & 3)) * 16u;
     const unsigned va = (unsigned)(wave * C::PA * 16 + (lane >> 2)) * (unsigned)K + chunk, vb = (unsigned)(wave * C::PB * 16 + (lane >> 2)) * (unsigned)K + chunk;
     auto issue = [&](int s) {                                            // half block s into its place in the ring; beyond the last one an empty range: zeros, no traffic, the same count
@@ -338,15 +340,15 @@ __global__ __launch_bounds__(WM * WN * 64) void matmul_fp8_kernel(const MatArgs 
         }
     };
 
-    issue(0);
-    issue(1);
-    fill(sca, g.sa, m0, TM, g.M - 1, 0);
-    fill(scb, g.sb, n0 >> g.bshift, C::BROWS, (g.N - 1) >> g.bshift, 0);
-    issue(2);
+    issue(2 * kb0);
+    issue(2 * kb0 + 1);
+    fill(sca, g.sa, m0, TM, g.M - 1, kb0 & ~(C::SC - 1));
+    fill(scb, g.sb, n0 >> g.bshift, C::BROWS, (g.N - 1) >> g.bshift, kb0 & ~(C::SC - 1));
+    issue(2 * kb0 + 2);
     __syncthreads();                                                     // everything issued so far is in LDS
-    load(0, 0);
-    for (int kb = 0; kb < Kb; ++kb) {
-        if (kb && (kb & (C::SC - 1)) == 0) {
+    load(2 * kb0, 0);
+    for (int kb = kb0; kb < kb1; ++kb) {
+        if (kb != kb0 && (kb & (C::SC - 1)) == 0) {
             __syncthreads();
             fill(sca, g.sa, m0, TM, g.M - 1, kb);
             fill(scb, g.sb, n0 >> g.bshift, C::BROWS, (g.N - 1) >> g.bshift, kb);
@@ -374,7 +376,8 @@ __global__ __launch_bounds__(WM * WN * 64) void matmul_fp8_kernel(const MatArgs 
         for (int j = 0; j < IN; ++j) asm volatile("" : "+v"(acc[i][j]));
     // the wave's outputs through LDS (its own part of the ring), so that they leave as whole 128-byte lines: straight from the accumulators a
     // store instruction would touch 32 rows, 16 bytes each
-    typedef typename Elem<DT>::T T;
+    constexpr int ST = SPLIT ? CNM_F32 : DT;                             // what is stored
+    typedef typename Elem<ST>::T T;
     constexpr int WTM = TM / WM, WTN = TN / WN, E = 16 / (int)sizeof(T), CH = WTN / E;    // 16-byte chunks per row, permuted by the row
     static_assert(TM * TN * (int)sizeof(T) <= C::NST * C::STAGE && CH % 8 == 0, "epilogue");
     typedef T T4 __attribute__((ext_vector_type(4)));
@@ -389,12 +392,12 @@ __global__ __launch_bounds__(WM * WN * 64) void matmul_fp8_kernel(const MatArgs 
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int n = j * 32 + 8 * q + 4 * fh;
-                const T4 v = {Elem<DT>::down(acc[i][j][4 * q]), Elem<DT>::down(acc[i][j][4 * q + 1]), Elem<DT>::down(acc[i][j][4 * q + 2]), Elem<DT>::down(acc[i][j][4 * q + 3])};
+                const T4 v = {Elem<ST>::down(acc[i][j][4 * q]), Elem<ST>::down(acc[i][j][4 * q + 1]), Elem<ST>::down(acc[i][j][4 * q + 2]), Elem<ST>::down(acc[i][j][4 * q + 3])};
                 *reinterpret_cast<T4*>(mine + (row * CH + ((n / E) ^ (row & 7))) * 16 + (n % E) * (int)sizeof(T)) = v;
             }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    T* const c = static_cast<T*>(g.c);
+    T* const c = static_cast<T*>(g.c) + (SPLIT ? (size_t)split * g.M * g.N : 0);
     const bool whole = g.ldc % E == 0 && (reinterpret_cast<uintptr_t>(c) & 15) == 0;
     constexpr int RPI = 64 / CH;                                         // rows per store instruction
 #pragma unroll 4
@@ -413,24 +416,64 @@ __global__ __launch_bounds__(WM * WN * 64) void matmul_fp8_kernel(const MatArgs 
     }
 }
 
-template <int TM, int TN, int WM, int WN, int DT>
+// the ranges' sums, in their order
+template <int DT>
+__global__ __launch_bounds__(256) void join_splits_kernel(const float* __restrict__ part, int splits, long long MN, int N, typename Elem<DT>::T* __restrict__ c, long long ldc) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < MN; i += (long long)gridDim.x * 256) {
+        float s = part[i];
+        for (int k = 1; k < splits; ++k) s += part[(size_t)k * MN + i];
+        const long long m = i / N;
+        c[m * ldc + (i - m * N)] = Elem<DT>::down(s);
+    }
+}
+
+// Into ranges of how many blocks (a multiple of four) the reduced axis is cut where there are few output tiles; Kb: not cut.  About one workgroup
+// per CU in all, at least eight blocks each, at most 16 ranges, and of those numbers the one with the least of: the tiles' time per block
+// (measured 0.4 us with 16-bit, 0.85 us with fp32 results) over the ranges, and for the ranges' fp32 sums a launch (4 us) and their way out and
+// back (8 bytes each at 4.6 TB/s).  300 x 520 x 8192: bf16 28.9 -> 14.5 us, fp32 57.4 -> 18.0; 200 x 4096 x 4096: bf16 17.7 us as it is and 21.0 cut in
+// four, fp32 32.5 -> 24.4.
+int split_chunk(bool f32, long long M, long long N, int Kb) {
+    const long long tiles = cnm_ceil_div_ll(M, 128) * cnm_ceil_div_ll(N, 128);
+    if (tiles > 128 || Kb < 16) return Kb;
+    const double per_block = f32 ? 0.85 : 0.4, join = 8.0 * (double)M * (double)N / 4.6e6;
+    int best = Kb;
+    double t = per_block * Kb;
+    for (int n = 2; n <= 16 && n <= 256 / tiles && n <= Kb / 8; ++n) {
+        const int chunk = ((Kb + n - 1) / n + 3) / 4 * 4, ranges = cnm_ceil_div(Kb, chunk);
+        const double tn = per_block * chunk + 4.0 + ranges * join;
+        if (tn < t) { t = tn; best = chunk; }
+    }
+    return best;
+}
+
+template <int TM, int TN, int WM, int WN, int DT, bool SPLIT = false>
 int launch_tiles(MatArgs g, hipStream_t stream) {
     g.tiles_m = cnm_ceil_div(g.M, TM); g.tiles_n = cnm_ceil_div(g.N, TN);
-    if (g.bshift) matmul_fp8_kernel<TM, TN, WM, WN, DT, true><<<g.tiles_m * g.tiles_n, WM * WN * 64, Mat<TM, TN, WM, WN, DT, true>::LDS, stream>>>(g);
-    else matmul_fp8_kernel<TM, TN, WM, WN, DT, false><<<g.tiles_m * g.tiles_n, WM * WN * 64, Mat<TM, TN, WM, WN, DT, false>::LDS, stream>>>(g);
+    const unsigned blocks = (unsigned)(g.tiles_m * g.tiles_n * (SPLIT ? g.splits : 1));
+    if (g.bshift) matmul_fp8_kernel<TM, TN, WM, WN, DT, true, SPLIT><<<blocks, WM * WN * 64, Mat<TM, TN, WM, WN, DT, true>::LDS, stream>>>(g);
+    else matmul_fp8_kernel<TM, TN, WM, WN, DT, false, SPLIT><<<blocks, WM * WN * 64, Mat<TM, TN, WM, WN, DT, false>::LDS, stream>>>(g);
     CNM_LAUNCH_CHECK();
     return CNM_OK;
 }
 
 template <int DT>
-int launch_matmul(const MatArgs& g, hipStream_t stream) {
+int launch_matmul(MatArgs g, float* ws, hipStream_t stream) {
     // 256 x 256 tiles (eight waves of 128 x 64, one workgroup per CU) from more tiles than half the CUs on; below that twice as many CUs
     // work on 128 x 128 tiles (four waves of 64 x 64, two workgroups per CU).  bf16, 4096 x 4096 x 8192 (256 / 1024 tiles): 117 us against
     // 166; 2048 x 2048 x 2048 (64 / 256 tiles): 25 us against 13.5.  fp32 results convert their operands on the way: 128 x 128 only
     // (64 accumulators per lane leave room for the bf16 fragments).
     if constexpr (DT != CNM_F32)
         if ((long long)cnm_ceil_div(g.M, 256) * cnm_ceil_div(g.N, 256) > 128) return launch_tiles<256, 256, 2, 4, DT>(g, stream);
-    return launch_tiles<128, 128, 2, 2, DT>(g, stream);
+    const int chunk = split_chunk(DT == CNM_F32, g.M, g.N, g.Kb);
+    if (chunk >= g.Kb) return launch_tiles<128, 128, 2, 2, DT>(g, stream);
+    MatArgs p = g;
+    p.c = ws; p.ldc = g.N; p.chunk = chunk; p.splits = cnm_ceil_div(g.Kb, chunk);
+    const int rc = launch_tiles<128, 128, 2, 2, DT, true>(p, stream);
+    if (rc != CNM_OK) return rc;
+    const long long MN = (long long)g.M * g.N, blocks = cnm_ceil_div_ll(MN, 256);
+    join_splits_kernel<DT><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, stream>>>(ws, p.splits, MN, g.N, static_cast<typename Elem<DT>::T*>(g.c), g.ldc);
+    CNM_LAUNCH_CHECK();
+    return CNM_OK;
 }
 
 // ------------------------------------------------------------------ few rows, or few columns
@@ -653,18 +696,32 @@ extern "C" int cnm_quantize_fp8(const void* x, int dtype, long long ldx, long lo
     return CNM_ERR_BAD_ARG;
 }
 
+extern "C" size_t cnm_matmul_fp8_workspace_bytes(int dtype, long long M, long long N, long long K) {
+    if (M <= FEW_ROWS || N <= 0 || K <= 0 || K > (1ll << 23)) return 0;
+    const int kb = (int)cnm_ceil_div_ll(K, QB), chunk = split_chunk(dtype == CNM_F32, M, N, kb);
+    return chunk < kb ? (size_t)cnm_ceil_div(kb, chunk) * (size_t)M * (size_t)N * sizeof(float) : 0;
+}
+// of either kind of result
+static size_t matmul_workspace(long long M, long long N, long long K) {
+    const size_t a = cnm_matmul_fp8_workspace_bytes(CNM_F32, M, N, K), b = cnm_matmul_fp8_workspace_bytes(CNM_BF16, M, N, K);
+    return a > b ? a : b;
+}
+
 extern "C" int cnm_matmul_fp8(const void* a, const void* a_scale, const void* b, const void* b_scale, int b_block_rows, void* c, int dtype,
-                              long long ldc, long long M, long long N, long long K, void* stream) {
+                              long long ldc, long long M, long long N, long long K, void* workspace, size_t workspace_bytes, void* stream) {
     CNM_REQUIRE(a && a_scale && b && b_scale && c && M > 0 && N > 0 && K > 0 && K % QB == 0 && ldc >= N, CNM_ERR_BAD_ARG);
     CNM_REQUIRE(b_block_rows == 1 || b_block_rows == QB, CNM_ERR_BAD_ARG);
     CNM_REQUIRE(((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0, CNM_ERR_BAD_ARG);
     CNM_REQUIRE(M < (1ll << 31) - 256 && N < (1ll << 31) - 256 && K <= (1ll << 23), CNM_ERR_BAD_SHAPE);   // 256 rows of an operand are one 32-bit buffer range
     CNM_REQUIRE(cnm_ceil_div_ll(M, 16) * cnm_ceil_div_ll(N, 16) < (1ll << 31), CNM_ERR_BAD_SHAPE);
     MatArgs g = {static_cast<const unsigned char*>(a), static_cast<const unsigned char*>(a_scale), static_cast<const unsigned char*>(b), static_cast<const unsigned char*>(b_scale),
-                 c, (int)M, (int)N, (int)(K / QB), b_block_rows == 1 ? 0 : 7, ldc, 0, 0};
+                 c, (int)M, (int)N, (int)(K / QB), b_block_rows == 1 ? 0 : 7, ldc, 0, 0, 1, 0};
+    const size_t need = cnm_matmul_fp8_workspace_bytes(dtype, M, N, K);
+    CNM_REQUIRE(!need || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0), CNM_ERR_WORKSPACE);
+    float* const ws = static_cast<float*>(workspace);
     const StreamArgs f = {a, 0, g.sa, g.b, g.sb, c, ldc, g.M, g.N, (int)K, g.Kb, g.bshift};
     const hipStream_t st = cnm_stream(stream);
-#define CNM_M(DT) return M <= FEW_ROWS ? launch_few_rows<DT>(f, st) : launch_matmul<DT>(g, st)
+#define CNM_M(DT) return M <= FEW_ROWS ? launch_few_rows<DT>(f, st) : launch_matmul<DT>(g, ws, st)
     switch (dtype) {
         case CNM_F32: CNM_M(CNM_F32);
         case CNM_F16: CNM_M(CNM_F16);
@@ -698,7 +755,9 @@ extern "C" size_t cnm_linear_fp8_keep_bytes(long long M, long long N, long long 
 }
 extern "C" size_t cnm_linear_fp8_train_workspace_bytes(long long M, long long N, long long K) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    const size_t fwd = fp8_bytes(M, K, false) + fp8_bytes(N, K, true), bwd = fp8_bytes(M, N, false) + fp8_bytes(N, M, false);
+    const auto up = [](long long n) { return cnm_ceil_div_ll(n, QB) * QB; };
+    const size_t dx = matmul_workspace(M, K, up(N)), dw = matmul_workspace(N, K, up(M));
+    const size_t fwd = fp8_bytes(M, K, false) + fp8_bytes(N, K, true) + matmul_workspace(M, N, up(K)), bwd = fp8_bytes(M, N, false) + fp8_bytes(N, M, false) + (dx > dw ? dx : dw);
     return fwd > bwd ? fwd : bwd;
 }
 
@@ -716,7 +775,7 @@ extern "C" int cnm_linear_fp8_forward(const void* x, int x_dtype, long long ldx,
     if (need_dw) xt = fp8_take(kp, K, M, false);
     int rc = cnm_quantize_fp8(w, w_dtype, ldw, N, K, QB, wq.q, wq.s, wt.q, wt.s, stream);
     if (rc == CNM_OK) rc = cnm_quantize_fp8(x, x_dtype, ldx, M, K, 1, xq.q, xq.s, xt.q, xt.s, stream);
-    return rc != CNM_OK ? rc : cnm_matmul_fp8(xq.q, xq.s, wq.q, wq.s, QB, y, x_dtype, N, M, N, cnm_ceil_div_ll(K, QB) * QB, stream);
+    return rc != CNM_OK ? rc : cnm_matmul_fp8(xq.q, xq.s, wq.q, wq.s, QB, y, x_dtype, N, M, N, cnm_ceil_div_ll(K, QB) * QB, ws, workspace_bytes - (ws - static_cast<unsigned char*>(workspace)), stream);
 }
 
 extern "C" int cnm_linear_fp8_backward(const void* dy, int dy_dtype, long long lddy, const void* keep, size_t keep_bytes, void* dx, int dx_dtype, void* dw, int dw_dtype,
@@ -732,16 +791,16 @@ extern "C" int cnm_linear_fp8_backward(const void* dy, int dy_dtype, long long l
     if (kept_dw) xt = fp8_take(kp, K, M, false);
     if (dx) dyq = fp8_take(ws, M, N, false);
     if (dw) dyt = fp8_take(ws, N, M, false);
+    const size_t left = workspace_bytes - (ws - static_cast<unsigned char*>(workspace));
     int rc = cnm_quantize_fp8(dy, dy_dtype, lddy, M, N, 1, dyq.q, dyq.s, dyt.q, dyt.s, stream);
-    if (rc == CNM_OK && dx) rc = cnm_matmul_fp8(dyq.q, dyq.s, wt.q, wt.s, QB, dx, dx_dtype, K, M, K, cnm_ceil_div_ll(N, QB) * QB, stream);
-    if (rc == CNM_OK && dw) rc = cnm_matmul_fp8(dyt.q, dyt.s, xt.q, xt.s, 1, dw, dw_dtype, K, N, K, cnm_ceil_div_ll(M, QB) * QB, stream);
+    if (rc == CNM_OK && dx) rc = cnm_matmul_fp8(dyq.q, dyq.s, wt.q, wt.s, QB, dx, dx_dtype, K, M, K, cnm_ceil_div_ll(N, QB) * QB, ws, left, stream);
+    if (rc == CNM_OK && dw) rc = cnm_matmul_fp8(dyt.q, dyt.s, xt.q, xt.s, 1, dw, dw_dtype, K, N, K, cnm_ceil_div_ll(M, QB) * QB, ws, left, stream);
     return rc;
 }
 
 extern "C" size_t cnm_linear_fp8_workspace_bytes(long long M, long long N, long long K) {
     if (M <= 0 || N <= 0 || K <= 0 || M <= 16 || N <= FEW_COLS) return 0;
-    const size_t kb = (size_t)cnm_ceil_div_ll(K, QB);
-    return (size_t)M * kb * (QB + 1);
+    return fp8_bytes(M, K, false) + matmul_workspace(M, N, cnm_ceil_div_ll(K, QB) * QB);
 }
 
 extern "C" int cnm_linear_fp8(const void* x, int dtype, long long ldx, const void* w, const void* w_scale, void* y, long long ldy,
@@ -753,10 +812,10 @@ extern "C" int cnm_linear_fp8(const void* x, int dtype, long long ldx, const voi
     const long long kb = cnm_ceil_div_ll(K, QB);
     if (need) {                                                          // quantise, then multiply
         CNM_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, CNM_ERR_WORKSPACE);
-        unsigned char* const q = static_cast<unsigned char*>(workspace);
-        unsigned char* const s = q + (size_t)M * kb * QB;
-        const int rc = cnm_quantize_fp8(x, dtype, ldx, M, K, 1, q, s, nullptr, nullptr, stream);
-        return rc != CNM_OK ? rc : cnm_matmul_fp8(q, s, w, w_scale, QB, y, dtype, ldy, M, N, kb * QB, stream);
+        unsigned char* at = static_cast<unsigned char*>(workspace);
+        const Fp8 q = fp8_take(at, M, K, false);
+        const int rc = cnm_quantize_fp8(x, dtype, ldx, M, K, 1, q.q, q.s, nullptr, nullptr, stream);
+        return rc != CNM_OK ? rc : cnm_matmul_fp8(q.q, q.s, w, w_scale, QB, y, dtype, ldy, M, N, kb * QB, at, need, stream);
     }
     const StreamArgs f = {x, ldx, nullptr, static_cast<const unsigned char*>(w), static_cast<const unsigned char*>(w_scale), y, ldy, (int)M, (int)N, (int)K, (int)kb, 7};
     const hipStream_t st = cnm_stream(stream);

@@ -855,8 +855,11 @@ def matmul_fp8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
     M, N, K = a.shape[0], b.shape[0], a.shape[1]
     c = torch.empty(M, N, device=a.device, dtype=dtype)
     if M and N:
+        lib = _lib.load()
+        n = lib.cnm_matmul_fp8_workspace_bytes(DTYPES[dtype], M, N, K)
+        ws = torch.empty(n, device=a.device, dtype=torch.uint8) if n else None
         with _on(a.device):
-            _lib.check(_lib.load().cnm_matmul_fp8(_p(a), _p(a_scale), _p(b), _p(b_scale), bb, _p(c), DTYPES[dtype], N, M, N, K, _raw_stream(a.device)))
+            _lib.check(lib.cnm_matmul_fp8(_p(a), _p(a_scale), _p(b), _p(b_scale), bb, _p(c), DTYPES[dtype], N, M, N, K, _p(ws), n, _raw_stream(a.device)))
     return c
 
 

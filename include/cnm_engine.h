@@ -869,9 +869,13 @@ int cnm_refinenet_forward_multi_cpu(const cnm_layer_weights* weights, float idep
 int cnm_quantize_fp8(const void* x, int dtype, long long ldx, long long rows, long long cols, int block_rows,
                      void* q, void* scale, void* q_t, void* scale_t, void* stream);
 /* c [M][ldc] of dtype = a b^T: a [M][K], b [N][K] as above (K a multiple of 128, at most 2^23; a, b on 16 bytes), a_scale [M][K/128],
- * b_scale [N][K/128] (b_block_rows 1) or [ceil(N/128)][K/128] (128).  fp32 accumulation, one rounding.  Any M, N >= 1; ldc >= N. */
+ * b_scale [N][K/128] (b_block_rows 1) or [ceil(N/128)][K/128] (128).  fp32 accumulation, one rounding (with 16-bit
+ * results the matrix instruction cuts products off at 2^-13 of the largest of eight neighbours; fp32 results are exact products in fp32 sums).
+ * Any M, N >= 1; ldc >= N.  workspace: cnm_matmul_fp8_workspace_bytes on 16 bytes (0 but where few output tiles share a long reduced axis),
+ * contents irrelevant. */
+size_t cnm_matmul_fp8_workspace_bytes(int dtype, long long M, long long N, long long K);
 int cnm_matmul_fp8(const void* a, const void* a_scale, const void* b, const void* b_scale, int b_block_rows, void* c, int dtype,
-                   long long ldc, long long M, long long N, long long K, void* stream);
+                   long long ldc, long long M, long long N, long long K, void* workspace, size_t workspace_bytes, void* stream);
 /* y [M][ldy] = x w^T for inference: x [M][ldx] of dtype (ldx >= K, any alignment), quantised here (block_rows 1), w [N][K padded to 128] and w_scale
  * as cnm_quantize_fp8 makes them with block_rows 128; y of x's dtype.  workspace: cnm_linear_fp8_workspace_bytes (0 for few rows or columns,
  * which are quantised on the way) on 16 bytes, contents irrelevant. */

@@ -28,7 +28,7 @@ def test_quantize_entry_refuses():
 
 def test_matmul_entry_refuses():
     f = _lib.load().cnm_matmul_fp8
-    ok = [4096, 64, 8192, 64, 1, 4096, 0, 64, 8, 64, 256, 0]
+    ok = [4096, 64, 8192, 64, 1, 4096, 0, 64, 8, 64, 256, 0, 0, 0]
     def with_(**kw):
         a = list(ok)
         for k, v in kw.items():
@@ -43,12 +43,15 @@ def test_matmul_entry_refuses():
     assert with_(_10=200) == -1 and with_(_10=0) == -1                  # K not in blocks
     assert with_(_10=(1 << 23) + 128) == -2
     assert with_(_0=4100) == -1
+    n = _lib.load().cnm_matmul_fp8_workspace_bytes(0, 200, 300, 8192)         # few tiles, long reduction: cut into ranges
+    assert n > 0 and n % (200 * 300 * 4) == 0 and _lib.load().cnm_matmul_fp8_workspace_bytes(0, 64, 300, 8192) == 0 and _lib.load().cnm_matmul_fp8_workspace_bytes(0, 4096, 4096, 4096) == 0
+    assert with_(_7=300, _8=200, _9=300, _10=8192) == -5 and with_(_7=300, _8=200, _9=300, _10=8192, _11=4096, _12=n - 1) == -5
 
 
 def test_linear_entry_refuses():
     lib = _lib.load()
     n = lib.cnm_linear_fp8_workspace_bytes(100, 300, 200)
-    assert n == 100 * 2 * 129 and lib.cnm_linear_fp8_workspace_bytes(16, 300, 200) == 0 and lib.cnm_linear_fp8_workspace_bytes(1000, 64, 200) == 0
+    assert n == (100 * 2 * 129 + 15) // 16 * 16 and lib.cnm_linear_fp8_workspace_bytes(16, 300, 200) == 0 and lib.cnm_linear_fp8_workspace_bytes(1000, 64, 200) == 0
     ok = [64, 0, 200, 4096, 64, 4096, 300, 100, 300, 200, 4096, n, 0]
     def with_(**kw):
         a = list(ok)

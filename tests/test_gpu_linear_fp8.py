@@ -107,6 +107,9 @@ def test_product_long_reduction(block_rows):
     product(130, 140, 9000, torch.float32, block_rows, 5)
     product(129, 257, 8320, torch.bfloat16, block_rows, 6)
     product(20, 50, 9000, torch.float16, block_rows, 7)
+    product(200, 131, 2100, torch.float32, block_rows, 8)               # cut into ranges: uneven last one, odd row length
+    product(100, 300, 16400, torch.float16, block_rows, 9)
+    product(260, 24, 4224, torch.bfloat16, block_rows, 10)
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
@@ -147,7 +150,7 @@ def test_product_leaves_the_gap_between_rows():
     for M, N in ((5, 33), (130, 130)):
         a, b = ops.quantize_fp8(data(M, 128, torch.float32, 1).to(DEV)), ops.quantize_fp8(data(N, 128, torch.float32, 2).to(DEV))
         c = torch.full((M + 3, N + 7), 5.0, device=DEV)
-        _lib.check(lib.cnm_matmul_fp8(a[0].data_ptr(), a[1].data_ptr(), b[0].data_ptr(), b[1].data_ptr(), 1, c.data_ptr(), 0, N + 7, M, N, 128, torch.cuda.current_stream().cuda_stream))
+        _lib.check(lib.cnm_matmul_fp8(a[0].data_ptr(), a[1].data_ptr(), b[0].data_ptr(), b[1].data_ptr(), 1, c.data_ptr(), 0, N + 7, M, N, 128, None, 0, torch.cuda.current_stream().cuda_stream))
         assert torch.equal(c[:M, :N], ops.matmul_fp8(*a, *b, dtype=torch.float32))
         assert bool((c[M:] == 5.0).all()) and bool((c[:, N:] == 5.0).all())
 
@@ -242,7 +245,7 @@ def train_case(M, N, K, xt, wt, seed):
     return x, w, dy, ((X, W), (D, W.t()), (Dt, Xt))
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 40, 300), (5, 129, 64), (130, 65, 257), (300, 200, 520), (1000, 96, 128)])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 40, 300), (5, 129, 64), (130, 65, 257), (300, 200, 520), (1000, 96, 128), (3001, 70, 66)])
 @pytest.mark.parametrize("xt,wt", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16)])
 def test_linear_training(M, N, K, xt, wt):
     x, w, dy, pairs = train_case(M, N, K, xt, wt, M + N)
