@@ -15,7 +15,9 @@ SOURCES = ["planesweep.hip", "conv_mfma.hip", "conv_winograd.hip", "conv_winogra
 HOST_SOURCES = ["host_twins.cpp"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 HOSTCXX = os.environ.get("CXX", "g++")
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"]
+# no packed fp32 instructions (v_pk_add / mul / fma_f32): hipcc makes them from scalar float code by itself, and some of their forms have
+# given wrong results now and then on this hardware
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # per-file extras: the plane sweep's blend must stay on full-rate scalar v_fma_f32 (the SLP vectoriser would
 # pack it into half-rate v_pk_fma_f32 plus the moves that feed them)
 # the staged 36-point kernel lives at the register limit (256 VGPRs, 106 SGPRs + spill lanes): the greedy allocator's class-priority
@@ -25,16 +27,12 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-u
 # the fp16 heads (half_ops.hip) multiply half inputs by fp32 weights: left alone, the SLP vectoriser packs the products into v_pk_fma_f32 (which
 # issues as two FMAs) behind 240 v_cvt_f32_f16 per channel group; without it the compiler selects v_fma_mix_f32 (conversion folded in): 656
 # instead of 896 VALU instructions per group and lane.
-# no packed fp32 instructions (v_pk_add / mul / fma_f32): hipcc makes them from scalar float code by itself, and some of their forms have
-# given wrong results now and then on this hardware
-NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-FILE_FLAGS = {"linear_fp8.hip": NO_PACKED_F32, "distill.hip": NO_PACKED_F32,
-              "planesweep.hip": ["-fno-slp-vectorize"],
+FILE_FLAGS = {"planesweep.hip": ["-fno-slp-vectorize"],
               "half_ops.hip": ["-fno-slp-vectorize"],
               "conv_winograd4s.hip": ["-mllvm", "-greedy-regclass-priority-trumps-globalness=1", "-mllvm", "-disable-machine-licm"],
               "conv_rows_staged.hip": ["-mllvm", "-greedy-regclass-priority-trumps-globalness=1", "-mllvm", "-disable-machine-licm"]}   # 37 instead of 60 spilled SGPRs
 if os.environ.get("CNM_NO_FILE_FLAGS") == "1":
-    FILE_FLAGS = {"linear_fp8.hip": NO_PACKED_F32, "distill.hip": NO_PACKED_F32, "planesweep.hip": ["-fno-slp-vectorize"], "half_ops.hip": ["-fno-slp-vectorize"]}
+    FILE_FLAGS = {"planesweep.hip": ["-fno-slp-vectorize"], "half_ops.hip": ["-fno-slp-vectorize"]}
 
 
 def _stale(target, deps):
