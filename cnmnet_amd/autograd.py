@@ -782,7 +782,16 @@ class LinearFP8(torch.autograd.Function):
 
 def linear_fp8(x, weight):
     """x [..., K], weight [N, K] (float32 / float16 / bfloat16, each its own) -> [..., N] of x's type, through 8-bit products both ways."""
+    if not torch.is_grad_enabled():                                      # (a Function is told of inputs that require gradients even then)
+        x, weight = x.detach(), weight.detach()
     return LinearFP8.apply(x, weight)
+
+
+def top_logits_distill(logits, top_idx, top_logits, top_lse=None, weight=None, temperature=1.0, dim=-1, reduction="mean"):
+    """ops.top_logits_distill with a gradient to the logits."""
+    if not torch.is_grad_enabled():
+        return ops.top_logits_distill(logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction)
+    return TopLogitsDistill.apply(logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction)
 
 
 class TopLogitsDistill(torch.autograd.Function):

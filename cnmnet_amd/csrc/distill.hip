@@ -23,6 +23,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int KMAX = 256;                    // entries per row
 constexpr int VMAX = 1 << 20;                // classes per row: one LDS bit each (128 KB)
 constexpr size_t LDS_BYTES = 160 * 1024;
+constexpr float TMIN = 1e-37f;                // smallest temperature: log2(e) / T is finite
 constexpr double LOG2E_D = 1.4426950408889634074, LN2_D = 0.69314718055994530942;
 
 template <int DT> struct Elem;
@@ -1050,7 +1051,7 @@ extern "C" size_t cnm_top_logits_workspace_bytes(int dtype, long long rows, int 
 
 extern "C" int cnm_top_logits(const void* z, int dtype, long long ldz, float temperature, void* values, int* indices, float* lse, void* workspace, size_t workspace_bytes,
                               long long rows, int classes, int entries, long long inner, void* stream) {
-    CNM_REQUIRE(z && values && indices && lse && rows > 0 && classes > 0 && inner > 0 && temperature > 0.f && temperature < __builtin_huge_valf(), CNM_ERR_BAD_ARG);
+    CNM_REQUIRE(z && values && indices && lse && rows > 0 && classes > 0 && inner > 0 && temperature >= TMIN && temperature < __builtin_huge_valf(), CNM_ERR_BAD_ARG);
     CNM_REQUIRE(entries > 0 && entries <= classes && entries <= (inner > 1 ? TOP_PLANES_KMAX : KMAX) && rows % inner == 0 && (inner > 1 || ldz >= classes), CNM_ERR_BAD_ARG);
     CNM_REQUIRE(rows < (1ll << 30) / 64 * 64 && classes <= VMAX && (inner > 1 || rows * cnm_ceil_div(classes, 4096) < (1ll << 31)), CNM_ERR_BAD_SHAPE);
     const size_t need = cnm_top_logits_workspace_bytes(dtype, rows, classes, entries, inner);
@@ -1079,7 +1080,7 @@ extern "C" int cnm_distill(const void* z, int dtype, long long ldz, const void* 
                            int reduction, float* loss, void* dz, double* workspace, size_t workspace_doubles, int workspace_ready,
                            long long rows, int classes, int entries, long long inner, void* stream) {
     CNM_REQUIRE(z && indices && entry_logits && rows > 0 && classes > 0 && entries > 0 && inner > 0 && (loss || dz), CNM_ERR_BAD_ARG);
-    CNM_REQUIRE(temperature > 0.f && temperature < __builtin_huge_valf() && reduction >= 0 && reduction <= 2 && entries <= KMAX, CNM_ERR_BAD_ARG);
+    CNM_REQUIRE(temperature >= TMIN && temperature < __builtin_huge_valf() && reduction >= 0 && reduction <= 2 && entries <= KMAX, CNM_ERR_BAD_ARG);
     CNM_REQUIRE(rows % inner == 0 && (inner > 1 || ldz >= classes) && dtype >= CNM_F32 && dtype <= CNM_BF16 && entry_dtype >= CNM_F32 && entry_dtype <= CNM_BF16, CNM_ERR_BAD_ARG);
     CNM_REQUIRE(!grad_out_rows || (grad_out && reduction == 0), CNM_ERR_BAD_ARG);
     CNM_REQUIRE(!workspace_ready || !loss, CNM_ERR_BAD_ARG);

@@ -131,5 +131,5 @@ class TopLogitsDistillLoss(nn.Module):
         self.temperature, self.dim, self.reduction = temperature, dim, reduction
 
     def forward(self, logits, top_idx, top_logits, top_lse=None, weight=None):
-        from ..autograd import TopLogitsDistill
-        return TopLogitsDistill.apply(logits, top_idx, top_logits, top_lse, weight, self.temperature, self.dim, self.reduction)
+        from ..autograd import top_logits_distill
+        return top_logits_distill(logits, top_idx, top_logits, top_lse, weight, self.temperature, self.dim, self.reduction)

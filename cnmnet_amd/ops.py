@@ -925,8 +925,8 @@ class _Classes:
 
 def _temperature(t):
     t = float(t)
-    if not 0.0 < t < float("inf"):
-        raise _lib.EngineError("temperature must be positive and finite; got %r" % t)
+    if not 1e-37 <= t < 3.4e38:
+        raise _lib.EngineError("temperature must lie between 1e-37 and float32's largest value; got %r" % t)
     return t
 
 

@@ -900,6 +900,8 @@ int cnm_linear_fp8_backward(const void* dy, int dy_dtype, long long lddy, const 
  * (inner > 1: e.g. [B, planes, H, W], inner = H W; ldz is ignored).  Entries, values, indices and per-row numbers follow the same order
  * ([rows][entries] or [rows / inner][entries][inner]; [rows]).
  *
+ * temperature: at least 1e-37, finite.
+ *
  * cnm_top_logits: the `entries` largest logits per row in descending order (ties: the lower class first; NaN above everything, -0 equal to
  * +0), their classes, and lse = log sum exp(z / temperature).  entries <= classes, <= cnm_distill_max_entries() (inner = 1) or
  * cnm_top_logits_planes_max_entries() (inner > 1); classes <= cnm_distill_max_classes().  workspace: cnm_top_logits_workspace_bytes on 8 bytes

@@ -102,7 +102,7 @@ def test_top_and_distill_entries_refuse():
         return lib.cnm_top_logits(*a)
     for i in (0, 4, 5, 6):
         assert t(**{"_%d" % i: 0}) == -1
-    assert t(_3=0.0) == -1 and t(_3=float("inf")) == -1 and t(_3=float("nan")) == -1
+    assert t(_3=0.0) == -1 and t(_3=1e-38) == -1 and t(_3=float("inf")) == -1 and t(_3=float("nan")) == -1
     assert t(_11=101) == -1 and t(_11=0) == -1 and t(_10=1000, _2=1000, _11=257) == -1
     assert t(_2=99) == -1 and t(_12=3) == -1                            # row stride; rows not a multiple of inner
     assert t(_12=4, _11=17) == -1                                        # planes: at most 16
