@@ -78,7 +78,7 @@ __global__ __launch_bounds__(512) void quantize_kernel(const typename Elem<DT>::
                                                        unsigned char* __restrict__ qt, unsigned char* __restrict__ st) {
     constexpr int NR = 4;                                                // rows per thread
     __shared__ float cmax[8][QB];
-    __shared__ __attribute__((aligned(16))) unsigned char tile[QB][QB + 16];
+    __shared__ __attribute__((aligned(16))) unsigned char tile[QB][QB];  // transposed; a row's 16-byte chunks permuted by (row >> 3) & 7: the rows that a wave writes at once are multiples of eight apart
     __shared__ float bmax[8];
     const int tid = threadIdx.x, lc = tid & 15, lr = tid >> 4;
     const int cb = blockIdx.x % Cb, rb = blockIdx.x / Cb;
@@ -161,13 +161,13 @@ __global__ __launch_bounds__(512) void quantize_kernel(const typename Elem<DT>::
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-        *reinterpret_cast<unsigned*>(&tile[lc * 8 + j][lr * NR]) = pack4(v[0][j] * k8[j], v[1][j] * k8[j], v[2][j] * k8[j], v[3][j] * k8[j]);
+        *reinterpret_cast<unsigned*>(&tile[lc * 8 + j][(lr * NR) ^ (16 * (lc & 7))]) = pack4(v[0][j] * k8[j], v[1][j] * k8[j], v[2][j] * k8[j], v[3][j] * k8[j]);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {                                        // 8 lanes x 16 bytes = one transposed row of the tile
         const int c = i * 64 + (tid >> 3), l = tid & 7;
         if (cb * QB + c < C)
-            *reinterpret_cast<uint4*>(qt + (size_t)(cb * QB + c) * ((size_t)Rb * QB) + (size_t)rb * QB + l * 16) = *reinterpret_cast<const uint4*>(&tile[c][l * 16]);
+            *reinterpret_cast<uint4*>(qt + (size_t)(cb * QB + c) * ((size_t)Rb * QB) + (size_t)rb * QB + l * 16) = *reinterpret_cast<const uint4*>(&tile[c][16 * (l ^ ((c >> 3) & 7))]);
     }
 }
 

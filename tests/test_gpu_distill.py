@@ -400,3 +400,45 @@ def test_distill_chain_as_it_is_used():
     for got, a, b in ((x.grad, bf.Operand(dz, 1), bf.Operand(ws, 128).t()), (w.grad, bf.Operand(dz.t().contiguous(), 1), bf.Operand(feat.t().contiguous(), 1))):
         want = bf.product(a, b)
         assert bool(((got.double().cpu() - want).abs() <= bf.product_bound(a, b, want, torch.float32)).all())
+
+
+@pytest.mark.parametrize("planes", [False, True])
+def test_offsets_beyond_32_bits(planes):
+    """More than 2^32 logits: the last rows give what the same rows give alone."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    K, T = 5, 2.0
+    if planes:
+        z = torch.empty(9, 500, 1000000, device=DEV, dtype=torch.float16)
+        tail = torch.randn(1, 500, 1000000, device=DEV, generator=g, dtype=torch.float16)
+        z[:-1] = 0.25
+        z[-1:] = tail
+        pick = lambda t: t[-1:]
+    else:
+        z = torch.empty(140000, 32768, device=DEV, dtype=torch.bfloat16)
+        tail = torch.randn(300, 32768, device=DEV, generator=g, dtype=torch.bfloat16)
+        z[:-300] = 0.25
+        z[-300:] = tail
+        pick = lambda t: t[-300:]
+    val, idx, lse = ops.top_logits(z, K, dim=1, temperature=T)
+    v, i, l = ops.top_logits(tail, K, dim=1, temperature=T)
+    assert torch.equal(pick(val), v) and torch.equal(pick(idx), i) and torch.equal(pick(lse), l)
+    assert torch.equal(idx[0].reshape(K, -1)[:, 0].cpu(), torch.arange(K, dtype=torch.int32))
+    loss, dz = ops.top_logits_distill(z, idx, val - 1, lse, temperature=T, dim=1, reduction="none", grad=True)
+    lt, dt = ops.top_logits_distill(tail, i, v - 1, l, temperature=T, dim=1, reduction="none", grad=True)
+    assert torch.equal(pick(loss), lt) and torch.equal(pick(dz), dt)
+    assert bool((loss[:-300] == loss.reshape(-1)[0]).all()) if not planes else bool((loss[:-1] == loss.reshape(-1)[0]).all())
+
+
+def test_distill_on_two_streams_at_once():
+    z, idx, val, lse, w = (dev(t) for t in make(300, 3000, 9, torch.float32, 6, True, True, True, 2.0))
+    want = ops.top_logits_distill(z, idx, val, lse, w, temperature=2.0, grad=True), ops.top_logits_distill(z[:3], idx[:3], val[:3], lse[:3], temperature=2.0, grad=True)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(8):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(ops.top_logits_distill(z, idx, val, lse, w, temperature=2.0, grad=True) if i == 0
+                              else ops.top_logits_distill(z[:3], idx[:3], val[:3], lse[:3], temperature=2.0, grad=True))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i in range(2) for r in got[i] for a, b in zip(r, want[i]))

@@ -346,3 +346,41 @@ def test_linear_training_step_captured():
         ye = autograd.linear_fp8(xe, we)
         want = torch.autograd.grad(ye, (xe, we), ds)
         assert torch.equal(y, ye) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_linear_offsets_beyond_32_bits():
+    """More than 2^32 elements of x: the last rows are those of the same rows alone (within the product's bound of float64)."""
+    M, K, N = 530000, 8192, 160
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.empty(M, K, device=DEV, dtype=torch.bfloat16)
+    x[:1000].zero_()
+    x[-300:] = torch.randn(300, K, device=DEV, generator=g)
+    x[1000:-300] = 0.5
+    w = torch.randn(N, K, device=DEV, generator=g) / 90
+    q, s = ops.pack_linear_fp8(w)
+    y = ops.linear_fp8(x, q, s)
+    A, B = bf.Operand(x[-300:].cpu(), 1), bf.Operand(w.cpu(), 128)
+    want = bf.product(A, B)
+    assert bool(((y[-300:].double().cpu() - want).abs() <= bf.product_bound(A, B, want, torch.bfloat16)).all())
+    assert bool((y[:1000] == 0).all()) and bool((y[1000:-300] == y[1000]).all())
+    qx = ops.quantize_fp8(x, 1, transposed=True)
+    tail = ops.quantize_fp8(x[-300:])
+    assert torch.equal(qx[0][-300:].view(torch.uint8), tail[0].view(torch.uint8)) and torch.equal(qx[1][-300:].view(torch.uint8), tail[1].view(torch.uint8))
+    last = (M // 128) * 128                                              # the last block of rows, transposed
+    qt = ops.quantize_fp8(x[last:].t().contiguous())
+    assert torch.equal(qx[2][:, last:].view(torch.uint8), qt[0].view(torch.uint8)) and torch.equal(qx[3][:, -1:].view(torch.uint8), qt[1].view(torch.uint8))
+
+
+def test_two_streams_at_once():
+    x, w = data(700, 640, torch.bfloat16, 1).to(DEV), data(300, 640, torch.float32, 2).to(DEV)
+    q, s = ops.pack_linear_fp8(w)
+    want = ops.linear_fp8(x, q, s), ops.linear_fp8(x[:20], q, s)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(ops.linear_fp8(x if i == 0 else x[:20], q, s))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
