@@ -309,7 +309,7 @@ __device__ inline DistillRow finish_row(const DistillArgs& a, size_t r, Lse rest
 }
 
 // NT threads per row (MODE ROW) or segment of a row, which they hold in registers (NV vectors of 16 bytes each): z is read once, the gradient
-// written once.  LDS: one bit per class (named by an entry), the entries.
+// written once.  LDS: one bit per class (named by an entry), one byte (by which), the entries.
 // A row that no workgroup can hold, or one of few, is cut into segments: statistics of each (SEG_STATS), the row's numbers (distill_join_kernel),
 // gradients of each (SEG_GRAD), the second reading from the caches.
 enum { ROW, SEG_STATS, SEG_GRAD };
@@ -321,7 +321,8 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 512 && NV == 8 ? 6 : 1) 
     __shared__ Entries entries[RPB];
     const int sub = NT == 64 ? threadIdx.x >> 6 : 0, t = NT == 64 ? threadIdx.x & 63 : threadIdx.x;
     const int nw = (a.seglen + 31) / 32;
-    unsigned* const bits = lds_words + sub * nw;
+    unsigned* const bits = lds_words + sub * 9 * nw;                     // [nw], then a byte per class: the entry that names it, written where a bit is set
+    unsigned char* const slot = reinterpret_cast<unsigned char*>(bits + nw);
     Entries& e = entries[sub];
     float go = 1.f;
     if (a.go && !a.go_rows) {
@@ -393,38 +394,46 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 512 && NV == 8 ? 6 : 1) 
         row_sync<NT>();
     }
     if (!a.dz) return;
-    if (t < 64) join_entries(e, a.K, lane);
+    if (t < 64) {                                                        // the named classes' gradients, each once, and which class each belongs to
+        join_entries(e, a.K, lane);
+        const DistillRow w = e.row;
+        const float B = w.B * go;
+        for (int k = lane; k < a.K; k += 64) {
+            const int i = e.idx[k] - v0;
+            if (e.idx[k] >= 0 && i >= 0 && i < n) {
+                slot[i] = (unsigned char)k;
+                // (a named class may lie far above the unnamed ones: its own exponent against the whole row's)
+                e.p[k] = B == 0.f ? 0.f : B * (exp2_((e.z[k] - w.oall) * c) * w.inv - e.p[k]);
+            }
+        }
+    }
     row_sync<NT>();
-    const DistillRow w = e.row;
-    const float A = w.A * go, B = w.B * go;
-    const bool zero = B == 0.f;                                          // rows that count for nothing: zeros, whatever the logits hold
+    const float A = e.row.A * go, orest = e.row.orest;
+    const bool zero = e.row.B * go == 0.f;                               // rows that count for nothing: zeros, whatever the logits hold
     T* const dz = static_cast<T*>(a.dz) + r * a.V + v0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int at = (i * NT + t) * E;
         if (at < n) {
             x[i].hold();
-            T g[E];
+            float g[E];
 #pragma unroll
-            for (int j = 0; j < E; ++j) g[j] = (T)(A * exp2_((x[i].get(j) - w.orest) * c));
+            for (int j = 0; j < E; ++j) g[j] = A * exp2_((x[i].get(j) - orest) * c);
             if (zero) {
 #pragma unroll
-                for (int j = 0; j < E; ++j) g[j] = (T)0.f;
-            } else if (b[i]) {
-                for (int k = 0; k < a.K; ++k) {                          // few classes are named: look up whose
-                    const int j = e.idx[k] - v0 - at;
-                    if (e.idx[k] >= 0 && j >= 0 && j < E) {
-                        // a named class may lie far above the unnamed ones: its own exponent against the whole row's
-                        const T q = (T)(B * (exp2_((e.z[k] - w.oall) * c) * w.inv - e.p[k]));
-#pragma unroll
-                        for (int jj = 0; jj < E; ++jj) g[jj] = jj == j ? q : g[jj];
-                    }
-                }
+                for (int j = 0; j < E; ++j) g[j] = 0.f;
             }
-            if (at + E <= n) __builtin_memcpy(dz + at, g, 16);
+            if (b[i]) {
+#pragma unroll
+                for (int j = 0; j < E; ++j) if (b[i] >> j & 1u) g[j] = e.p[slot[at + j]];
+            }
+            T out[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j) out[j] = (T)g[j];
+            if (at + E <= n) __builtin_memcpy(dz + at, out, 16);
             else {
 #pragma unroll
-                for (int j = 0; j < E; ++j) if (at + j < n) dz[at + j] = g[j];
+                for (int j = 0; j < E; ++j) if (at + j < n) dz[at + j] = out[j];
             }
         }
     }
@@ -650,7 +659,7 @@ void launch_rows(const DistillArgs& a, hipStream_t stream) {
     constexpr int E = 16 / (int)sizeof(typename Elem<DT>::T);
     const int vecs = a.seglen / E;
     const unsigned units = (unsigned)(a.rows * a.segments);
-    const size_t lds = (size_t)((a.seglen + 31) / 32) * 4;
+    const size_t lds = (size_t)((a.seglen + 31) / 32) * 4 * 9;           // a bit and a byte per class
     if (vecs <= 64) distill_rows_kernel<DT, 64, 1, MODE><<<(units + 3) / 4, 256, 4 * lds, stream>>>(a);
     else if (vecs <= 256) distill_rows_kernel<DT, 64, 4, MODE><<<(units + 3) / 4, 256, 4 * lds, stream>>>(a);
     else if (vecs <= 512) distill_rows_kernel<DT, 256, 2, MODE><<<units, 256, lds, stream>>>(a);
@@ -720,6 +729,8 @@ struct TopShared {
     unsigned hist[256];
     unsigned sel[4];                                                     // digit, rank left within it, its count, output cursor
     float shf[32];
+    unsigned nhits;
+    int hits[CAND];                                                      // vectors with a number above the bound
     u64 cand[CAND];
 };
 template <int NT>
@@ -865,18 +876,26 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 256 && NV == 16 ? 4 : 1)
     const float low = kth_bound<NT>(m, a.K, sh.shf);
     if (a.segments == 1) { if (t == 0) a.lse[r] = lse_value(l, a.T); }
     else if (t == 0) { a.lpart[2 * unit] = l.o; a.lpart[2 * unit + 1] = l.s; }
+    // few lanes of a wave hold a vector with a logit above the bound: those vectors are listed, and looked at side by side
     const auto pass = [&](auto put) {
+        if (t == 0) sh.nhits = 0u;
+        group_sync<NT>();
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (odd || vm[i] >= low) {
-                x[i].hold();
+            if (odd || vm[i] >= low) { const unsigned h = atomicAdd(&sh.nhits, 1u); if (h < CAND) sh.hits[h] = i * NT + t; }
+        group_sync<NT>();
+        const unsigned H = sh.nhits;
+        if (H > CAND) { if (t == 0) sh.sel[3] = CAND + 1; return; }       // too many: the exact selection
+        for (unsigned h = t; h < H; h += NT) {
+            const int at = sh.hits[h] * E;
+            Raw<DT> y;
+            y.load(z, at, n);
 #pragma unroll
-                for (int j = 0; j < E; ++j) {
-                    const float y = x[i].get(j);
-                    const int at = (i * NT + t) * E + j;
-                    if (!(y < low) && at < n) put(rank_of(y, (unsigned)(v0 + at)));
-                }
+            for (int j = 0; j < E; ++j) {
+                const float v = y.get(j);
+                if (!(v < low) && at + j < n) put(rank_of(v, (unsigned)(v0 + at + j)));
             }
+        }
     };
     const auto item = [=](int i) -> u64 { const int at = i * NT + t; return at < n ? rank_of((float)z[at], (unsigned)(v0 + at)) : 0ull; };
     const int K = min(a.K, n), N = (n + NT - 1) / NT;

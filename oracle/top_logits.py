@@ -5,9 +5,12 @@ import torch
 def top(z, k, T):
     """values, indices (ties: lowest class; NaN above everything), lse."""
     v = z.double()
-    key = torch.where(torch.isnan(v), torch.full_like(v, float("inf")), v)
-    rank = torch.isnan(v).double()                                       # NaN above +inf
-    order = torch.stack([torch.tensor(sorted(range(z.shape[1]), key=lambda i: (-float(rank[r, i]), -float(key[r, i]), i))[:k]) for r in range(z.shape[0])])
+    nan = torch.isnan(v)
+    key = torch.where(nan, torch.full_like(v, float("inf")), v)
+    order = torch.sort(key, dim=1, descending=True, stable=True)[1]      # stable: the lower class first
+    if bool(nan.any()):                                                  # NaN above +inf: a stable sort by that alone
+        order = order.gather(1, torch.sort(nan.gather(1, order).to(torch.int8), dim=1, descending=True, stable=True)[1])
+    order = order[:, :k]
     return z.gather(1, order), order, torch.logsumexp(v / T, 1)
 
 

@@ -171,6 +171,15 @@ def test_distill_rows(R, V, K, dtype, tail):
         check_distill(z, idx, val, lse, w, T, reduction)
 
 
+@pytest.mark.parametrize("V,dtype", [(131072, torch.bfloat16), (65536, torch.float32), (40000, torch.float32), (60001, torch.float16)])
+def test_distill_long_rows_of_many(V, dtype):
+    """Rows that one workgroup holds whole (up to 256 KB), and rows of many that are a little longer."""
+    for n in (V, V + 40000):
+        z, idx, val, lse, w = make(130, n, 20, dtype, V, True, True, True, 2.0)
+        check_distill(z, idx, val, lse, w, 2.0, "mean")
+    check_top(z.to(DEV), 40)
+
+
 @pytest.mark.parametrize("B,V,H,W,K", [(1, 2, 1, 2, 1), (2, 64, 3, 21, 8), (1, 64, 16, 16, 4), (2, 96, 5, 7, 16), (1, 33, 2, 65, 33), (2, 128, 4, 4, 64), (1, 700, 3, 5, 6)])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("tail", [False, True])
