@@ -348,12 +348,11 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 512 && NV == 8 ? 6 : 1) 
     row_sync<NT>();
     const int lane = threadIdx.x & 63;
     // named classes leave the row: their places are -inf from here on
-    unsigned b[NV];
+    const auto named = [&](int at) { return at < n ? bits[at >> 5] >> (at & 31) & ((1u << E) - 1) : 0u; };
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int at = (i * NT + t) * E;
-        b[i] = at < n ? bits[at >> 5] >> (at & 31) & ((1u << E) - 1) : 0u;
-        if (b[i]) x[i].drop(b[i]);
+        const unsigned b = named((i * NT + t) * E);
+        if (b) x[i].drop(b);
     }
     if constexpr (MODE != SEG_GRAD) {
         if (MODE == ROW && t < 64) { const Teacher teach = entry_numbers(a, r, e, c, lane); if (lane == 0) e.teach = teach; }
@@ -423,9 +422,10 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 512 && NV == 8 ? 6 : 1) 
 #pragma unroll
                 for (int j = 0; j < E; ++j) g[j] = 0.f;
             }
-            if (b[i]) {
+            const unsigned b = named(at);
+            if (b) {
 #pragma unroll
-                for (int j = 0; j < E; ++j) if (b[i] >> j & 1u) g[j] = e.p[slot[at + j]];
+                for (int j = 0; j < E; ++j) if (b >> j & 1u) g[j] = e.p[slot[at + j]];
             }
             T out[E];
 #pragma unroll
