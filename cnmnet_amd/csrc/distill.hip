@@ -18,10 +18,8 @@
 
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
 constexpr int KMAX = 256;                    // entries per row
-constexpr int VMAX = 1 << 20;                // classes per row: one LDS bit each (128 KB)
+constexpr int VMAX = 1 << 20;                // classes per row
 constexpr size_t LDS_BYTES = 160 * 1024;
 constexpr float TMIN = 1e-37f;                // smallest temperature: log2(e) / T is finite
 constexpr double LOG2E_D = 1.4426950408889634074, LN2_D = 0.69314718055994530942;
@@ -33,6 +31,41 @@ template <> struct Elem<CNM_BF16> { typedef __bf16 T; };
 
 __device__ inline float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Sums and maxima over a wave's 64 lanes (all of them active), the result in every lane: data-parallel moves within the vector unit -- shifts inside
+// rows of 16, then the rows' last lanes handed on --, a few cycles a step where an exchange through LDS takes a hundred.
+template <int CTRL, int ROWS>
+__device__ inline float lane_move(float x, float none) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(x), CTRL, ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS>
+__device__ inline double lane_move(double x) {                           // (lanes without a source: 0)
+    const long long u = __double_as_longlong(x);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)u, CTRL, ROWS, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __longlong_as_double((long long)hi << 32 | (unsigned)lo);
+}
+__device__ inline float last_lane(float x) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63)); }
+__device__ inline double last_lane(double x) {
+    const long long u = __double_as_longlong(x);
+    return __longlong_as_double((long long)__builtin_amdgcn_readlane((int)(u >> 32), 63) << 32 | (unsigned)__builtin_amdgcn_readlane((int)u, 63));
+}
+constexpr int SHR1 = 0x111, SHR2 = 0x112, SHR4 = 0x114, SHR8 = 0x118, BCAST15 = 0x142, BCAST31 = 0x143;
+__device__ inline float sum_wave(float x) {
+    x += lane_move<SHR1, 0xf>(x, 0.f); x += lane_move<SHR2, 0xf>(x, 0.f); x += lane_move<SHR4, 0xf>(x, 0.f); x += lane_move<SHR8, 0xf>(x, 0.f);
+    x += lane_move<BCAST15, 0xa>(x, 0.f); x += lane_move<BCAST31, 0xc>(x, 0.f);
+    return last_lane(x);
+}
+__device__ inline double sum_wave(double x) {
+    x += lane_move<SHR1, 0xf>(x); x += lane_move<SHR2, 0xf>(x); x += lane_move<SHR4, 0xf>(x); x += lane_move<SHR8, 0xf>(x);
+    x += lane_move<BCAST15, 0xa>(x); x += lane_move<BCAST31, 0xc>(x);
+    return last_lane(x);
+}
+__device__ inline float max_wave(float x) {
+    constexpr float none = -__builtin_huge_valf();
+    x = fmaxf(x, lane_move<SHR1, 0xf>(x, none)); x = fmaxf(x, lane_move<SHR2, 0xf>(x, none)); x = fmaxf(x, lane_move<SHR4, 0xf>(x, none)); x = fmaxf(x, lane_move<SHR8, 0xf>(x, none));
+    x = fmaxf(x, lane_move<BCAST15, 0xa>(x, none)); x = fmaxf(x, lane_move<BCAST31, 0xc>(x, none));
+    return last_lane(x);
+}
+
 // (offset, sum) of exponentials 2^((x - offset) c); offset = -inf: none yet
 struct Lse { float o, s; };
 __device__ inline Lse lse_join(Lse a, Lse b, float c) {
@@ -42,8 +75,8 @@ __device__ inline Lse lse_join(Lse a, Lse b, float c) {
     return {o, a.s * exp2_((a.o - so) * c) + b.s * exp2_((b.o - so) * c)};
 }
 __device__ inline Lse lse_wave(Lse a, float c) {
-    for (int d = 32; d; d >>= 1) a = lse_join(a, Lse{__shfl_xor(a.o, d), __shfl_xor(a.s, d)}, c);
-    return a;
+    const float o = max_wave(a.o), so = o == -__builtin_huge_valf() ? 0.f : o;
+    return {o, sum_wave(a.s * exp2_((a.o - so) * c))};
 }
 // the natural logarithm of the sum, in units of 1 / T
 __device__ inline float lse_value(Lse l, float T) {
@@ -63,14 +96,11 @@ __device__ inline Lse lse_block(Lse a, float c, float* sh) {
 }
 template <int NT>
 __device__ inline double sum_block(double a, double* sh) {
-    for (int d = 32; d; d >>= 1) a += __shfl_xor(a, d);
-    if (NT == 64) return a;
+    a = sum_wave(a);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
     __syncthreads();
-    a = (threadIdx.x & 63) < NT / 64 ? sh[threadIdx.x & 63] : 0.0;
-    for (int d = 32; d; d >>= 1) a += __shfl_xor(a, d);
-    return a;
+    return sum_wave((threadIdx.x & 63) < NT / 64 ? sh[threadIdx.x & 63] : 0.0);
 }
 // sixteen bytes of a row as they are in memory, elements beyond the row -inf.  hold(): conversions done so far are forgotten (left alone, hipcc
 // keeps every converted element in a register of its own from one pass over the row to the next)
@@ -132,7 +162,7 @@ struct DistillArgs {
     const void* idx; int wide;               // [rows][K] or [outer][K][inner], int32 / int64
     const void* val; int vdt;                // the entries' logits
     const float* lse;                        // [rows] or null: renormalised
-    float T;
+    float T, c; double iT, l2T;              // temperature; log2(e) / T in fp32, 1 / T and log2(e) / T in fp64
     const float* weight;                     // [rows] or null
     const double* wpart; int nwpart;         // the weights' partial sums (gradients are divided by their sum), or null
     double inv_norm;                         // otherwise multiplied by this
@@ -151,9 +181,7 @@ struct DistillRow { double L; float A, B, orest, oall, inv, pad; };
 
 // sum of up to 64 partial sums, in a fixed order, by a whole wave
 __device__ inline double wave_total(const double* part, int n) {
-    double s = (int)(threadIdx.x & 63) < n ? part[threadIdx.x & 63] : 0.0;
-    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
-    return s;
+    return sum_wave((int)(threadIdx.x & 63) < n ? part[threadIdx.x & 63] : 0.0);
 }
 
 // 2^x, relative error of a few 2^-24 whatever x's size
@@ -200,7 +228,7 @@ __device__ inline void mark_entries(Entries& e, int K, unsigned* bits, int v0, i
         if (e.idx[k] >= 0 && i >= 0 && i < n && (atomicOr(&bits[i >> 5], 1u << (i & 31)) >> (i & 31) & 1u)) e.dup = 1;
     }
 }
-__device__ inline double entry_log2p(const DistillArgs& a, float logit, double L) { return ((double)logit / (double)a.T - L) * LOG2E_D; }
+__device__ inline double entry_log2p(const DistillArgs& a, float logit, double L) { return (double)logit * a.l2T - L * LOG2E_D; }
 
 // a class that is named more than once: its first entry gets the sum, the others become none (one wave)
 __device__ inline void join_entries(Entries& e, int K, int lane) {
@@ -226,19 +254,16 @@ __device__ inline void join_entries(Entries& e, int K, int lane) {
 // A row's numbers, by one wave while the others go over the classes: the fp64 logarithms are hundreds of instructions, too many for every wave.
 // First what the entries alone say (e.p becomes the probabilities), then, with the unnamed classes' statistics, the loss and the gradient's
 // coefficients for an upstream gradient of 1.
-__device__ inline double sum_wave(double a) { for (int d = 32; d; d >>= 1) a += __shfl_xor(a, d); return a; }
-__device__ inline double max_wave(double a) { for (int d = 32; d; d >>= 1) a = fmax(a, __shfl_xor(a, d)); return a; }
-
 __device__ inline Teacher entry_numbers(const DistillArgs& a, size_t r, Entries& e, float c, int lane) {
     const float ninf = -__builtin_huge_valf();
     Teacher w;
     w.named = {ninf, 0.f};
-    double best = -__builtin_huge_val();
+    float best = ninf;
     bool have = false;
     for (int k = lane; k < a.K; k += 64) {
         const int i = e.idx[k];
         bool first = i >= 0;
-        if (first) { have = true; best = fmax(best, (double)e.p[k]); }
+        if (first) { have = true; best = fmaxf(best, e.p[k]); }
         if (e.dup) for (int j = 0; j < k && first; ++j) first = e.idx[j] != i;
         if (first) {
             const float x = e.z[k];
@@ -250,10 +275,10 @@ __device__ inline Teacher entry_numbers(const DistillArgs& a, size_t r, Entries&
     if (a.lse) w.L = (double)a.lse[r];
     else {
         best = max_wave(best);
-        if (best == -__builtin_huge_val()) best = 0.0;
+        if (best == ninf) best = 0.f;
         double s = 0.0;
-        for (int k = lane; k < a.K; k += 64) if (e.idx[k] >= 0) s += (double)exp2_of(((double)e.p[k] - best) * (LOG2E_D / (double)a.T));
-        w.L = best / (double)a.T + log(sum_wave(s));
+        for (int k = lane; k < a.K; k += 64) if (e.idx[k] >= 0) s += (double)exp2_of(((double)e.p[k] - (double)best) * a.l2T);
+        w.L = (double)best * a.iT + log(sum_wave(s));
     }
     double P = 0.0, lp = 0.0;
     for (int k = lane; k < a.K; k += 64) {
@@ -336,7 +361,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 512 && NV == 8 ? 6 : 1) 
     const T* const zrow = static_cast<const T*>(a.z) + r * a.ldz;
     const T* const z = zrow + v0;
     if (a.go && a.go_rows) go = a.go[r];
-    const float c = (float)(LOG2E_D / (double)a.T), ninf = -__builtin_huge_valf();
+    const float c = a.c, ninf = -__builtin_huge_valf();
     Raw<DT> x[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) x[i].load(z, (i * NT + t) * E, n);
@@ -385,6 +410,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 512 && NV == 8 ? 6 : 1) 
             row_sync<64>();
             const DistillRow row = finish_row(a, r, rest, e.teach, e, c, lane);
             if (lane == 0) e.row = row;
+            row_sync<64>();
         }
     } else {
         if (t == 0) e.row = a.rec[r];
@@ -446,7 +472,7 @@ __global__ __launch_bounds__(64) void distill_join_kernel(const DistillArgs a) {
     const int t = threadIdx.x;
     if (a.skip_if_one && a.go && a.go[0] == 1.f) return;
     const size_t r = blockIdx.x;
-    const float c = (float)(LOG2E_D / (double)a.T);
+    const float c = a.c;
     if (t == 0) e.dup = 1;                                               // (no bits here to tell: looked up)
     load_entries<DT, 64>(a, r, static_cast<const T*>(a.z) + r * a.ldz, e, t);
     row_sync<64>();
@@ -484,7 +510,7 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
     const size_t at = live ? p0 + px : 0;                                // position in a plane
     const T* const z = static_cast<const T*>(a.z) + (size_t)ob * V * a.inner + at;
     const size_t ebase = (size_t)ob * K * a.inner + at, r = (size_t)ob * a.inner + at;
-    const float c = (float)(LOG2E_D / (double)a.T), ninf = -__builtin_huge_valf();
+    const float c = a.c, ninf = -__builtin_huge_valf();
 
     for (int i = w; i < nw; i += 4) bits[i * 64 + px] = 0u;
     T first[16];                                                         // sixteen of the wave's classes are requested before anything waits
@@ -532,8 +558,8 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
             for (int k = 0; k < K; ++k) if (eidx[k * 64 + px] != -1) best = fmaxf(best, ep[k * 64 + px]);
             if (best == ninf) best = 0.f;
             double s = 0.0;
-            for (int k = 0; k < K; ++k) if (eidx[k * 64 + px] != -1) s += (double)exp2_of(((double)ep[k * 64 + px] - (double)best) * (LOG2E_D / (double)a.T));
-            L = (double)best / (double)a.T + log(s);
+            for (int k = 0; k < K; ++k) if (eidx[k * 64 + px] != -1) s += (double)exp2_of(((double)ep[k * 64 + px] - (double)best) * a.l2T);
+            L = (double)best * a.iT + log(s);
         }
         for (int k = 0; k < K; ++k) {
             float p = 0.f;
@@ -654,6 +680,12 @@ int distill_segments(long long rows, int V, int esize) {
     return want;
 }
 
+// threads that share a row or segment of so many vectors
+int distill_threads(int vecs) { return vecs <= 256 ? 64 : vecs <= 1024 ? 256 : vecs <= 4096 ? 512 : 1024; }
+int top_threads(int vecs) { return vecs <= 64 ? 64 : vecs <= 256 ? 256 : vecs <= 2048 ? 512 : 256; }
+// a launch holds fewer than 2^32 threads; rows by fours where a wave takes a whole one
+bool launch_fits(long long units, int threads) { return (units + 3) * threads < (1ll << 32); }
+
 template <int DT, int MODE>
 void launch_rows(const DistillArgs& a, hipStream_t stream) {
     constexpr int E = 16 / (int)sizeof(typename Elem<DT>::T);
@@ -716,7 +748,7 @@ __device__ inline u64 rank_of(float x, unsigned v) { return (u64)key_of(x) << 32
 
 struct TopArgs {
     const void* z; long long ldz;
-    float T;
+    float T, c;                              // temperature, log2(e) / T
     void* val; int* idx; float* lse;
     u64* part; float* lpart;                 // [rows][segments][K] ranks and [rows][segments][2] (offset, sum), where a row is split
     long long rows; int V, K; long long inner;
@@ -800,11 +832,6 @@ __device__ inline void take_largest(P pass, F item, int N, int K, int t, TopShar
     }
 }
 
-// wave-wide maximum, in every lane
-__device__ inline float wave_max(float x) {
-    for (int d = 32; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
-    return x;
-}
 // a lower bound of the K-th largest of the NT threads' numbers: every wave's r-th largest, r = K / waves rounded up, the smallest of these
 template <int NT>
 __device__ inline float kth_bound(float m, int K, float* sh) {
@@ -814,7 +841,7 @@ __device__ inline float kth_bound(float m, int K, float* sh) {
     if (r > 64) return ninf;
     const int lane = threadIdx.x & 63;
     // the wave's numbers in order (bitonic, descending: 21 exchanges), or for the first of them six exchanges
-    if (r == 1) m = wave_max(m);
+    if (r == 1) m = max_wave(m);
     else {
 #pragma unroll
         for (int size = 2; size <= 64; size <<= 1)
@@ -849,7 +876,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 256 && NV == 16 ? 4 : 1)
     const long long r = unit / a.segments;
     const int seg = (int)(unit - r * a.segments), v0 = seg * a.seglen, n = min(a.V - v0, a.seglen);
     const T* z = static_cast<const T*>(a.z) + (size_t)r * a.ldz + v0;
-    const float c = (float)(LOG2E_D / (double)a.T), ninf = -__builtin_huge_valf();
+    const float c = a.c, ninf = -__builtin_huge_valf();
     Raw<DT> x[NV];
     float m = ninf;
 #pragma unroll
@@ -919,7 +946,7 @@ __global__ __launch_bounds__(1024) void top_join_kernel(const TopArgs a) {
     const int t = threadIdx.x;
     const long long r = blockIdx.x;
     const int total = a.segments * a.K;
-    const float c = (float)(LOG2E_D / (double)a.T), ninf = -__builtin_huge_valf();
+    const float c = a.c, ninf = -__builtin_huge_valf();
     u64 k[N];
     float m = ninf;
 #pragma unroll
@@ -960,7 +987,7 @@ __global__ __launch_bounds__(256) void top_planes_kernel(const TopArgs a) {
     if (r >= a.rows) return;
     const long long ob = r / a.inner, at = r % a.inner;
     const T* z = static_cast<const T*>(a.z) + (size_t)ob * a.V * a.inner + at;
-    const float c = (float)(LOG2E_D / (double)a.T), ninf = -__builtin_huge_valf();
+    const float c = a.c, ninf = -__builtin_huge_valf();
     unsigned key[KM];                                                    // 0 is below every key
     int cls[KM];
 #pragma unroll
@@ -1072,12 +1099,15 @@ extern "C" int cnm_top_logits(const void* z, int dtype, long long ldz, float tem
                               long long rows, int classes, int entries, long long inner, void* stream) {
     CNM_REQUIRE(z && values && indices && lse && rows > 0 && classes > 0 && inner > 0 && temperature >= TMIN && temperature < __builtin_huge_valf(), CNM_ERR_BAD_ARG);
     CNM_REQUIRE(entries > 0 && entries <= classes && entries <= (inner > 1 ? TOP_PLANES_KMAX : KMAX) && rows % inner == 0 && (inner > 1 || ldz >= classes), CNM_ERR_BAD_ARG);
-    CNM_REQUIRE(rows < (1ll << 30) / 64 * 64 && classes <= VMAX && (inner > 1 || rows * cnm_ceil_div(classes, 4096) < (1ll << 31)), CNM_ERR_BAD_SHAPE);
+    CNM_REQUIRE(dtype >= CNM_F32 && dtype <= CNM_BF16, CNM_ERR_BAD_ARG);
+    CNM_REQUIRE(rows < (1ll << 30) && classes <= VMAX, CNM_ERR_BAD_SHAPE);
+    const int E = dtype == CNM_F32 ? 4 : 8, cut = inner > 1 ? 1 : top_segments(rows, classes, entries, 16 / E);
+    CNM_REQUIRE(inner > 1 || launch_fits(rows * cut, top_threads(cnm_ceil_div(cnm_ceil_div(classes, cut), E))), CNM_ERR_BAD_SHAPE);
     const size_t need = cnm_top_logits_workspace_bytes(dtype, rows, classes, entries, inner);
     CNM_REQUIRE(!need || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 7) == 0), CNM_ERR_WORKSPACE);
     u64* const part = static_cast<u64*>(workspace);
     float* const lpart = need ? reinterpret_cast<float*>(part + (need - (size_t)2 * sizeof(float) * (need / ((size_t)entries * sizeof(u64) + 2 * sizeof(float)))) / sizeof(u64)) : nullptr;
-    const TopArgs a = {z, ldz, temperature, values, indices, lse, part, lpart, rows, classes, entries, inner, 1, 0};
+    const TopArgs a = {z, ldz, temperature, (float)(LOG2E_D / (double)temperature), values, indices, lse, part, lpart, rows, classes, entries, inner, 1, 0};
     switch (dtype) {
         case CNM_F32: return launch_top<CNM_F32>(a, cnm_stream(stream));
         case CNM_F16: return launch_top<CNM_F16>(a, cnm_stream(stream));
@@ -1103,22 +1133,24 @@ extern "C" int cnm_distill(const void* z, int dtype, long long ldz, const void* 
     CNM_REQUIRE(rows % inner == 0 && (inner > 1 || ldz >= classes) && dtype >= CNM_F32 && dtype <= CNM_BF16 && entry_dtype >= CNM_F32 && entry_dtype <= CNM_BF16, CNM_ERR_BAD_ARG);
     CNM_REQUIRE(!grad_out_rows || (grad_out && reduction == 0), CNM_ERR_BAD_ARG);
     CNM_REQUIRE(!workspace_ready || !loss, CNM_ERR_BAD_ARG);
-    CNM_REQUIRE(rows < (1ll << 31) && classes <= VMAX && (inner == 1 || cnm_distill_planes_ok(classes, entries)), CNM_ERR_BAD_SHAPE);
+    CNM_REQUIRE(rows < (1ll << 30) && classes <= VMAX && (inner == 1 || cnm_distill_planes_ok(classes, entries)), CNM_ERR_BAD_SHAPE);
     const int seg = inner > 1 ? 1 : distill_segments(rows, classes, dtype == CNM_F32 ? 4 : 2);
-    CNM_REQUIRE(rows * seg < (1ll << 31), CNM_ERR_BAD_SHAPE);
+    const int E = dtype == CNM_F32 ? 4 : 8;
+    const long long tiles = inner > 1 ? (rows / inner) * cnm_ceil_div_ll(inner, 64) : 0;
+    CNM_REQUIRE(inner > 1 ? launch_fits(tiles, 256) : launch_fits(rows * seg, distill_threads(cnm_ceil_div(cnm_ceil_div(classes, seg), E))), CNM_ERR_BAD_SHAPE);
     CNM_REQUIRE(workspace && workspace_doubles >= cnm_distill_workspace_doubles(dtype, rows, classes, inner), CNM_ERR_WORKSPACE);
     const hipStream_t st = cnm_stream(stream);
     const bool mean = reduction == 1;
     double* const wpart = workspace;
     double* const lpart = workspace + WPARTS;
-    const long long parts = inner > 1 ? (rows / inner) * cnm_ceil_div_ll(inner, 64) : rows;
+    const long long parts = inner > 1 ? tiles : rows;
     DistillRow* const rec = seg > 1 ? reinterpret_cast<DistillRow*>(lpart + parts) : nullptr;
     float* const segs = seg > 1 ? reinterpret_cast<float*>(rec + rows) : nullptr;
     const int nw = mean && weight ? (int)(cnm_ceil_div_ll(rows, 4096) < WPARTS ? cnm_ceil_div_ll(rows, 4096) : WPARTS) : 0;
     if (nw && !workspace_ready) { weight_parts_kernel<<<nw, 1024, 0, st>>>(weight, rows, wpart); CNM_LAUNCH_CHECK(); }
     const double inv_norm = mean && !weight ? 1.0 / (double)rows : 1.0;
     const bool total = reduction != 0 && loss;
-    const DistillArgs a = {z, ldz, indices, wide_indices, entry_logits, entry_dtype, teacher_lse, temperature, weight, nw ? wpart : nullptr, nw, inv_norm,
+    const DistillArgs a = {z, ldz, indices, wide_indices, entry_logits, entry_dtype, teacher_lse, temperature, (float)(LOG2E_D / (double)temperature), 1.0 / (double)temperature, LOG2E_D / (double)temperature, weight, nw ? wpart : nullptr, nw, inv_norm,
                            grad_out, grad_out_rows, skip_if_one, total ? nullptr : loss, total ? lpart : nullptr, dz, rows, classes, entries, inner, rec, segs, seg, 0};
     int rc = CNM_ERR_BAD_ARG;
     switch (dtype) {

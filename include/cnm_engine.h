@@ -900,7 +900,7 @@ int cnm_linear_fp8_backward(const void* dy, int dy_dtype, long long lddy, const 
  * (inner > 1: e.g. [B, planes, H, W], inner = H W; ldz is ignored).  Entries, values, indices and per-row numbers follow the same order
  * ([rows][entries] or [rows / inner][entries][inner]; [rows]).
  *
- * temperature: at least 1e-37, finite.
+ * temperature: at least 1e-37, finite.  rows: what one launch holds, fewer than 2^32 threads of 64 (short rows) to 1024 each; more: CNM_ERR_BAD_SHAPE.
  *
  * cnm_top_logits: the `entries` largest logits per row in descending order (ties: the lower class first; NaN above everything, -0 equal to
  * +0), their classes, and lse = log sum exp(z / temperature).  entries <= classes, <= cnm_distill_max_entries() (inner = 1) or

@@ -128,6 +128,8 @@ def test_top_and_distill_entries_refuse():
     assert d(_16=0) == -5 and d(_17=n - 1) == -5
     assert d(_20=(1 << 20) + 1, _2=1 << 21) == -2
     assert d(_18=1) == -1                                               # a loss needs its own pass
+    # more rows than one launch has threads for: refused before anything is launched
+    assert t(_9=1 << 27) == -2 and d(_19=1 << 27, _17=1 << 40) == -2 and d(_19=1 << 28, _22=2, _17=1 << 40) == -2
     assert d(_22=2, _20=100000) == -2                                   # planes that do not fit LDS
     assert lib.cnm_distill_planes_ok(64, 8) == 1 and lib.cnm_distill_planes_ok(100000, 8) == 0 and lib.cnm_distill_planes_ok(64, 0) == 0
 
