@@ -797,7 +797,8 @@ def top_logits_distill(logits, top_idx, top_logits, top_lse=None, weight=None, t
 class TopLogitsDistill(torch.autograd.Function):
     """ops.top_logits_distill on the tape; gradient to the logits only.  For "mean" and "sum" the gradient is written by the forward launch, which
     has the row at hand, and the backward pass only looks at the upstream gradient: where it is 1 (the loss is the root) there is nothing left
-    to do, otherwise the kernel recomputes the gradient from the logits with it -- never by scaling what was already rounded."""
+    to do, otherwise the kernel recomputes the gradient from the logits with it -- never by scaling what was already rounded.  Captured, the
+    two passes belong in one graph, or in two that are replayed in turn."""
 
     @staticmethod
     def forward(ctx, logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction):

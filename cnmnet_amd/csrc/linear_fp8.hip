@@ -13,10 +13,10 @@
 // to the output type.  Both operands are [rows][K] with K contiguous ("NT"); the second one's scales are per row or per 128 rows.
 //
 // Two ways through the matrix pipe, by the type of the result.
-//   16-bit results: v_mfma_scale_f32_16x16x128_f8f6f4 on the bytes as they are, twice the bf16 rate.  Its accumulator is fp32, but it adds
+//   16-bit results: v_mfma_scale_f32_32x32x64_f8f6f4 (tiles; 16x16x128 where rows are few) on the bytes as they are, twice the bf16 rate.  Its accumulator is fp32, but it adds
 //     eight consecutive products at a time, each cut off at 2^-13 of the eight's largest exponent (measured: probes of single terms; rms
 //     1.5e-5 of the result on normal data): a choice for results that are rounded to 2^-9 or 2^-12 anyway.
-//   fp32 results: the bytes become bf16 with their scale applied (exact within bf16's exponent range) and v_mfma_f32_16x16x32_bf16 adds them:
+//   fp32 results: the bytes become bf16 with their scale applied (exact within bf16's exponent range) and v_mfma_f32_32x32x16_bf16 (16x16x32) adds them:
 //     rms 1e-8 of the result, as fp32 sums are.
 #include "cnm_common.h"
 
@@ -72,6 +72,8 @@ __device__ inline void load8(const typename Elem<DT>::T* p, int have, float v[8]
 // One workgroup quantises a 128 x 128 tile, read once: 16 lanes per row (8 values each), a thread's four rows consecutive, so that the
 // transposed copy leaves as 4-byte columns through LDS.  Row form: q [R][Cp], s [R][Cp/128] (BLK = false) or s [R/128][Cp/128] (BLK = true).
 // Transposed form (optional): qt [C][Rp], blocked along R: st [C][Rp/128], or the same 128 x 128 block's byte at st [C/128][Rp/128].
+// Bound by memory: bf16 8192 x 8192 without the transposed form 51 us (4.0 TB/s of read and written bytes, a large copy 4.6), 8192 x 4096
+// with it 45 us (3.0 TB/s: 128-byte pieces of 128 transposed rows per workgroup; through a tile without the chunk permutation 50).
 template <int DT, bool BLK>
 __global__ __launch_bounds__(512) void quantize_kernel(const typename Elem<DT>::T* __restrict__ x, long long ldx, int R, int C, int Cb, int Rb,
                                                        unsigned char* __restrict__ q, unsigned char* __restrict__ s,
@@ -217,6 +219,8 @@ __device__ inline void tile_of(int id, const MatArgs& g, int& tm, int& tn) {
 // all 64 banks.  The DMA writes 64 lanes x 16 bytes in order, so the permutation is in the lanes' source addresses.
 // Scale bytes: rows of SC blocks in LDS, refilled every SC blocks; a lane reads four blocks' bytes as one word.
 // The weight is the instruction's first operand: a lane then holds outputs of one row, in fours.
+// 8192 x 8192 x 8192, bf16 results: about 430 us, 2.4 to 2.6 PF from card to card (a library product of plain bytes 2.6), held back by the package's
+// power limit; 8192 x 4096 x 4096: 122 to 133 us (2.1 to 2.3 PF), of which 9 us per tile are its first loads and its stores.
 // The order within a half block: its NM matrix instructions start at once, the next fragments' ND reads and the NV DMA instructions go evenly
 // between them (left alone, the scheduler puts all of these in front, or the matrix instructions of two half blocks behind one barrier).
 template <int I, int NM, int ND, int NV>
@@ -484,6 +488,7 @@ int launch_matmul(MatArgs g, float* ws, hipStream_t stream) {
 //   few columns (N <= 128): a wave takes 16 MT rows of x and all of w, which stays in the caches (KS = 1).
 // QUANT: x comes as it is (float32 / float16 / bfloat16) and is quantised in registers: a lane holds 32 consecutive values of one row, its
 // block's maximum is two exchanges away; x is then read once and never written in 8 bits.
+// bf16 1 x 4096 x 4096: 7.0 us (2.4 TB/s of the 16 MB weight, the launch's own latency half of it); fp32 49152 x 64 x 512: 26.7 us (4.2 TB/s).
 struct StreamArgs {
     const void* x; long long ldx;            // [M][ldx] as it is, or e4m3 [M][Kb * 128] with scale sx [M][Kb]
     const unsigned char *sx, *w, *sw;
