@@ -868,7 +868,7 @@ __device__ inline float kth_bound(float m, int K, float* sh) {
 
 // NT threads per row or segment of a row, which they hold in registers (NV vectors of 16 bytes each), read once.  Log-sum-exp, then a lower bound of
 // the K-th largest logit from the threads' own maxima, the few logits above it to LDS, and their order by counting.
-// bf16 4096 x 32768, 64 entries: 57 us (4.7 TB/s, what a large copy reaches); one row of 131072 in segments 9 us, their join 7: latency.
+// bf16 4096 x 32768, 32 entries: 57 us (4.7 TB/s, what a large copy reaches); one row of 131072 in segments 9 us, their join 7: latency.
 template <int DT, int NT, int NV>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 256 && NV == 16 ? 4 : 1) void top_rows_kernel(const TopArgs a) {
     typedef typename Elem<DT>::T T;
