@@ -168,7 +168,7 @@ struct DistillArgs {
     double inv_norm;                         // otherwise multiplied by this
     const float* go; int go_rows;            // upstream gradient: one value, or one per row; null: 1
     int skip_if_one;                         // *go == 1: the gradient is already there (written by the forward pass)
-    float* loss;                             // [rows] or null
+    float* loss;                             // [rows]: weight * loss, or null
     double* lpart;                           // per row or per workgroup: weight * loss, or null
     void* dz;                                // as z but dense, or null
     long long rows; int V, K; long long inner;
@@ -320,8 +320,9 @@ __device__ inline DistillRow finish_row(const DistillArgs& a, size_t r, Lse rest
     if (!w.have) loss = 0.0;
     const float wrow = a.weight ? a.weight[r] : 1.f;
     if (lane == 0) {
-        if (a.loss) a.loss[r] = (float)loss;
-        if (a.lpart) a.lpart[r] = wrow != 0.f ? (double)wrow * loss : 0.0;
+        const double l = wrow != 0.f ? (double)wrow * loss : 0.0;        // (weight 0: whatever the logits hold)
+        if (a.loss) a.loss[r] = (float)l;
+        if (a.lpart) a.lpart[r] = l;
     }
     double norm = a.inv_norm;
     if (a.wpart) { const double s = wave_total(a.wpart, a.nwpart); norm = s > 0.0 ? a.inv_norm / s : 0.0; }
@@ -605,9 +606,10 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
         loss *= (double)a.T * (double)a.T;
         if (!have) loss = 0.0;
         const float wrow = live ? (a.weight ? a.weight[r] : 1.f) : 0.f;
-        if (a.loss && live) a.loss[r] = (float)loss;
+        const double wloss = wrow != 0.f ? (double)wrow * loss : 0.0;
+        if (a.loss && live) a.loss[r] = (float)wloss;
         if (a.lpart) {
-            const double l = sum_wave(wrow != 0.f ? (double)wrow * loss : 0.0);
+            const double l = sum_wave(wloss);
             if (px == 0) a.lpart[blockIdx.x] = l;
         }
         if (a.dz) {

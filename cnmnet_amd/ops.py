@@ -1011,8 +1011,8 @@ def top_logits_distill(logits, top_idx, top_logits, top_lse=None, weight=None, t
     """Distillation loss of a student's logits against a teacher's stored top logits (ops.top_logits of the teacher at the same temperature):
     T^2 KL(teacher || student) with the teacher's classes outside the entries lumped into one (top_lse given), or the entries renormalised
     (top_lse None); include/cnm_engine.h states the formula.  top_idx (int32 / int64; an index outside the classes is no entry) and top_logits
-    have K in the place of the classes; top_lse and weight are float32 without that dim.  reduction "mean": sum weight loss / sum weight, "sum",
-    or "none".  grad=True: (loss, gradient of the logits) in one pass over them, for programs that call backward on the logits themselves."""
+    have K in the place of the classes; top_lse and weight are float32 without that dim.  reduction "mean": sum weight loss / sum weight, "sum":
+    sum weight loss, or "none": weight loss per row.  grad=True: (loss, gradient of the logits) in one pass over them, for programs that call backward on the logits themselves."""
     call = DistillCall(logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction)
     dz = call.new_grad() if grad else None
     loss = call.run(True, dz)

@@ -919,9 +919,9 @@ int cnm_distill_planes_ok(int classes, int entries);
  *   loss = T^2 [ sum_k p_k (log p_k - log q_{i_k}) + p_r (log p_r - log q_r) ], p_r = max(0, 1 - sum p_k) and q_r = the probability of the
  *   classes that no entry names, with teacher_lse only and only if these classes have any.
  * An index outside 0 .. classes-1 is no entry; a row without entries has loss 0 and gradient 0; a class may be named more than once.
- * reduction 0: loss [rows]; 1: loss [1] = sum weight loss / sum weight (0 if the weights sum to 0); 2: loss [1] = sum weight loss.
- * weight [rows] or NULL (1).  dz (dense, z's dtype) = the gradient of what `loss` is (reduction 0: of sum weight loss), times grad_out[0], or
- * grad_out[row] with grad_out_rows (reduction 0 only), or 1 (NULL).  skip_if_one: if grad_out[0] == 1 the launch leaves dz as it is.
+ * reduction 0: loss [rows] = weight loss; 1: loss [1] = sum weight loss / sum weight (0 if the weights sum to 0); 2: loss [1] = sum weight loss.
+ * weight [rows] or NULL (1); a row of weight 0 counts 0 whatever it holds.  dz (dense, z's dtype) = the gradient of what `loss` is (reduction 0: of
+ * its sum), times grad_out[0], or grad_out[row] with grad_out_rows (reduction 0 only), or 1 (NULL).  skip_if_one: if grad_out[0] == 1 the launch leaves dz as it is.
  * loss or dz may be NULL, not both.  workspace: cnm_distill_workspace_doubles doubles, contents irrelevant; with workspace_ready (loss NULL) it
  * is as an earlier call with the same arguments but for loss, dz and grad_out has left it.  Every sum has a fixed order: results repeat bit
  * by bit. */

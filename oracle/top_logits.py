@@ -15,7 +15,7 @@ def top(z, k, T):
 
 
 def distill(z, idx, val, lse, w, T, reduction, go=None):
-    """-> (loss, gradient of sum(go * loss) for "none", of go * loss otherwise, error scale of the loss rows)."""
+    """-> (loss -- "none": w times each row's --, gradient of sum(go * loss) for "none", of go * loss otherwise, error scale of the loss rows)."""
     z, val, idx = z.double(), val.double(), idx.long()
     R, V = z.shape
     w = torch.ones(R, dtype=torch.float64) if w is None else w.double()
@@ -45,10 +45,10 @@ def distill(z, idx, val, lse, w, T, reduction, go=None):
                 g[out] = q[out] - pr * torch.softmax(z[r][out] / T, 0)
         rows.append(T * T * loss); grads.append(T * g); scale.append(float(1 + mag))
     rows, grads = torch.stack(rows), torch.stack(grads)
+    live = w != 0
     if reduction == "none":
         go = torch.ones(R, dtype=torch.float64) if go is None else go.double()
-        return rows, grads * (go * w)[:, None], torch.tensor(scale)
-    live = w != 0
+        return torch.where(live, w * rows, torch.zeros_like(rows)), torch.where(live[:, None], grads * (go * w)[:, None], torch.zeros_like(grads)), torch.tensor(scale)
     total = (w[live] * rows[live]).sum()
     c = torch.where(live, w, torch.zeros_like(w))
     if reduction == "mean":

@@ -1,0 +1,35 @@
+"""CPU: the distillation oracle against itself -- its gradient is the derivative of the loss that it returns -- and against the formula."""
+import pytest
+import torch
+
+from oracle import top_logits as tl
+
+
+def case(R=7, V=12, K=4, seed=2):
+    g = torch.Generator().manual_seed(seed)
+    z = torch.randn(R, V, dtype=torch.float64, generator=g)
+    teacher = torch.randn(R, V, dtype=torch.float64, generator=g)
+    val, idx = teacher.topk(K, 1)
+    idx[3, 2:] = -1
+    return z, idx, val, torch.logsumexp(teacher / 2.0, 1), torch.tensor([0.5, 0.0, -1.5, 2.0, 1.0, 0.25, 3.0], dtype=torch.float64)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_oracle_gradient_is_that_of_its_loss(reduction, tail):
+    """Central differences, weights (0 among them) and upstream gradients included; step 1e-5: off by 1e-10 of the third derivative and 1e-16 / 1e-5."""
+    z, idx, val, lse, w = case()
+    go = torch.linspace(-2, 3, 7, dtype=torch.float64) if reduction == "none" else torch.tensor(1.5, dtype=torch.float64)
+    lse = lse if tail else None
+    g = tl.distill(z, idx, val, lse, w, 2.0, reduction, go)[1]
+    rng = torch.Generator().manual_seed(5)
+    for _ in range(6):
+        d, h = torch.randn(7, 12, dtype=torch.float64, generator=rng), 1e-5
+        num = ((tl.distill(z + h * d, idx, val, lse, w, 2.0, reduction)[0] - tl.distill(z - h * d, idx, val, lse, w, 2.0, reduction)[0]) / (2 * h) * go).sum()
+        assert abs(float(num) - float((g * d).sum())) < 1e-8
+
+
+def test_oracle_weights_each_row():
+    z, idx, val, lse, w = case()
+    plain, weighted = (tl.distill(z, idx, val, lse, x, 2.0, "none")[0] for x in (None, w))
+    assert torch.equal(weighted, w * plain)

@@ -1,0 +1,115 @@
+"""GPU: what the distillation operators promise at the edges of their contract -- weights, special values, reused graphs, memory -- against the
+formula in float64, differentiated by torch on the CPU.
+
+Bounds.  A sum of exponentials: a thread adds at most 128 of them one after another, then 6 steps within a wave, 4 across a workgroup and 6 across
+segments, three roundings each: 176 times 2^-24; an exponential is off by 2^-23 and its argument by three roundings of its size X = range / T:
+D = (178 + 3 X) 2^-24 relative.  A row's loss: D times 1 + the size of its terms, an entry's p by 8 * 2^-24 more; a gradient element: 2 D of its
+q, D + 64 * 2^-24 of its p, half a step of its type."""
+import pytest
+import torch
+
+from cnmnet_amd import ops
+from cnmnet_amd.depthnet.losses import TopLogitsDistillLoss
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+INF, NAN = float("inf"), float("nan")
+
+
+def spread(z, T):
+    f = z.double()[torch.isfinite(z)]
+    return (178 + 3 * float(f.max() - f.min()) / T) * 2.0 ** -24
+
+
+def formula(z, idx, val, lse, T):
+    """[R, V] on the CPU -> rows' losses, their gradients, the size of their terms; float64, the gradient by torch's own differentiation."""
+    z = z.double().requires_grad_()
+    R, V = z.shape
+    lq = torch.log_softmax(z / T, 1)
+    ok = (idx >= 0) & (idx < V)
+    at = torch.where(ok, idx, 0).long()
+    b = torch.where(ok, val.double() / T, -INF)
+    lp = b - (lse.double()[:, None] if lse is not None else torch.logsumexp(b, 1, keepdim=True))
+    p = torch.where(ok, lp.exp(), 0.0)
+    t = torch.where(p > 0, p * (torch.where(p > 0, lp, 0.0) - lq.gather(1, at)), 0.0)
+    loss, mag = t.sum(1), t.abs().sum(1).detach()
+    if lse is not None:
+        named = torch.zeros(R, V).scatter_add_(1, at, ok.float()) > 0
+        rest = torch.logsumexp(torch.where(named, torch.full_like(z, -INF), z / T), 1) - torch.logsumexp(z / T, 1)
+        pr = (1 - p.sum(1)).clamp(min=0)
+        t = torch.where(pr > 0, pr * (torch.where(pr > 0, pr, 1.0).log() - rest), 0.0)
+        loss, mag = loss + t, mag + t.abs().detach()
+    loss = T * T * loss
+    (g,) = torch.autograd.grad(loss.sum(), z)
+    return loss.detach(), g, T * T * (1 + mag), lq.exp().detach(), torch.zeros(R, V, dtype=torch.float64).scatter_add_(1, at, p)
+
+
+def case(R, V, K, seed, T, tail=True):
+    g = torch.Generator().manual_seed(seed)
+    z = 3 * torch.randn(R, V, generator=g)
+    teacher = 0.7 * z + 1.5 * torch.randn(R, V, generator=g)
+    val, idx = teacher.topk(K, 1)
+    return z, idx, val, torch.logsumexp(teacher / T, 1) if tail else None
+
+
+class Layout:
+    """The same rows as [R, V], or as planes [2, V, R / 4, 2] with the classes in dim 1."""
+
+    def __init__(self, planes, R):
+        self.planes, self.R, self.dim = planes, R, 1 if planes else -1
+
+    def put(self, t):
+        if t is None:
+            return None
+        if self.planes:
+            t = t.view(2, self.R // 4, 2, -1).permute(0, 3, 1, 2).contiguous() if t.dim() == 2 else t.view(2, self.R // 4, 2)
+        return t.to(DEV)
+
+    def back(self, t):
+        t = t.detach().cpu()
+        if t.dim() == 4:
+            return t.permute(0, 2, 3, 1).reshape(self.R, -1)
+        return t.reshape(-1) if self.planes or t.dim() == 0 else t
+
+
+# few short rows, rows of a whole workgroup, rows cut into segments, planes
+FORMS = [(8, 50, False), (8, 3000, False), (4, 40000, False), (8, 64, True)]
+
+
+def bounds(z, T, lossmag, q, p, c, want):
+    D = spread(z, T)
+    return 2 * (D + 8 * 2.0 ** -24) * lossmag, T * c.abs()[:, None] * (2 * D * q + (D + 64 * 2.0 ** -24) * (p + q)) + want.abs() * 2.0 ** -23
+
+
+@pytest.mark.parametrize("R,V,planes", FORMS)
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_the_gradient_is_that_of_the_returned_loss(R, V, planes, reduction):
+    """Weights (0 and others) and upstream gradients: what backward gives is the derivative of what forward returned, for every reduction."""
+    T, K = 2.0, 6
+    z, idx, val, lse = case(R, V, K, V, T)
+    w = torch.linspace(-0.5, 2, R)
+    w[1], w[2] = 0.0, 0.5
+    up = torch.linspace(1.5, -3, R) if reduction == "none" else torch.tensor(0.75)
+    L, g, mag, q, p = formula(z, idx, val, lse, T)
+    n = w.double().sum() if reduction == "mean" else 1.0
+    c = w.double() / n
+    lay = Layout(planes, R)
+    zd = lay.put(z).requires_grad_()
+    loss = TopLogitsDistillLoss(T, lay.dim, reduction)(zd, lay.put(idx), lay.put(val), lay.put(lse), lay.put(w))
+    (dz,) = torch.autograd.grad(loss, zd, lay.put(up) if reduction == "none" else up.to(DEV))
+    want = (c * up.double())[:, None] * g
+    bl, bg = bounds(z, T, mag, q, p, c * up.double(), want)
+    got = lay.back(loss).double()
+    if reduction == "none":
+        assert bool(((got - c * L).abs() <= c.abs() * (bl + L.abs() * 2.0 ** -23)).all())
+    else:
+        assert abs(float(got) - float((c * L).sum())) <= float((c.abs() * bl).sum()) + abs(float((c * L).sum())) * 2.0 ** -23
+    assert bool(((lay.back(dz).double() - want).abs() <= bg).all())
+
+
+def test_a_row_of_weight_zero_has_loss_zero():
+    z, idx, val, lse = case(6, 30, 4, 1, 1.0)
+    z[2] = NAN
+    w = torch.tensor([1.0, 0, 0, 2, 1, 0.5])
+    loss = ops.top_logits_distill(z.to(DEV), idx.to(DEV), val.to(DEV), lse.to(DEV), w.to(DEV), reduction="none")
+    assert float(loss[1]) == 0 and float(loss[2]) == 0 and bool(torch.isfinite(loss).all())
