@@ -245,7 +245,7 @@ def run(state):
         return (y.detach(),) + torch.autograd.grad(y, (state["x"], state["w"]), state["dy"])
     if c["op"] == "top":
         return ops.top_logits(state["z"], c["k"], dim=1, temperature=c["t"])
-    loss = state["loss"](state["z"], state["idx"], state["val"], state["lse"], state["w"])
+    loss = state["loss"](state["z"], state["idx"], state["val"], state["lse"], state["w"] if c["grad"] else None)      # rows' losses by themselves: unweighted
     if not c["grad"]:
         return loss
     return loss.detach(), torch.autograd.grad(loss, state["z"])[0]
