@@ -184,6 +184,14 @@ __device__ inline double wave_total(const double* part, int n) {
     return sum_wave((int)(threadIdx.x & 63) < n ? part[threadIdx.x & 63] : 0.0);
 }
 
+// what a mean multiplies by: inv_norm / (sum of the weights), 0 where they sum to 0.  A sum below 0 is a sum like any other, and one that is NaN or
+// infinite goes on: a mask with a NaN in it gives NaN, not a loss of 0
+__device__ inline double weight_norm(const double* part, int n, double inv_norm, bool* none = nullptr) {
+    const double s = wave_total(part, n);
+    if (none) *none = s == 0.0;
+    return s == 0.0 ? 0.0 : inv_norm / s;
+}
+
 // 2^x, relative error of a few 2^-24 whatever x's size
 __device__ inline float exp2_of(double x) {
     if (!(x > -160.0)) return x != x ? (float)x : 0.f;
@@ -325,8 +333,8 @@ __device__ inline DistillRow finish_row(const DistillArgs& a, size_t r, Lse rest
         if (a.lpart) a.lpart[r] = l;
     }
     double norm = a.inv_norm;
-    if (a.wpart) { const double s = wave_total(a.wpart, a.nwpart); norm = s > 0.0 ? a.inv_norm / s : 0.0; }
-    const double scale = w.have && wrow != 0.f ? (double)a.T * (double)wrow * norm : 0.0;
+    if (a.wpart) norm = weight_norm(a.wpart, a.nwpart, a.inv_norm);
+    const double scale = w.have ? (double)a.T * (double)wrow * norm : 0.0;
     row.inv = 1.f / all.s;
     row.A = rest.s == 0.f ? 0.f : (float)(scale * ((double)exp2_((row.orest - row.oall) * c) / (double)all.s - ratio));   // (no mass outside the entries: nothing to scale)
     row.B = (float)scale;
@@ -614,9 +622,9 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
         }
         if (a.dz) {
             double norm = a.inv_norm;
-            if (a.wpart) { const double s = wave_total(a.wpart, a.nwpart); norm = s > 0.0 ? a.inv_norm / s : 0.0; }
+            if (a.wpart) norm = weight_norm(a.wpart, a.nwpart, a.inv_norm);
             if (a.go && a.go_rows) go = a.go[r];
-            const float B = (float)(have && wrow != 0.f ? (double)a.T * (double)go * (double)wrow * norm : 0.0);
+            const float B = (float)(have ? (double)a.T * (double)go * (double)wrow * norm : 0.0);
             const float A = rest.s == 0.f ? 0.f : (float)((double)B * ((double)exp2_((orest - oall) * c) / (double)all.s - ratio));
             const float inv = 1.f / all.s;
             for (int k = 0; k < K; ++k) {                                // the named classes' gradients into their places
@@ -670,8 +678,9 @@ __global__ __launch_bounds__(1024) void loss_total_kernel(const double* __restri
     s = sum_block<1024>(s, sh);
     if (threadIdx.x >= 64) return;
     double norm = inv_norm;
-    if (wpart) { const double w = wave_total(wpart, nwpart); norm = w > 0.0 ? inv_norm / w : 0.0; }
-    if (threadIdx.x == 0) out[0] = norm != 0.0 ? (float)(s * norm) : 0.f;
+    bool none = false;
+    if (wpart) norm = weight_norm(wpart, nwpart, inv_norm, &none);
+    if (threadIdx.x == 0) out[0] = none ? 0.f : (float)(s * norm);
 }
 
 // How rows are split: 1024 threads hold 256 KB of a row in registers; longer rows, and long ones of fewer than 128, are cut into segments.

@@ -53,6 +53,6 @@ def distill(z, idx, val, lse, w, T, reduction, go=None):
     c = torch.where(live, w, torch.zeros_like(w))
     if reduction == "mean":
         n = w.sum()
-        total = total / n if float(n) > 0 else torch.zeros((), dtype=torch.float64)
-        c = c / n if float(n) > 0 else torch.zeros_like(c)
+        total = total / n if float(n) != 0 else torch.zeros((), dtype=torch.float64)
+        c = c / n if float(n) != 0 else torch.zeros_like(c)
     return total, torch.where(live[:, None], grads * c[:, None], torch.zeros_like(grads)) * (1.0 if go is None else float(go)), torch.tensor(scale)

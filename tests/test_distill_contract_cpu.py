@@ -33,3 +33,14 @@ def test_oracle_weights_each_row():
     z, idx, val, lse, w = case()
     plain, weighted = (tl.distill(z, idx, val, lse, x, 2.0, "none")[0] for x in (None, w))
     assert torch.equal(weighted, w * plain)
+
+
+def test_oracle_mean_of_weights_of_any_sum():
+    z, idx, val, lse, w = case()
+    rows = tl.distill(z, idx, val, lse, None, 2.0, "none")[0]
+    for w in (-w, torch.linspace(-2, 0.5, 7, dtype=torch.float64)):
+        loss, g, _ = tl.distill(z, idx, val, lse, w, 2.0, "mean")
+        assert float(w.sum()) < 0 and abs(float(loss) - float((w * rows).sum() / w.sum())) < 1e-14 and float(g.abs().max()) > 0
+    w[2] = float("nan")
+    loss, g, _ = tl.distill(z, idx, val, lse, w, 2.0, "mean")
+    assert bool(torch.isnan(loss)) and bool(torch.isnan(g).any())

@@ -5,6 +5,8 @@ Bounds.  A sum of exponentials: a thread adds at most 128 of them one after anot
 segments, three roundings each: 176 times 2^-24; an exponential is off by 2^-23 and its argument by three roundings of its size X = range / T:
 D = (178 + 3 X) 2^-24 relative.  A row's loss: D times 1 + the size of its terms, an entry's p by 8 * 2^-24 more; a gradient element: 2 D of its
 q, D + 64 * 2^-24 of its p, half a step of its type."""
+import math
+
 import pytest
 import torch
 
@@ -113,3 +115,34 @@ def test_a_row_of_weight_zero_has_loss_zero():
     w = torch.tensor([1.0, 0, 0, 2, 1, 0.5])
     loss = ops.top_logits_distill(z.to(DEV), idx.to(DEV), val.to(DEV), lse.to(DEV), w.to(DEV), reduction="none")
     assert float(loss[1]) == 0 and float(loss[2]) == 0 and bool(torch.isfinite(loss).all())
+
+
+@pytest.mark.parametrize("R,V,planes", FORMS)
+def test_mean_over_weights_of_any_sum(R, V, planes):
+    """sum w loss / sum w for a negative sum; a NaN or an infinity among the weights is seen; weights that cancel to 0 give 0."""
+    T, K = 2.0, 6
+    z, idx, val, lse = case(R, V, K, V + 1, T)
+    L, g, mag, q, p = formula(z, idx, val, lse, T)
+    lay = Layout(planes, R)
+
+    def run(w):
+        zd = lay.put(z).requires_grad_()
+        loss = TopLogitsDistillLoss(T, lay.dim)(zd, lay.put(idx), lay.put(val), lay.put(lse), lay.put(w))
+        return float(loss.detach()), lay.back(torch.autograd.grad(loss, zd)[0]).double()
+    w = torch.linspace(-2, 0.25, R)
+    loss, dz = run(w)
+    c = w.double() / w.double().sum()
+    want = c[:, None] * g
+    bl, bg = bounds(z, T, mag, q, p, c, want)
+    assert abs(loss - float((c * L).sum())) <= float((c.abs() * bl).sum()) + abs(loss) * 2.0 ** -23
+    assert bool(((dz - want).abs() <= bg).all())
+    w = torch.ones(R)
+    w[1] = NAN
+    loss, dz = run(w)
+    assert math.isnan(loss) and bool(torch.isnan(dz).all())
+    w[1] = INF
+    loss, dz = run(w)
+    assert math.isnan(loss) and bool(torch.isnan(dz[1]).all()) and bool((dz[[0, 2, 3]] == 0).all())   # inf / inf, and 1 / inf
+    w = torch.tensor([1.0, -1.0] * (R // 2))
+    loss, dz = run(w)
+    assert loss == 0 and bool((dz == 0).all())
