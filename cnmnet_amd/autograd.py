@@ -804,10 +804,10 @@ class TopLogitsDistill(torch.autograd.Function):
     def forward(ctx, logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction):
         call = ops.DistillCall(logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction)
         ctx.dz = call.new_grad() if ctx.needs_input_grad[0] and call.reduction else None
-        loss = call.run(True, ctx.dz)
+        loss, ws = call.run(True, ctx.dz)
         if ctx.needs_input_grad[0]:
             ctx.save_for_backward(logits, top_idx, top_logits, top_lse, weight)
-            ctx.call, ctx.captured = call, torch.cuda.is_current_stream_capturing()
+            ctx.call, ctx.ws, ctx.captured = call, ws, torch.cuda.is_current_stream_capturing()
         return loss
 
     @staticmethod
@@ -822,5 +822,5 @@ class TopLogitsDistill(torch.autograd.Function):
         skip = dz is not None
         if dz is None:
             dz = call.new_grad()
-        call.run(False, dz, go.contiguous().float(), skip, call.ws if same else None)
+        call.run(False, dz, go.contiguous().float(), skip, ctx.ws if same else None)
         return call.c.back(dz), None, None, None, None, None, None, None

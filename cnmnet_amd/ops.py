@@ -990,21 +990,19 @@ class DistillCall:
         return torch.empty(self.c.sized(self.c.V), device=self.dev, dtype=self.dtype)
 
     def run(self, need_loss, dz, grad_out=None, skip_if_one=False, ready=None):
-        """Launches; returns the loss (or None).  dz: a new_grad() buffer to fill, or None.  self.ws: the workspace, which a later call for the
-        gradient alone may pass on as `ready`."""
+        """Launches; returns (loss or None, workspace).  dz: a new_grad() buffer to fill, or None.  The workspace of a call for loss and gradient
+        may be passed on as `ready` to later calls for the gradient alone; the workspace of those calls is nobody else's."""
         c = self.c
         loss = torch.empty(c.row_shape if self.reduction == 0 else (), device=self.dev, dtype=torch.float32) if need_loss else None
-        self.ws = ready
         if c.rows == 0:
-            return loss.zero_() if need_loss else None
+            return loss.zero_() if need_loss else None, None
         n = self.lib.cnm_distill_workspace_doubles(DTYPES[self.dtype], c.rows, c.V, c.inner)
-        if ready is None:
-            self.ws = torch.empty(n, device=self.dev, dtype=torch.float64)
+        ws = torch.empty(n, device=self.dev, dtype=torch.float64) if ready is None else ready
         with _on(self.dev):
             _lib.check(self.lib.cnm_distill(_p(c.z), DTYPES[self.dtype], c.ld, _p(self.idx), int(self.idx.dtype == torch.int64), _p(self.val), DTYPES[self.val.dtype],
                                             _p(self.lse), self.T, _p(self.weight), _p(grad_out), int(grad_out is not None and self.reduction == 0), int(skip_if_one),
-                                            self.reduction, _p(loss), _p(dz), _p(self.ws), n, int(ready is not None), c.rows, c.V, self.K, c.inner, _raw_stream(self.dev)))
-        return loss
+                                            self.reduction, _p(loss), _p(dz), _p(ws), n, int(ready is not None), c.rows, c.V, self.K, c.inner, _raw_stream(self.dev)))
+        return loss, ws
 
 
 def top_logits_distill(logits, top_idx, top_logits, top_lse=None, weight=None, temperature=1.0, dim=-1, reduction="mean", grad=False):
@@ -1015,5 +1013,5 @@ def top_logits_distill(logits, top_idx, top_logits, top_lse=None, weight=None, t
     sum weight loss, or "none": weight loss per row.  grad=True: (loss, gradient of the logits) in one pass over them, for programs that call backward on the logits themselves."""
     call = DistillCall(logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction)
     dz = call.new_grad() if grad else None
-    loss = call.run(True, dz)
+    loss, _ = call.run(True, dz)
     return (loss, call.c.back(dz)) if grad else loss

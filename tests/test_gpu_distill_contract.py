@@ -146,3 +146,70 @@ def test_mean_over_weights_of_any_sum(R, V, planes):
     w = torch.tensor([1.0, -1.0] * (R // 2))
     loss, dz = run(w)
     assert loss == 0 and bool((dz == 0).all())
+
+
+@pytest.mark.parametrize("R,V,planes", FORMS)
+def test_backward_passes_eager_and_captured_over_one_forward(R, V, planes):
+    """An eager forward whose backward is captured and run eagerly too, and a captured forward with both: each backward pass gives the gradient,
+    whichever comes first."""
+    T, K = 2.0, 6
+    z, idx, val, lse = case(R, V, K, V + 2, T)
+    w = torch.linspace(0.5, 2, R)
+    lay = Layout(planes, R)
+    args = [lay.put(t) for t in (idx, val, lse, w)]
+    crit = TopLogitsDistillLoss(T, lay.dim)
+    zd = lay.put(z).requires_grad_()
+    up = torch.tensor(2.5, device=DEV)
+    (want,) = torch.autograd.grad(crit(zd, *args), zd, up)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+
+    def eager(loss, n=2):
+        return [torch.autograd.grad(loss, zd, up, retain_graph=True)[0] for _ in range(n)]
+    with torch.cuda.stream(side):                                        # (a captured backward pass runs on its forward's stream: the same for all of them)
+        loss = crit(zd, *args)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        (dg,) = torch.autograd.grad(loss, zd, up, retain_graph=True)
+    with torch.cuda.stream(side):
+        got = eager(loss)                                                # before the graph has run for the first time
+        g.replay()
+        got += eager(loss, 1)
+    torch.cuda.synchronize()
+    for t in got + [dg]:
+        assert torch.equal(t, want)
+    dg.fill_(7.0)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(dg, want)
+
+    f = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(f, stream=side):
+        loss = crit(zd, *args)
+    with torch.cuda.stream(side):
+        f.replay()
+        got = eager(loss, 1)
+    torch.cuda.synchronize()
+    b = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(b, stream=side):
+        (d1,) = torch.autograd.grad(loss, zd, up, retain_graph=True)
+        (d2,) = torch.autograd.grad(loss, zd, up, retain_graph=True)
+    torch.cuda.synchronize()
+    junk = [torch.full((1 << k,), NAN, device=DEV) for k in range(4, 22)]    # whatever was freed is somebody else's by now
+    for r in range(3):
+        if r:                                                            # other inputs in place: the two graphs, replayed in turn, follow
+            with torch.no_grad():
+                zd.copy_(lay.put(z * (1 + 0.1 * r)))
+                args[3].copy_(lay.put(w + r))
+            ze = zd.detach().clone().requires_grad_()
+            (want,) = torch.autograd.grad(crit(ze, *args), ze, up)
+            torch.cuda.synchronize()
+        f.replay()
+        b.replay()
+        torch.cuda.synchronize()
+        for t in (got if r == 0 else []) + [d1, d2]:
+            assert torch.equal(t, want)
+        d1.fill_(7.0), d2.fill_(7.0)
+    del junk
