@@ -66,21 +66,22 @@ __device__ inline float max_wave(float x) {
     return last_lane(x);
 }
 
-// (offset, sum) of exponentials 2^((x - offset) c); offset = -inf: none yet
+// (offset, sum) of exponentials 2^((x - offset) c); offset = -inf: none yet; +inf: the sum is +inf, or NaN
 struct Lse { float o, s; };
+__device__ inline float finite_or_0(float o) { return fabsf(o) == __builtin_huge_valf() ? 0.f : o; }   // what an offset is subtracted as
 __device__ inline Lse lse_join(Lse a, Lse b, float c) {
     const float o = fmaxf(a.o, b.o);                                     // (fmaxf drops a NaN: it is in the sum then)
-    const float so = o == -__builtin_huge_valf() ? 0.f : o;
+    const float so = finite_or_0(o);
     // an empty side has s = 0 and offset -inf: 0 * 2^-inf = 0
     return {o, a.s * exp2_((a.o - so) * c) + b.s * exp2_((b.o - so) * c)};
 }
 __device__ inline Lse lse_wave(Lse a, float c) {
-    const float o = max_wave(a.o), so = o == -__builtin_huge_valf() ? 0.f : o;
+    const float o = max_wave(a.o), so = finite_or_0(o);
     return {o, sum_wave(a.s * exp2_((a.o - so) * c))};
 }
 // the natural logarithm of the sum, in units of 1 / T
 __device__ inline float lse_value(Lse l, float T) {
-    return l.s == 0.f ? -__builtin_huge_valf() : (float)((double)(l.o == -__builtin_huge_valf() ? 0.f : l.o) / (double)T + log((double)l.s));
+    return l.s == 0.f ? -__builtin_huge_valf() : (float)((double)finite_or_0(l.o) / (double)T + log((double)l.s));
 }
 // joined over NT threads in a fixed order; every thread gets the result.  `sh` holds 2 * NT / 64 floats
 template <int NT>
@@ -140,12 +141,12 @@ struct Raw {
     }
 };
 
-// running largest value and sum of the exponentials 2^((x - o) c), o = the largest value (0 while there is none but -inf)
+// running largest value and sum of the exponentials 2^((x - o) c), o = the largest value (0 while there is none but -inf, and where it is +inf)
 struct Run {
     float m = -__builtin_huge_valf(), o = 0.f, s = 0.f;
     __device__ void raise(float x, float c) {                            // a new largest value
         if (m != -__builtin_huge_valf()) s *= exp2_((m - x) * c);
-        m = o = x;
+        m = x; o = finite_or_0(x);
     }
     __device__ Lse lse() const { return {m == -__builtin_huge_valf() ? m : o, s}; }
 };
@@ -275,7 +276,7 @@ __device__ inline Teacher entry_numbers(const DistillArgs& a, size_t r, Entries&
         if (e.dup) for (int j = 0; j < k && first; ++j) first = e.idx[j] != i;
         if (first) {
             const float x = e.z[k];
-            w.named = lse_join(w.named, Lse{x, x == ninf ? 0.f : x == x ? 1.f : x}, c);
+            w.named = lse_join(w.named, Lse{x, x == ninf ? 0.f : 1.f + (x - x)}, c);   // (NaN for an infinite or NaN logit: there is no softmax)
         }
     }
     w.have = __any(have);
@@ -557,7 +558,7 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
                     const float x = tile[i * 64 + px];
                     ez[k * 64 + px] = x;
                     tile[i * 64 + px] = ninf;
-                    named = lse_join(named, Lse{x, x == ninf ? 0.f : x == x ? 1.f : x}, c);
+                    named = lse_join(named, Lse{x, x == ninf ? 0.f : 1.f + (x - x)}, c);
                 }
             }
         }
@@ -906,7 +907,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 256 && NV == 16 ? 4 : 1)
         for (int j = 1; j < E; ++j) vm[i] = fmaxf(vm[i], x[i].get(j));
         m = fmaxf(m, vm[i]);
     }
-    const float o = m == ninf ? 0.f : m;
+    const float o = finite_or_0(m);
     Lse l = {m, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -914,7 +915,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 256 && NV == 16 ? 4 : 1)
 #pragma unroll
         for (int j = 0; j < E; ++j) l.s += exp2_((x[i].get(j) - o) * c);
     }
-    const bool odd = l.s != l.s;                                         // a NaN or +inf here: every vector is looked at
+    const bool odd = l.s != l.s;                                         // a NaN here: every vector is looked at
     l = lse_block<NT>(l, c, sh.shf);
     const float low = kth_bound<NT>(m, a.K, sh.shf);
     if (a.segments == 1) { if (t == 0) a.lse[r] = lse_value(l, a.T); }

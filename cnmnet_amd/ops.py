@@ -933,7 +933,7 @@ def _temperature(t):
 def top_logits(logits, k, dim=-1, temperature=1.0):
     """What a teacher's cache holds of its logits: (values, indices int32, lse) with the k largest logits along `dim` in descending order --
     ties: the lower class first; NaN above everything --, their classes, and lse = log sum exp(logits / temperature) over all classes
-    (float32).  logits: float32 / float16 / bfloat16, any shape; classes along the last dim are read in place (row stride allowed), classes
+    (float32; +inf where a logit is, NaN where one is).  logits: float32 / float16 / bfloat16, any shape; classes along the last dim are read in place (row stride allowed), classes
     along an inner dim ([B, planes, H, W], dim=1) too for k <= 16.  k <= 256."""
     dev = _dev_any(logits)
     T = _temperature(temperature)

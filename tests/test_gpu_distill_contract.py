@@ -213,3 +213,41 @@ def test_backward_passes_eager_and_captured_over_one_forward(R, V, planes):
             assert torch.equal(t, want)
         d1.fill_(7.0), d2.fill_(7.0)
     del junk
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("R,V,planes", FORMS + [(300, 40000, False), (8, 700, False)])
+def test_log_sum_exp_of_infinite_logits(R, V, planes, dtype):
+    """+inf among the logits: the log-sum-exp is +inf; NaN beside it: NaN; the values and classes as ever."""
+    lay = Layout(planes, R)
+    z = torch.randn(R, V, generator=torch.Generator().manual_seed(V)).to(dtype)
+    z[0, 3] = INF
+    z[1, V - 1], z[1, 0] = INF, -INF
+    z[2, 1:] = INF
+    z[3, 5], z[3, 7] = INF, NAN
+    val, idx, lse = ops.top_logits(lay.put(z), 4, dim=lay.dim, temperature=2.0)
+    lse, val, idx = lay.back(lse), lay.back(val), lay.back(idx)
+    assert bool((lse[:3] == INF).all()) and bool(torch.isnan(lse[3]))
+    assert idx[0, 0] == 3 and idx[1, 0] == V - 1 and idx[2].tolist() == [1, 2, 3, 4] and idx[3, :2].tolist() == [7, 5]
+    assert bool((val[[0, 1], 0] == INF).all()) and bool((val[2] == INF).all())
+    if R > 4:
+        ref = torch.logsumexp(z[4:].double() / 2, 1)
+        assert bool(((lse[4:].double() - ref).abs() <= spread(z[4:], 2.0) + ref.abs() * 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("R,V,planes", FORMS)
+@pytest.mark.parametrize("tail", [False, True])
+def test_an_infinite_student_logit_has_no_softmax(R, V, planes, tail):
+    """+inf at a named or an unnamed class: loss and gradient of that row are NaN, the other rows' are as ever."""
+    T, K = 2.0, 6
+    z, idx, val, lse = case(R, V, K, V + 5, T, tail)
+    named = torch.zeros(R, V, dtype=torch.bool).scatter_(1, idx, True)
+    z[0, idx[0, 2]] = INF
+    z[1, int((~named[1]).nonzero()[7])] = INF
+    lay = Layout(planes, R)
+    zd = lay.put(z).requires_grad_()
+    loss = TopLogitsDistillLoss(T, lay.dim, "none")(zd, lay.put(idx), lay.put(val), lay.put(lse))
+    dz = lay.back(torch.autograd.grad(loss.sum(), zd)[0])
+    loss = lay.back(loss)
+    assert bool(torch.isnan(loss[:2]).all()) and bool(torch.isnan(dz[:2]).all())
+    assert bool(torch.isfinite(loss[2:]).all()) and bool(torch.isfinite(dz[2:]).all())
