@@ -794,6 +794,10 @@ def top_logits_distill(logits, top_idx, top_logits, top_lse=None, weight=None, t
     return TopLogitsDistill.apply(logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction)
 
 
+def _kinds(*tensors):
+    return [None if t is None else (t.shape, t.dtype, t.device) for t in tensors]
+
+
 class TopLogitsDistill(torch.autograd.Function):
     """ops.top_logits_distill on the tape; gradient to the logits only.  For "mean" and "sum" the gradient is written by the forward launch, which
     has the row at hand, and the backward pass only looks at the upstream gradient: where it is 1 (the loss is the root) there is nothing left
@@ -804,17 +808,20 @@ class TopLogitsDistill(torch.autograd.Function):
     def forward(ctx, logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction):
         call = ops.DistillCall(logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction)
         ctx.dz = call.new_grad() if ctx.needs_input_grad[0] and call.reduction else None
-        loss, ws = call.run(True, ctx.dz)
+        data = call.take()
+        loss, ws = call.run(data, True, ctx.dz)
         if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(logits, top_idx, top_logits, top_lse, weight)
-            ctx.call, ctx.ws, ctx.captured = call, ws, torch.cuda.is_current_stream_capturing()
+            ctx.save_for_backward(*data, ws)                             # (what the launch read, copies among them: the tape frees it, and its hooks may move it)
+            ctx.call, ctx.kinds, ctx.captured = call, _kinds(*data, ws), torch.cuda.is_current_stream_capturing()
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, go):
-        ctx.saved_tensors                                                # (raises if one of them has been changed in place, or the graph freed)
+        *data, ws = ctx.saved_tensors                                    # (raises if one of them has been changed in place, or the graph freed)
         call = ctx.call
+        if _kinds(*data, ws) != ctx.kinds:
+            raise _lib.EngineError("top_logits_distill: saved tensors came back as %s instead of %s" % (_kinds(*data, ws), ctx.kinds))
         # the forward's gradient serves one backward pass (its buffer is given away); it and the forward's workspace do not serve a captured
         # backward pass of an eager forward, which is replayed
         same = ctx.captured == torch.cuda.is_current_stream_capturing()
@@ -822,5 +829,5 @@ class TopLogitsDistill(torch.autograd.Function):
         skip = dz is not None
         if dz is None:
             dz = call.new_grad()
-        call.run(False, dz, go.contiguous().float(), skip, ctx.ws if same else None)
+        call.run(data, False, dz, go.contiguous().float(), skip, ws if same else None)
         return call.c.back(dz), None, None, None, None, None, None, None

@@ -958,7 +958,8 @@ REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
 class DistillCall:
-    """One checked call of the distillation loss, its arguments laid out for the engine (ops.top_logits_distill, autograd.TopLogitsDistill)."""
+    """One checked call of the distillation loss (ops.top_logits_distill, autograd.TopLogitsDistill).  take() gives its tensors, laid out for the
+    engine, to whoever runs the call: an object that lives as long as a loss does holds none of them."""
 
     def __init__(self, logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction):
         self.dev = _dev_any(logits, top_logits, top_lse, weight)
@@ -982,26 +983,34 @@ class DistillCall:
             if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != tuple(c.row_shape)):
                 raise _lib.EngineError("%s must be float32 %s; got %s %s" % (name, tuple(c.row_shape), t.dtype, tuple(t.shape)))
         self.dtype = logits.dtype
-        self.idx, self.val = c.entries(top_idx), c.entries(top_logits)
-        self.lse = None if top_lse is None else top_lse.contiguous()
-        self.weight = None if weight is None else weight.contiguous()
+        self.data = (c.z, c.entries(top_idx), c.entries(top_logits), None if top_lse is None else top_lse.contiguous(), None if weight is None else weight.contiguous())
+
+    def take(self):
+        """(logits, indices, entries' logits, lse, weight), which are not held here any longer."""
+        data, self.data, self.c.z = self.data, None, None
+        return data
 
     def new_grad(self):
         return torch.empty(self.c.sized(self.c.V), device=self.dev, dtype=self.dtype)
 
-    def run(self, need_loss, dz, grad_out=None, skip_if_one=False, ready=None):
-        """Launches; returns (loss or None, workspace).  dz: a new_grad() buffer to fill, or None.  The workspace of a call for loss and gradient
-        may be passed on as `ready` to later calls for the gradient alone; the workspace of those calls is nobody else's."""
+    def run(self, data, need_loss, dz, grad_out=None, skip_if_one=False, ready=None):
+        """Launches on what take() gave (the same values: their strides may have changed on the tape); returns (loss or None, workspace).  dz: a
+        new_grad() buffer to fill, or None.  The workspace of a call for loss and gradient may be passed on as `ready` to later calls for the
+        gradient alone; the workspace of those calls is nobody else's."""
         c = self.c
+        idx, val, lse, weight = (None if t is None else t.contiguous() for t in data[1:])
+        strided = c.ld != c.V and data[0].stride(1) == 1 and data[0].stride(0) >= c.V
+        z = data[0] if strided else data[0].contiguous()
+        ld = z.stride(0) if strided else c.V
         loss = torch.empty(c.row_shape if self.reduction == 0 else (), device=self.dev, dtype=torch.float32) if need_loss else None
         if c.rows == 0:
             return loss.zero_() if need_loss else None, None
         n = self.lib.cnm_distill_workspace_doubles(DTYPES[self.dtype], c.rows, c.V, c.inner)
         ws = torch.empty(n, device=self.dev, dtype=torch.float64) if ready is None else ready
         with _on(self.dev):
-            _lib.check(self.lib.cnm_distill(_p(c.z), DTYPES[self.dtype], c.ld, _p(self.idx), int(self.idx.dtype == torch.int64), _p(self.val), DTYPES[self.val.dtype],
-                                            _p(self.lse), self.T, _p(self.weight), _p(grad_out), int(grad_out is not None and self.reduction == 0), int(skip_if_one),
-                                            self.reduction, _p(loss), _p(dz), _p(ws), n, int(ready is not None), c.rows, c.V, self.K, c.inner, _raw_stream(self.dev)))
+            _lib.check(self.lib.cnm_distill(_p(z), DTYPES[self.dtype], ld, _p(idx), int(idx.dtype == torch.int64), _p(val), DTYPES[val.dtype],
+                                            _p(lse), self.T, _p(weight), _p(grad_out), int(grad_out is not None and self.reduction == 0), int(skip_if_one),
+                                            self.reduction, _p(loss), _p(dz), _p(ws), ws.numel(), int(ready is not None), c.rows, c.V, self.K, c.inner, _raw_stream(self.dev)))
         return loss, ws
 
 
@@ -1010,8 +1019,9 @@ def top_logits_distill(logits, top_idx, top_logits, top_lse=None, weight=None, t
     T^2 KL(teacher || student) with the teacher's classes outside the entries lumped into one (top_lse given), or the entries renormalised
     (top_lse None); include/cnm_engine.h states the formula.  top_idx (int32 / int64; an index outside the classes is no entry) and top_logits
     have K in the place of the classes; top_lse and weight are float32 without that dim.  reduction "mean": sum weight loss / sum weight, "sum":
-    sum weight loss, or "none": weight loss per row.  grad=True: (loss, gradient of the logits) in one pass over them, for programs that call backward on the logits themselves."""
+    sum weight loss, or "none": weight loss per row.  grad=True: (loss, gradient of the logits) in one pass over them, for programs that call backward on
+    the logits themselves."""
     call = DistillCall(logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction)
     dz = call.new_grad() if grad else None
-    loss, _ = call.run(True, dz)
+    loss, _ = call.run(call.take(), True, dz)
     return (loss, call.c.back(dz)) if grad else loss

@@ -10,7 +10,7 @@ import math
 import pytest
 import torch
 
-from cnmnet_amd import ops
+from cnmnet_amd import _lib, ops
 from cnmnet_amd.depthnet.losses import TopLogitsDistillLoss
 
 pytestmark = pytest.mark.gpu
@@ -251,3 +251,61 @@ def test_an_infinite_student_logit_has_no_softmax(R, V, planes, tail):
     loss = lay.back(loss)
     assert bool(torch.isnan(loss[:2]).all()) and bool(torch.isnan(dz[:2]).all())
     assert bool(torch.isfinite(loss[2:]).all()) and bool(torch.isfinite(dz[2:]).all())
+
+
+def test_nothing_is_held_after_backward():
+    """A loss that is kept (for a log) holds none of the step's memory once its backward pass has run."""
+    R, V, K = 512, 16384, 8
+    leaf = torch.randn(V, R, device=DEV, requires_grad=True)             # classes strided: the operator works on a copy
+    idx = torch.zeros(R, K, device=DEV, dtype=torch.int64) + torch.arange(K, device=DEV)
+    crit = TopLogitsDistillLoss()
+    torch.autograd.grad(crit(leaf.t(), idx, torch.randn(R, K, device=DEV)), leaf)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    loss = crit(leaf.t(), idx, torch.randn(R, K, device=DEV))
+    torch.autograd.grad(loss, leaf)
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() - before <= 4096
+    assert bool(torch.isfinite(loss))
+
+
+def test_saved_tensors_follow_the_hooks():
+    """torch.autograd.graph.save_on_cpu: the logits leave the card between the passes, and the gradient is the same."""
+    R, V, K = 512, 16384, 8
+    z0 = torch.randn(R, V, device=DEV, requires_grad=True)
+    idx = torch.zeros(R, K, device=DEV, dtype=torch.int64) + torch.arange(K, device=DEV)
+    val = torch.randn(R, K, device=DEV)
+    for reduction in ("mean", "none"):
+        crit = TopLogitsDistillLoss(reduction=reduction)
+        (want,) = torch.autograd.grad((crit(z0 * 2, idx, val) * 3).sum(), z0)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        with torch.autograd.graph.save_on_cpu():
+            z = z0 * 2
+            loss = (crit(z, idx, val) * 3).sum()
+        del z
+        torch.cuda.synchronize()
+        held = torch.cuda.memory_allocated() - before
+        assert held <= (1.1 if reduction == "mean" else 0.1) * R * V * 4     # "mean": the gradient itself is already there
+        assert torch.equal(torch.autograd.grad(loss, z0)[0], want)
+
+
+def test_saved_rows_come_back_dense():
+    """Logits that are columns of a wider matrix lose their row stride on the way to the host and back; a hook that changes more is refused."""
+    R, V, K = 40, 300, 5
+    wide = torch.randn(R, V + 31, device=DEV, requires_grad=True)
+    idx = torch.zeros(R, K, device=DEV, dtype=torch.int64) + torch.arange(K, device=DEV)
+    val = torch.randn(R, 2 * K, device=DEV)[:, ::2]
+    crit = TopLogitsDistillLoss()
+    (want,) = torch.autograd.grad(crit(wide[:, 3:V + 3], idx, val) * 3, wide)
+    with torch.autograd.graph.save_on_cpu():
+        loss = crit(wide[:, 3:V + 3], idx, val) * 3
+    assert torch.equal(torch.autograd.grad(loss, wide)[0], want)
+    for change in (lambda t: t.half() if t.is_floating_point() else t, lambda t: t[:1], lambda t: t.cpu()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            loss = crit(wide[:, 3:V + 3], idx, val)
+            with pytest.raises(_lib.EngineError, match="came back"):
+                torch.autograd.grad(loss * 3, wide)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2 else t):
+        loss = crit(wide[:, 3:V + 3], idx, val)
+        assert torch.equal(torch.autograd.grad(loss * 3, wide)[0], want)
