@@ -802,7 +802,8 @@ def quantize_fp8(x, block_rows=1, transposed=False):
     """x [..., C] float32 / float16 / bfloat16 -> (q [R, C padded to 128] float8_e4m3fn, scale float8_e8m0fnu), R the product of the leading
     sizes: one power of two per 1 x 128 block (block_rows 1: scale [R, ceil(C/128)]) or 128 x 128 block (block_rows 128: scale [ceil(R/128),
     ceil(C/128)]); include/cnm_engine.h states the format.  transposed=True also returns (q_t [C, R padded to 128], scale_t), the same for x^T
-    (blocked along the rows), from the same pass over x."""
+    (blocked along the rows), from the same pass over x.  The values remember the length of the axis that was padded (attribute `columns`; a copy
+    of the tensor does not): linear_fp8 and matmul_fp8 refuse a partner of another length where they know it."""
     dev = _dev_any(x)
     if block_rows not in (1, 128):
         raise _lib.EngineError("block_rows must be 1 or 128; got %r" % (block_rows,))
@@ -811,10 +812,12 @@ def quantize_fp8(x, block_rows=1, transposed=False):
     Cb, Rb = (C + 127) // 128, (R + 127) // 128
     q = torch.empty(R, Cb * 128, device=dev, dtype=torch.float8_e4m3fn)
     s = torch.empty(R if block_rows == 1 else Rb, Cb, device=dev, dtype=torch.float8_e8m0fnu)
+    q.columns = C
     out = (q, s)
     if transposed:
         out += (torch.empty(C, Rb * 128, device=dev, dtype=torch.float8_e4m3fn),
                 torch.empty(C if block_rows == 1 else Cb, Rb, device=dev, dtype=torch.float8_e8m0fnu))
+        out[2].columns = R
     if R:
         with _on(dev):
             _lib.check(_lib.load().cnm_quantize_fp8(_p(x), DTYPES[x.dtype], ld, R, C, block_rows, _p(q), _p(s), *([_p(t) for t in out[2:]] or [0, 0]), _raw_stream(dev)))
@@ -850,6 +853,9 @@ def matmul_fp8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
     bb = _fp8_operand(b, b_scale, "matmul_fp8 b", per_block=True)
     if a.device != b.device or a.shape[1] != b.shape[1]:
         raise _lib.EngineError("matmul_fp8: operands %s on %s and %s on %s" % (tuple(a.shape), a.device, tuple(b.shape), b.device))
+    ka, kb = getattr(a, "columns", None), getattr(b, "columns", None)
+    if ka is not None and kb is not None and ka != kb:
+        raise _lib.EngineError("matmul_fp8: operands of %d and %d columns, both padded to %d" % (ka, kb, a.shape[1]))
     if dtype not in DTYPES:
         raise _lib.EngineError("matmul_fp8 gives float32, float16 or bfloat16; got %s" % dtype)
     M, N, K = a.shape[0], b.shape[0], a.shape[1]
@@ -871,6 +877,8 @@ def linear_fp8(x, w_packed, w_scale):
         raise _lib.EngineError("linear_fp8: x on %s, weight on %s" % (dev, w_packed.device))
     if x.dim() == 0 or (x.shape[-1] + 127) // 128 * 128 != w_packed.shape[1]:
         raise _lib.EngineError("linear_fp8: x %s does not fit a weight packed as %s" % (tuple(x.shape), tuple(w_packed.shape)))
+    if getattr(w_packed, "columns", x.shape[-1]) != x.shape[-1]:
+        raise _lib.EngineError("linear_fp8: x %s does not fit a weight of %d columns" % (tuple(x.shape), w_packed.columns))
     x2, ld = _rows2d(x, "linear_fp8")
     (M, K), N = x2.shape, w_packed.shape[0]
     y = torch.empty(x.shape[:-1] + (N,), device=dev, dtype=x.dtype)
