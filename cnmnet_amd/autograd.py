@@ -794,10 +794,6 @@ def top_logits_distill(logits, top_idx, top_logits, top_lse=None, weight=None, t
     return TopLogitsDistill.apply(logits, top_idx, top_logits, top_lse, weight, temperature, dim, reduction)
 
 
-def _kinds(*tensors):
-    return [None if t is None else (t.shape, t.dtype, t.device) for t in tensors]
-
-
 class TopLogitsDistill(torch.autograd.Function):
     """ops.top_logits_distill on the tape; gradient to the logits only.  For "mean" and "sum" the gradient is written by the forward launch, which
     has the row at hand, and the backward pass only looks at the upstream gradient: where it is 1 (the loss is the root) there is nothing left
@@ -812,16 +808,15 @@ class TopLogitsDistill(torch.autograd.Function):
         loss, ws = call.run(data, True, ctx.dz)
         if ctx.needs_input_grad[0]:
             ctx.save_for_backward(*data, ws)                             # (what the launch read, copies among them: the tape frees it, and its hooks may move it)
-            ctx.call, ctx.kinds, ctx.captured = call, _kinds(*data, ws), torch.cuda.is_current_stream_capturing()
+            ctx.call, ctx.captured = call, torch.cuda.is_current_stream_capturing()
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, go):
-        *data, ws = ctx.saved_tensors                                    # (raises if one of them has been changed in place, or the graph freed)
+        saved = ctx.saved_tensors                                        # (raises if one of them has been changed in place, or the graph freed)
         call = ctx.call
-        if _kinds(*data, ws) != ctx.kinds:
-            raise _lib.EngineError("top_logits_distill: saved tensors came back as %s instead of %s" % (_kinds(*data, ws), ctx.kinds))
+        data, ld = call.again(*saved)
         # the forward's gradient serves one backward pass (its buffer is given away); it and the forward's workspace do not serve a captured
         # backward pass of an eager forward, which is replayed
         same = ctx.captured == torch.cuda.is_current_stream_capturing()
@@ -829,5 +824,5 @@ class TopLogitsDistill(torch.autograd.Function):
         skip = dz is not None
         if dz is None:
             dz = call.new_grad()
-        call.run(data, False, dz, go.contiguous().float(), skip, ws if same else None)
+        call.run(data, False, dz, go.contiguous().float(), skip, saved[5] if same else None, ld)
         return call.c.back(dz), None, None, None, None, None, None, None

@@ -16,6 +16,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..autograd import top_logits_distill
+
 
 def total(x):
     """Sum of all elements (integer for a bool mask) as rows of 256, then the row sums, until at most 1024 values are left.
@@ -131,5 +133,4 @@ class TopLogitsDistillLoss(nn.Module):
         self.temperature, self.dim, self.reduction = temperature, dim, reduction
 
     def forward(self, logits, top_idx, top_logits, top_lse=None, weight=None):
-        from ..autograd import top_logits_distill
         return top_logits_distill(logits, top_idx, top_logits, top_lse, weight, self.temperature, self.dim, self.reduction)

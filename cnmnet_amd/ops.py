@@ -984,11 +984,11 @@ class DistillCall:
         self.c = c = _Classes(logits, dim, lambda V: bool(self.lib.cnm_distill_planes_ok(V, K)))
         if not 1 <= K <= self.lib.cnm_distill_max_entries() or c.V > self.lib.cnm_distill_max_classes():
             raise _lib.EngineError("%d entries over %d classes: at most %d over %d" % (K, c.V, self.lib.cnm_distill_max_entries(), self.lib.cnm_distill_max_classes()))
-        want = tuple(c.shape[:c.dim]) + (K,) + tuple(c.shape[c.dim + 1:])
-        if tuple(top_idx.shape) != want or tuple(top_logits.shape) != want:
+        want = c.shape[:c.dim] + (K,) + c.shape[c.dim + 1:]
+        if top_idx.shape != want or top_logits.shape != want:
             raise _lib.EngineError("top_idx %s and top_logits %s: both must be %s" % (tuple(top_idx.shape), tuple(top_logits.shape), want))
         for name, t in (("top_lse", top_lse), ("weight", weight)):
-            if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != tuple(c.row_shape)):
+            if t is not None and (t.dtype != torch.float32 or t.shape != c.row_shape):
                 raise _lib.EngineError("%s must be float32 %s; got %s %s" % (name, tuple(c.row_shape), t.dtype, tuple(t.shape)))
         self.dtype = logits.dtype
         self.data = (c.z, c.entries(top_idx), c.entries(top_logits), None if top_lse is None else top_lse.contiguous(), None if weight is None else weight.contiguous())
@@ -996,27 +996,40 @@ class DistillCall:
     def take(self):
         """(logits, indices, entries' logits, lse, weight), which are not held here any longer."""
         data, self.data, self.c.z = self.data, None, None
+        self.kinds = self.dtype, data[1].dtype, data[2].dtype, data[3] is None, data[4] is None
         return data
+
+    def again(self, z, idx, val, lse, weight, ws):
+        """What take() gave and run() left, back from the tape -> (tensors, row stride) for run(): the same values, but hooks may have brought them
+        back with other strides; anything else would send the launch out of bounds."""
+        c, i = self.c, self.dev.index
+        rows, entries, f32 = c.rows, c.rows * self.K, torch.float32
+        if not ((z.dtype, idx.dtype, val.dtype, lse is None, weight is None) == self.kinds and z.numel() == rows * c.V and idx.numel() == val.numel() == entries
+                and z.get_device() == idx.get_device() == val.get_device() == i
+                and (lse is None or lse.numel() == rows and lse.dtype is f32 and lse.get_device() == i)
+                and (weight is None or weight.numel() == rows and weight.dtype is f32 and weight.get_device() == i)
+                and (ws is None or ws.dtype is torch.float64 and ws.get_device() == i) and (c.ld == c.V or z.dim() == 2)):
+            raise _lib.EngineError("top_logits_distill: a saved tensor came back as something else")
+        if c.ld == c.V or z.stride(1) != 1 or z.stride(0) < c.V:
+            z = z.contiguous()
+        return ((z, idx.contiguous(), val.contiguous(), None if lse is None else lse.contiguous(), None if weight is None else weight.contiguous()),
+                c.V if c.ld == c.V else z.stride(0))
 
     def new_grad(self):
         return torch.empty(self.c.sized(self.c.V), device=self.dev, dtype=self.dtype)
 
-    def run(self, data, need_loss, dz, grad_out=None, skip_if_one=False, ready=None):
-        """Launches on what take() gave (the same values: their strides may have changed on the tape); returns (loss or None, workspace).  dz: a
-        new_grad() buffer to fill, or None.  The workspace of a call for loss and gradient may be passed on as `ready` to later calls for the
-        gradient alone; the workspace of those calls is nobody else's."""
-        c = self.c
-        idx, val, lse, weight = (None if t is None else t.contiguous() for t in data[1:])
-        strided = c.ld != c.V and data[0].stride(1) == 1 and data[0].stride(0) >= c.V
-        z = data[0] if strided else data[0].contiguous()
-        ld = z.stride(0) if strided else c.V
+    def run(self, data, need_loss, dz, grad_out=None, skip_if_one=False, ready=None, ld=None):
+        """Launches on what take() or again() gave; returns (loss or None, workspace).  dz: a new_grad() buffer to fill, or None.  The workspace of a
+        call for loss and gradient may be passed on as `ready` to later calls for the gradient alone; the workspace of those calls is nobody else's."""
+        c, (z, idx, val, lse, weight) = self.c, data
         loss = torch.empty(c.row_shape if self.reduction == 0 else (), device=self.dev, dtype=torch.float32) if need_loss else None
         if c.rows == 0:
             return loss.zero_() if need_loss else None, None
-        n = self.lib.cnm_distill_workspace_doubles(DTYPES[self.dtype], c.rows, c.V, c.inner)
-        ws = torch.empty(n, device=self.dev, dtype=torch.float64) if ready is None else ready
+        ws = ready
+        if ws is None:
+            ws = torch.empty(self.lib.cnm_distill_workspace_doubles(DTYPES[self.dtype], c.rows, c.V, c.inner), device=self.dev, dtype=torch.float64)
         with _on(self.dev):
-            _lib.check(self.lib.cnm_distill(_p(z), DTYPES[self.dtype], ld, _p(idx), int(idx.dtype == torch.int64), _p(val), DTYPES[val.dtype],
+            _lib.check(self.lib.cnm_distill(_p(z), DTYPES[self.dtype], ld or c.ld, _p(idx), int(idx.dtype == torch.int64), _p(val), DTYPES[val.dtype],
                                             _p(lse), self.T, _p(weight), _p(grad_out), int(grad_out is not None and self.reduction == 0), int(skip_if_one),
                                             self.reduction, _p(loss), _p(dz), _p(ws), ws.numel(), int(ready is not None), c.rows, c.V, self.K, c.inner, _raw_stream(self.dev)))
         return loss, ws
