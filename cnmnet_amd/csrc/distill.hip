@@ -177,8 +177,9 @@ struct DistillArgs {
     int segments, seglen;
 };
 
-// What a row amounts to: an unnamed class's gradient is A 2^((z - orest) c), a named one's B (2^((z - oall) c) inv - p); B = 0: nothing
-struct DistillRow { double L; float A, B, orest, oall, inv, pad; };
+// What a row amounts to: an unnamed class's gradient is A 2^((z - orest) c), a named one's B (2^((z - oall) c) inv - p); B = 0: nothing.  A and B
+// for an upstream gradient of 1, in fp64: with the upstream gradient they become fp32, and only that product has to be one
+struct DistillRow { double L, A, B; float orest, oall, inv, pad; };
 
 // sum of up to 64 partial sums, in a fixed order, by a whole wave
 __device__ inline double wave_total(const double* part, int n) {
@@ -337,8 +338,8 @@ __device__ inline DistillRow finish_row(const DistillArgs& a, size_t r, Lse rest
     if (a.wpart) norm = weight_norm(a.wpart, a.nwpart, a.inv_norm);
     const double scale = w.have ? (double)a.T * (double)wrow * norm : 0.0;
     row.inv = 1.f / all.s;
-    row.A = rest.s == 0.f ? 0.f : (float)(scale * ((double)exp2_((row.orest - row.oall) * c) / (double)all.s - ratio));   // (no mass outside the entries: nothing to scale)
-    row.B = (float)scale;
+    row.A = rest.s == 0.f ? 0.0 : scale * ((double)exp2_((row.orest - row.oall) * c) / (double)all.s - ratio);   // (no mass outside the entries: nothing to scale)
+    row.B = scale;
     row.pad = 0.f;
     return row;
 }
@@ -434,7 +435,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 512 && NV == 8 ? 6 : 1) 
     if (t < 64) {                                                        // the named classes' gradients, each once, and which class each belongs to
         join_entries(e, a.K, lane);
         const DistillRow w = e.row;
-        const float B = w.B * go;
+        const float B = (float)(w.B * (double)go);
         for (int k = lane; k < a.K; k += 64) {
             const int i = e.idx[k] - v0;
             if (e.idx[k] >= 0 && i >= 0 && i < n) {
@@ -445,8 +446,8 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT, NT == 512 && NV == 8 ? 6 : 1) 
         }
     }
     row_sync<NT>();
-    const float A = e.row.A * go, orest = e.row.orest;
-    const bool zero = e.row.B * go == 0.f;                               // rows that count for nothing: zeros, whatever the logits hold
+    const float A = (float)(e.row.A * (double)go), orest = e.row.orest;
+    const bool zero = (float)(e.row.B * (double)go) == 0.f;                // rows that count for nothing: zeros, whatever the logits hold
     T* const dz = static_cast<T*>(a.dz) + r * a.V + v0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -625,8 +626,9 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
             double norm = a.inv_norm;
             if (a.wpart) norm = weight_norm(a.wpart, a.nwpart, a.inv_norm);
             if (a.go && a.go_rows) go = a.go[r];
-            const float B = (float)(have ? (double)a.T * (double)go * (double)wrow * norm : 0.0);
-            const float A = rest.s == 0.f ? 0.f : (float)((double)B * ((double)exp2_((orest - oall) * c) / (double)all.s - ratio));
+            const double scale = have ? (double)a.T * (double)go * (double)wrow * norm : 0.0;
+            const float B = (float)scale;
+            const float A = rest.s == 0.f ? 0.f : (float)(scale * ((double)exp2_((orest - oall) * c) / (double)all.s - ratio));
             const float inv = 1.f / all.s;
             for (int k = 0; k < K; ++k) {                                // the named classes' gradients into their places
                 const int i = eidx[k * 64 + px];

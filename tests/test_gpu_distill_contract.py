@@ -309,3 +309,22 @@ def test_saved_rows_come_back_dense():
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2 else t):
         loss = crit(wide[:, 3:V + 3], idx, val)
         assert torch.equal(torch.autograd.grad(loss * 3, wide)[0], want)
+
+
+@pytest.mark.parametrize("R,V,planes", FORMS)
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_tiny_weights_times_large_upstream_gradients(R, V, planes, reduction):
+    """Only their product has to be a float32: neither is rounded before it meets the other."""
+    T, K = 1.7, 6
+    z, idx, val, lse = case(R, V, K, V + 3, T)
+    w = torch.full((R,), 1e-43)
+    up = torch.tensor(1e35)
+    L, g, mag, q, p = formula(z, idx, val, lse, T)
+    lay = Layout(planes, R)
+    zd = lay.put(z).requires_grad_()
+    loss = TopLogitsDistillLoss(T, lay.dim, reduction)(zd, lay.put(idx), lay.put(val), lay.put(lse), lay.put(w))
+    (dz,) = torch.autograd.grad(loss, zd, up.to(DEV).expand(loss.shape))
+    c = w.double() * up.double()
+    want = c[:, None] * g
+    _, bg = bounds(z, T, mag, q, p, c, want)
+    assert bool(((lay.back(dz).double() - want).abs() <= bg).all())
