@@ -9,7 +9,7 @@
 // with p_r = max(0, 1 - sum p_k) and q_r = sum of q over the classes that no entry names, only if L is given and such classes have mass.
 //     d loss / d z_v = T (q_v - sum_{k: i_k = v} p_k)      for a named class, and for every class when renormalised;
 //                    = T q_v (1 - p_r / q_r)               for the others when L is given.
-// The same class may be named twice (its p add up).  A row without entries: loss 0, gradient 0.
+// The same class may be named twice (its p add up).  A row without entries, or with none but -inf to renormalise: loss 0, gradient 0.
 //
 // Numerics: q_v = 2^((z_v - o) c) / S with c = log2(e) / T and the row's largest logit o: fp32; the difference first, so that a row of the type's
 // lowest values neither overflows nor loses its ratios.  Sums of exponentials in fp32 per thread, joined across threads with their offsets.  The row's few scalars -- lse, log p, log q,
@@ -288,7 +288,9 @@ __device__ inline Teacher entry_numbers(const DistillArgs& a, size_t r, Entries&
         if (best == ninf) best = 0.f;
         double s = 0.0;
         for (int k = lane; k < a.K; k += 64) if (e.idx[k] >= 0) s += (double)exp2_of(((double)e.p[k] - (double)best) * a.l2T);
-        w.L = (double)best * a.iT + log(sum_wave(s));
+        s = sum_wave(s);
+        w.L = (double)best * a.iT + log(s);
+        if (s == 0.0) { w.L = 0.0; w.have = 0; }                         // entries of -inf: no mass, no entries
     }
     double P = 0.0, lp = 0.0;
     for (int k = lane; k < a.K; k += 64) {
@@ -296,7 +298,7 @@ __device__ inline Teacher entry_numbers(const DistillArgs& a, size_t r, Entries&
         if (e.idx[k] >= 0) {
             const double l = entry_log2p(a, e.p[k], w.L);
             p = exp2_of(l);
-            if (p > 0.f) lp += (double)p * l;
+            if (p != 0.f) lp += (double)p * l;                           // (a NaN is not 0)
             P += (double)p;
         }
         e.p[k] = p;
@@ -313,12 +315,12 @@ __device__ inline DistillRow finish_row(const DistillArgs& a, size_t r, Lse rest
     const double lq0 = -log2((double)all.s);                             // log2 q_v = (z_v - oall) c + lq0
     double loss = 0.0;
     for (int k = lane; k < a.K; k += 64)
-        if (e.p[k] > 0.f) loss -= (double)e.p[k] * (((double)e.z[k] - (double)row.oall) * (double)c + lq0);
+        if (e.p[k] != 0.f) loss -= (double)e.p[k] * (((double)e.z[k] - (double)row.oall) * (double)c + lq0);
     loss = (w.lp + sum_wave(loss)) * LN2_D;
     double ratio = 0.0;                                                  // p_r / (sum of the unnamed exponentials)
-    if (a.lse && rest.s > 0.f) {
+    if (a.lse && rest.s != 0.f) {
         const double pr = 1.0 - w.P;
-        if (pr > 0.0) {
+        if (!(pr <= 0.0)) {
             // q_r from the smaller side: 1 - Q keeps its digits where the named classes hold little
             const double Q = w.named.o == ninf ? 0.0 : (double)w.named.s * (double)exp2_of(((double)w.named.o - (double)row.oall) * (double)c + lq0);
             const double lqr = Q < 0.5 ? log1p(-Q) : (((double)row.orest - (double)row.oall) * (double)c + log2((double)rest.s) + lq0) * LN2_D;
@@ -575,13 +577,14 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
             double s = 0.0;
             for (int k = 0; k < K; ++k) if (eidx[k * 64 + px] != -1) s += (double)exp2_of(((double)ep[k * 64 + px] - (double)best) * a.l2T);
             L = (double)best * a.iT + log(s);
+            if (s == 0.0) { L = 0.0; have = false; }                     // entries of -inf: no mass, no entries
         }
         for (int k = 0; k < K; ++k) {
             float p = 0.f;
             if (eidx[k * 64 + px] != -1) {
                 const double l = entry_log2p(a, ep[k * 64 + px], L);
                 p = exp2_of(l);
-                if (p > 0.f) loss += (double)p * l;
+                if (p != 0.f) loss += (double)p * l;                     // (a NaN is not 0)
                 P += (double)p;
             }
             ep[k * 64 + px] = p;
@@ -601,12 +604,12 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
         const float oall = all.o == ninf ? 0.f : all.o, orest = rest.o == ninf ? 0.f : rest.o;
         const double lq0 = -log2((double)all.s);
         for (int k = 0; k < K; ++k)
-            if (ep[k * 64 + px] > 0.f) loss -= (double)ep[k * 64 + px] * (((double)ez[k * 64 + px] - (double)oall) * (double)c + lq0);
+            if (ep[k * 64 + px] != 0.f) loss -= (double)ep[k * 64 + px] * (((double)ez[k * 64 + px] - (double)oall) * (double)c + lq0);
         loss *= LN2_D;
         double ratio = 0.0;
-        if (a.lse && rest.s > 0.f) {
+        if (a.lse && rest.s != 0.f) {
             const double pr = 1.0 - P;
-            if (pr > 0.0) {
+            if (!(pr <= 0.0)) {
                 const double Q = named.o == ninf ? 0.0 : (double)named.s * (double)exp2_of(((double)named.o - (double)oall) * (double)c + lq0);
                 const double lqr = Q < 0.5 ? log1p(-Q) : (((double)orest - (double)oall) * (double)c + log2((double)rest.s) + lq0) * LN2_D;
                 loss += pr * (log1p(-P) - lqr);

@@ -918,7 +918,8 @@ int cnm_distill_planes_ok(int classes, int entries);
  *   p_k = exp(t_k / T - L), L = teacher_lse[row] or, NULL, log sum_k exp(t_k / T);  q = softmax(z / T)
  *   loss = T^2 [ sum_k p_k (log p_k - log q_{i_k}) + p_r (log p_r - log q_r) ], p_r = max(0, 1 - sum p_k) and q_r = the probability of the
  *   classes that no entry names, with teacher_lse only and only if these classes have any.
- * An index outside 0 .. classes-1 is no entry; a row without entries has loss 0 and gradient 0; a class may be named more than once.
+ * An index outside 0 .. classes-1 is no entry; a row without entries, or without teacher_lse with none but -inf, has loss 0 and gradient 0; a
+ * class may be named more than once.  A NaN among a row's entries, or in teacher_lse, goes on into its loss and gradient.
  * reduction 0: loss [rows] = weight loss; 1: loss [1] = sum weight loss / sum weight (0 if the weights sum to 0); 2: loss [1] = sum weight loss.
  * weight [rows] or NULL (1); a row of weight 0 counts 0 whatever it holds.  dz (dense, z's dtype) = the gradient of what `loss` is (reduction 0: of
  * its sum), times grad_out[0], or grad_out[row] with grad_out_rows (reduction 0 only), or 1 (NULL).  skip_if_one: if grad_out[0] == 1 the launch leaves dz as it is.

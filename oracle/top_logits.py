@@ -23,14 +23,14 @@ def distill(z, idx, val, lse, w, T, reduction, go=None):
     for r in range(R):
         ok = (idx[r] >= 0) & (idx[r] < V)
         i, t = idx[r][ok], val[r][ok]
-        if i.numel() == 0:
+        if i.numel() == 0 or lse is None and bool((t == -float("inf")).all()):
             rows.append(torch.zeros((), dtype=torch.float64)); grads.append(torch.zeros(V, dtype=torch.float64)); scale.append(1.0)
             continue
         lq = torch.log_softmax(z[r] / T, 0)
         q = lq.exp()
         lp = t / T - (lse[r].double() if lse is not None else torch.logsumexp(t / T, 0))
         p = lp.exp()
-        terms = torch.where(p > 0, p * (lp - lq[i]), torch.zeros_like(p))
+        terms = torch.where(p != 0, p * (lp - lq[i]), torch.zeros_like(p))
         g = q.clone()
         g.index_add_(0, i, -p)
         loss, mag = terms.sum(), terms.abs().sum()
@@ -38,7 +38,7 @@ def distill(z, idx, val, lse, w, T, reduction, go=None):
             out = torch.ones(V, dtype=torch.bool)
             out[i] = False
             pr, qr = (1 - p.sum()).clamp(min=0), q[out].sum()
-            if float(qr) > 0 and float(pr) > 0:
+            if float(qr) != 0 and float(pr) != 0:
                 lqr = torch.logsumexp(z[r][out] / T, 0) - torch.logsumexp(z[r] / T, 0)
                 loss = loss + pr * (pr.log() - lqr)
                 mag = mag + (pr * (pr.log() - lqr)).abs()

@@ -44,3 +44,14 @@ def test_oracle_mean_of_weights_of_any_sum():
     w[2] = float("nan")
     loss, g, _ = tl.distill(z, idx, val, lse, w, 2.0, "mean")
     assert bool(torch.isnan(loss)) and bool(torch.isnan(g).any())
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_oracle_teacher_entries_that_say_nothing(tail):
+    """A NaN among a row's entries is in its loss and gradient; renormalised entries that are all -inf are no entries."""
+    z, idx, val, lse, w = case()
+    val[0, 1], val[1] = float("nan"), -float("inf")
+    loss, g, _ = tl.distill(z, idx, val, lse if tail else None, None, 2.0, "none")
+    assert bool(torch.isnan(loss[0])) and bool(torch.isnan(g[0]).any()) and bool(torch.isfinite(loss[1:]).all()) and bool(torch.isfinite(g[1:]).all())
+    if not tail:
+        assert float(loss[1]) == 0 and float(g[1].abs().max()) == 0

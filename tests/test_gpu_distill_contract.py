@@ -328,3 +328,31 @@ def test_tiny_weights_times_large_upstream_gradients(R, V, planes, reduction):
     want = c[:, None] * g
     _, bg = bounds(z, T, mag, q, p, c, want)
     assert bool(((lay.back(dz).double() - want).abs() <= bg).all())
+
+
+@pytest.mark.parametrize("R,V,planes", FORMS)
+def test_teacher_entries_that_say_nothing(R, V, planes):
+    """Renormalised entries that are all -inf hold no mass: a row without entries.  A NaN in the teacher is seen in the loss and in the gradient."""
+    T, K = 2.0, 6
+    z, idx, val, lse = case(R, V, K, V + 4, T)
+    lay = Layout(planes, R)
+    none = val.clone()
+    none[1] = -INF
+    zd = lay.put(z).requires_grad_()
+    loss = TopLogitsDistillLoss(T, lay.dim, "none")(zd, lay.put(idx), lay.put(none))
+    dz = lay.back(torch.autograd.grad(loss.sum(), zd)[0])
+    loss = lay.back(loss)
+    assert float(loss[1]) == 0 and bool((dz[1] == 0).all()) and bool(torch.isfinite(loss).all()) and bool(torch.isfinite(dz).all()) and float(loss[0]) > 0
+    bad = val.clone()
+    bad[0, 2], bad[1, 0], bad[2, 5] = NAN, NAN, INF
+    dead = lse.clone()
+    dead[3] = NAN
+    for l in (None, dead):
+        zd = lay.put(z).requires_grad_()
+        loss = TopLogitsDistillLoss(T, lay.dim, "none")(zd, lay.put(idx), lay.put(bad), lay.put(l))
+        dz = lay.back(torch.autograd.grad(loss.sum(), zd)[0])
+        loss = lay.back(loss)
+        assert bool(torch.isnan(loss[:2]).all()) and bool(torch.isnan(dz[:2]).any(1).all())
+        assert not bool(torch.isfinite(loss[2]))
+        assert bool(torch.isnan(loss[3])) == (l is not None) and bool(torch.isnan(dz[3]).any()) == (l is not None)
+        assert bool(torch.isfinite(loss[4:]).all()) and bool(torch.isfinite(dz[4:]).all())
