@@ -681,6 +681,13 @@ int launch_quantizing(const StreamArgs& g, hipStream_t stream) {
 
 constexpr int FEW_ROWS = 64, FEW_COLS = 128;
 
+// a launch holds fewer than 2^32 threads: what the kernels above take for a matrix or product of these sizes
+bool launch_fits(long long blocks, int threads) { return blocks < (1ll << 32) / threads; }
+bool quantize_fits(long long rows, long long cols) { return launch_fits(cnm_ceil_div_ll(rows, QB) * cnm_ceil_div_ll(cols, QB), 512); }
+bool matmul_fits(long long M, long long N) {
+    return M <= FEW_ROWS ? launch_fits(cnm_ceil_div_ll(N, 16), 512) : launch_fits(cnm_ceil_div_ll(M, 128) * cnm_ceil_div_ll(N, 128), 256);
+}
+
 }  // namespace
 
 extern "C" int cnm_quantize_fp8(const void* x, int dtype, long long ldx, long long rows, long long cols, int block_rows,
@@ -688,7 +695,7 @@ extern "C" int cnm_quantize_fp8(const void* x, int dtype, long long ldx, long lo
     CNM_REQUIRE(x && rows > 0 && cols > 0 && ldx >= cols && (block_rows == 1 || block_rows == QB), CNM_ERR_BAD_ARG);
     CNM_REQUIRE((q || q_t) && !q == !scale && !q_t == !scale_t, CNM_ERR_BAD_ARG);
     CNM_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_t)) & 15) == 0, CNM_ERR_BAD_ARG);
-    CNM_REQUIRE(rows < (1ll << 31) - QB && cols < (1ll << 31) - QB && cnm_ceil_div_ll(rows, QB) * cnm_ceil_div_ll(cols, QB) < (1ll << 31), CNM_ERR_BAD_SHAPE);
+    CNM_REQUIRE(rows < (1ll << 31) - QB && cols < (1ll << 31) - QB && quantize_fits(rows, cols), CNM_ERR_BAD_SHAPE);
     const int R = (int)rows, C = (int)cols;
     const hipStream_t st = cnm_stream(stream);
 #define CNM_Q(DT) return block_rows == 1 ? launch_quantize<DT, false>(x, ldx, R, C, q, scale, q_t, scale_t, st) : launch_quantize<DT, true>(x, ldx, R, C, q, scale, q_t, scale_t, st)
@@ -718,7 +725,7 @@ extern "C" int cnm_matmul_fp8(const void* a, const void* a_scale, const void* b,
     CNM_REQUIRE(b_block_rows == 1 || b_block_rows == QB, CNM_ERR_BAD_ARG);
     CNM_REQUIRE(((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0, CNM_ERR_BAD_ARG);
     CNM_REQUIRE(M < (1ll << 31) - 256 && N < (1ll << 31) - 256 && K <= (1ll << 23), CNM_ERR_BAD_SHAPE);   // 256 rows of an operand are one 32-bit buffer range
-    CNM_REQUIRE(cnm_ceil_div_ll(M, 16) * cnm_ceil_div_ll(N, 16) < (1ll << 31), CNM_ERR_BAD_SHAPE);
+    CNM_REQUIRE(matmul_fits(M, N), CNM_ERR_BAD_SHAPE);
     MatArgs g = {static_cast<const unsigned char*>(a), static_cast<const unsigned char*>(a_scale), static_cast<const unsigned char*>(b), static_cast<const unsigned char*>(b_scale),
                  c, (int)M, (int)N, (int)(K / QB), b_block_rows == 1 ? 0 : 7, ldc, 0, 0, 1, 0};
     const size_t need = cnm_matmul_fp8_workspace_bytes(dtype, M, N, K);
@@ -751,7 +758,8 @@ static Fp8 fp8_take(unsigned char*& at, long long rows, long long cols, bool blo
 static bool dtype_ok(int d) { return d >= CNM_F32 && d <= CNM_BF16; }
 static bool train_shape_ok(long long M, long long N, long long K) {
     const long long most = 1ll << 23;                                    // each of them is a reduced axis of some product
-    return M <= most - QB && N <= most - QB && K <= most - QB;
+    return M <= most - QB && N <= most - QB && K <= most - QB
+        && quantize_fits(M, K) && quantize_fits(N, K) && quantize_fits(M, N) && matmul_fits(M, N) && matmul_fits(M, K) && matmul_fits(N, K);
 }
 
 extern "C" size_t cnm_linear_fp8_keep_bytes(long long M, long long N, long long K, int need_dx, int need_dw) {
@@ -812,7 +820,8 @@ extern "C" int cnm_linear_fp8(const void* x, int dtype, long long ldx, const voi
                               long long M, long long N, long long K, void* workspace, size_t workspace_bytes, void* stream) {
     CNM_REQUIRE(x && w && w_scale && y && M > 0 && N > 0 && K > 0 && ldx >= K && ldy >= N, CNM_ERR_BAD_ARG);
     CNM_REQUIRE((reinterpret_cast<uintptr_t>(w) & 15) == 0 && dtype_ok(dtype), CNM_ERR_BAD_ARG);
-    CNM_REQUIRE(M < (1ll << 31) - 256 && N < (1ll << 31) - 256 && K <= (1ll << 23) && cnm_ceil_div_ll(M, 16) * cnm_ceil_div_ll(N, 16) < (1ll << 31), CNM_ERR_BAD_SHAPE);
+    CNM_REQUIRE(M < (1ll << 31) - 256 && N < (1ll << 31) - 256 && K <= (1ll << 23), CNM_ERR_BAD_SHAPE);
+    CNM_REQUIRE(M <= 16 ? launch_fits(cnm_ceil_div_ll(N, 16), 512) : N <= FEW_COLS ? launch_fits(cnm_ceil_div_ll(M, 64), 256) : quantize_fits(M, K) && matmul_fits(M, N), CNM_ERR_BAD_SHAPE);
     const size_t need = cnm_linear_fp8_workspace_bytes(M, N, K);
     const long long kb = cnm_ceil_div_ll(K, QB);
     if (need) {                                                          // quantise, then multiply

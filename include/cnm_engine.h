@@ -865,7 +865,8 @@ int cnm_refinenet_forward_multi_cpu(const cnm_layer_weights* weights, float idep
  *
  * cnm_quantize_fp8: x [rows][ldx] of dtype (ldx >= cols, any alignment) -> q, scale and / or the transposed matrix's form q_t [cols][rows
  * padded to 128], scale_t (block_rows 1: blocked along the rows, [cols][ceil(rows/128)]; 128: the same blocks, [ceil(cols/128)][ceil(rows/128)])
- * in one pass over x.  q / q_t (with their scales) may be NULL, not both; q and q_t on 16 bytes. */
+ * in one pass over x.  q / q_t (with their scales) may be NULL, not both; q and q_t on 16 bytes.  Here and in the products below a size is bounded by
+ * what one launch holds (fewer than 2^32 threads: 512 per 128 x 128 block, or per 16 columns where rows are few); more: CNM_ERR_BAD_SHAPE. */
 int cnm_quantize_fp8(const void* x, int dtype, long long ldx, long long rows, long long cols, int block_rows,
                      void* q, void* scale, void* q_t, void* scale_t, void* stream);
 /* c [M][ldc] of dtype = a b^T: a [M][K], b [N][K] as above (K a multiple of 128, at most 2^23; a, b on 16 bytes), a_scale [M][K/128],

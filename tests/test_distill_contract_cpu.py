@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from cnmnet_amd import _lib
 from oracle import top_logits as tl
 
 
@@ -55,3 +56,22 @@ def test_oracle_teacher_entries_that_say_nothing(tail):
     assert bool(torch.isnan(loss[0])) and bool(torch.isnan(g[0]).any()) and bool(torch.isfinite(loss[1:]).all()) and bool(torch.isfinite(g[1:]).all())
     if not tail:
         assert float(loss[1]) == 0 and float(g[1].abs().max()) == 0
+
+
+def test_linear_entries_refuse_more_than_one_launch_holds():
+    """2^32 threads and more are refused before anything is launched; just below that the workspace (absent here) is what is missed."""
+    lib = _lib.load()
+    big = 1 << 60
+    quantize = lambda rows, cols: lib.cnm_quantize_fp8(64, 0, cols, rows, cols, 1, 4096, 4096, 0, 0, 0)
+    assert quantize(1 << 30, 1) == -2 and quantize(1 << 26, 2048) == -2
+    matmul = lambda M, N: lib.cnm_matmul_fp8(4096, 64, 8192, 64, 1, 4096, 0, N, M, N, 128, 0, 0, 0)
+    assert matmul(1, 1 << 27) == -2 and matmul(64, 1 << 30) == -2 and matmul(1 << 20, 1 << 19) == -2
+    linear = lambda M, N, K, n=0: lib.cnm_linear_fp8(64, 1, K, 4096, 64, 4096, N, M, N, K, 4096 if n else 0, n, 0)
+    assert linear(1, 1 << 27, 8) == -2 and linear(1 << 30, 100, 8) == -2                  # few rows, few columns
+    assert linear(1 << 30, 200, 8, big) == -2 and linear(1 << 20, 1 << 20, 8, big) == -2  # its quantisation, its product
+    assert linear(1 << 20, 200, 8) == -5
+    forward = lambda M, N, K: lib.cnm_linear_fp8_forward(4096, 0, K, 4096, 0, K, 4096, M, N, K, 0, 0, 0, 0, 4096, big, 0)
+    backward = lambda M, N, K: lib.cnm_linear_fp8_backward(4096, 0, N, 4096, big, 4096, 0, 0, 0, M, N, K, 1, 0, 4096, big, 0)
+    for f in (forward, backward):
+        for shape in ((1 << 22, 8, 1 << 16), (8, 1 << 22, 1 << 16), (1 << 22, 1 << 16, 8)):
+            assert f(*shape) == -2
