@@ -356,3 +356,29 @@ def test_teacher_entries_that_say_nothing(R, V, planes):
         assert not bool(torch.isfinite(loss[2]))
         assert bool(torch.isnan(loss[3])) == (l is not None) and bool(torch.isnan(dz[3]).any()) == (l is not None)
         assert bool(torch.isfinite(loss[4:]).all()) and bool(torch.isfinite(dz[4:]).all())
+
+
+@pytest.mark.parametrize("R", [5, 140])
+@pytest.mark.parametrize("V,dtype", [(131072, torch.bfloat16), (131069, torch.float16), (65533, torch.float32), (100003, torch.float32), (32768, torch.bfloat16)])
+def test_every_class_of_a_long_row_counts(R, V, dtype):
+    """Equal logits: the log-sum-exp is log V, and sixteen bytes that a thread leaves out would be missed; a heavy class at either end or at the seams of
+    vectors, threads and segments; the bound is that of the sums' depth, not of the row's length."""
+    z = torch.zeros(R, V, dtype=dtype)
+    seams = [0, V - 1, V - 2, V // 2, 8191, 8192, 4095, 4096, 16384, 32767]
+    for r in range(1, R):
+        z[r, seams[r % len(seams)]] = 10.0
+    val, idx, lse = ops.top_logits(z.to(DEV), 3)
+    ref = torch.logsumexp(z.double(), 1)
+    D = spread(z, 1.0)
+    assert D < 8.0 / V
+    assert bool(((lse.cpu().double() - ref).abs() <= D + ref * 2.0 ** -24).all())
+    assert idx[1:, 0].cpu().tolist() == [seams[r % len(seams)] for r in range(1, R)]
+    # one entry that holds the teacher's whole mass: the loss is log(V) or log(V + e^10 - 1) less the entry's logit
+    at = torch.full((R, 1), 7)
+    L, g, mag, q, p = formula(z, at, torch.ones(R, 1), None, 1.0)
+    zd = z.to(DEV).requires_grad_()
+    loss = TopLogitsDistillLoss(reduction="none")(zd, at.to(DEV), torch.ones(R, 1, device=DEV))
+    assert bool(((loss.detach().cpu().double() - L).abs() <= D + L * 2.0 ** -24).all())
+    (dz,) = torch.autograd.grad(loss.sum(), zd)
+    got = dz.cpu().double()
+    assert bool(((got - g).abs() <= 2 * D * q + 8 * 2.0 ** -24 * p + g.abs() * torch.finfo(dtype).eps / 2 * 1.01 + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps).all())
