@@ -17,7 +17,7 @@
 //     eight consecutive products at a time, each cut off at 2^-13 of the eight's largest exponent (measured: probes of single terms; rms
 //     1.5e-5 of the result on normal data): a choice for results that are rounded to 2^-9 or 2^-12 anyway.
 //   fp32 results: the bytes become bf16 with their scale applied (exact within bf16's exponent range) and v_mfma_f32_32x32x16_bf16 (16x16x32) adds them:
-//     rms 1e-8 of the result, as fp32 sums are.
+//     rms 1e-8 of the result, as fp32 sums are.  Below a block exponent of -117 an e4m3 value's low bits fall under bf16's normal range and are lost.
 #include "cnm_common.h"
 
 namespace {
@@ -219,8 +219,10 @@ __device__ inline void tile_of(int id, const MatArgs& g, int& tm, int& tn) {
 // all 64 banks.  The DMA writes 64 lanes x 16 bytes in order, so the permutation is in the lanes' source addresses.
 // Scale bytes: rows of SC blocks in LDS, refilled every SC blocks; a lane reads four blocks' bytes as one word.
 // The weight is the instruction's first operand: a lane then holds outputs of one row, in fours.
-// 8192 x 8192 x 8192, bf16 results: about 430 us, 2.4 to 2.6 PF from card to card (a library product of plain bytes 2.6), held back by the package's
-// power limit; 8192 x 4096 x 4096: 122 to 133 us (2.1 to 2.3 PF), of which 9 us per tile are its first loads and its stores.
+// 8192 x 8192 x 8192, bf16 results, one launch after another: 408 to 430 us from card to card, 2.6 to 2.7 PF (a library product of plain bytes 2.6),
+// held back by the package's power limit (under a profiler's kernel trace 513 us); 8192 x 4096 x 4096: 110 us back to back (2.5 PF), 125 to 136 between
+// the quantisations of a training step, of which 9 us per tile are its first loads and its stores.  fp32 results: 4096^3 122 us (1.1 PF), 8192^3 870
+// (1.26 PF): half the instruction rate, and the conversions.
 // The order within a half block: its NM matrix instructions start at once, the next fragments' ND reads and the NV DMA instructions go evenly
 // between them (left alone, the scheduler puts all of these in front, or the matrix instructions of two half blocks behind one barrier).
 template <int I, int NM, int ND, int NV>
@@ -671,7 +673,10 @@ int launch_few_rows(const StreamArgs& g, hipStream_t stream) {
     return launch_stream<DT, false, 4, 1, 8, 2>(g, stream);
 }
 
-// x as it is: few columns, or at most 16 rows
+// x as it is: few columns, or at most 16 rows.  The few-columns form splits nothing: it pays with many rows (fp32 49152 x 64 x 512: 27 us,
+// quantised first and multiplied in tiles 21 + 14; 16384 x 128 x 512: 15 against 10 + 11) and is the slower one where few rows meet a long reduced
+// axis, one workgroup per 64 rows walking it alone (bf16 4096 x 64 x 2048: 24 us against 9 + 11; 1000 x 64 x 8192: 87 against 9 + 15;
+// 64 x 128 x 8192: 143 against 9 + 27).
 template <int DT>
 int launch_quantizing(const StreamArgs& g, hipStream_t stream) {
     if (g.M <= 16) return launch_stream<DT, true, 1, 1, 8, 4>(g, stream);

@@ -848,7 +848,10 @@ def _fp8_operand(q, s, what, per_row=True, per_block=False):
 
 
 def matmul_fp8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
-    """a [M, K], b [N, K] as quantize_fp8 makes them -> a b^T [M, N] of `dtype`; a with one scale per row and block, b with either kind."""
+    """a [M, K], b [N, K] as quantize_fp8 makes them -> a b^T [M, N] of `dtype`; a with one scale per row and block, b with either kind.  float32
+    results are sums of exact products; float16 and bfloat16 ones go through an instruction that cuts a product off at 2^-13 of the largest of
+    its eight neighbours (1.5e-5 of a sum of ordinary terms, more than the type's own rounding only where the terms cancel): for such
+    sums take float32."""
     _fp8_operand(a, a_scale, "matmul_fp8 a")
     bb = _fp8_operand(b, b_scale, "matmul_fp8 b", per_block=True)
     if a.device != b.device or a.shape[1] != b.shape[1]:
@@ -871,7 +874,8 @@ def matmul_fp8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
 
 def linear_fp8(x, w_packed, w_scale):
     """x [..., K] times a packed weight (pack_linear_fp8, [N, K]) -> [..., N] of x's type.  x is quantised here, one scale per row and 128
-    columns.  Inference; autograd.linear_fp8 is the training form."""
+    columns.  Inference; autograd.linear_fp8 is the training form.  A row's result depends on the batch around it in its last bits (another kernel,
+    another order of the sum)."""
     dev = _dev_any(x)
     if _fp8_operand(w_packed, w_scale, "linear_fp8 weight", per_row=False, per_block=True) != 128 or w_packed.device != dev:
         raise _lib.EngineError("linear_fp8: x on %s, weight on %s" % (dev, w_packed.device))

@@ -871,7 +871,8 @@ int cnm_quantize_fp8(const void* x, int dtype, long long ldx, long long rows, lo
                      void* q, void* scale, void* q_t, void* scale_t, void* stream);
 /* c [M][ldc] of dtype = a b^T: a [M][K], b [N][K] as above (K a multiple of 128, at most 2^23; a, b on 16 bytes), a_scale [M][K/128],
  * b_scale [N][K/128] (b_block_rows 1) or [ceil(N/128)][K/128] (128).  fp32 accumulation, one rounding (with 16-bit
- * results the matrix instruction cuts products off at 2^-13 of the largest of eight neighbours; fp32 results are exact products in fp32 sums).
+ * results the matrix instruction cuts products off at 2^-13 of the largest of eight neighbours, which shows where a sum cancels to less than that;
+ * fp32 results are exact products in fp32 sums, for block exponents from -117 on: below, low bits of the values are lost).
  * Any M, N >= 1; ldc >= N.  workspace: cnm_matmul_fp8_workspace_bytes on 16 bytes (0 but where few output tiles share a long reduced axis),
  * contents irrelevant. */
 size_t cnm_matmul_fp8_workspace_bytes(int dtype, long long M, long long N, long long K);
