@@ -124,9 +124,9 @@ class TopLogitsDistillLoss(nn.Module):
     students that predict a distribution: over depth planes ([B, planes, H, W], dim=1) or over any classes along the last dim.
 
     forward(logits, top_idx, top_logits, top_lse=None, weight=None): T^2 KL(teacher || student); with top_lse the teacher's remaining mass is one
-    class of its own, without it the entries are renormalised.  weight: per-row, e.g. the frame's valid mask as float32, a factor of each
-    row's loss for every reduction; "mean" divides by its sum (0 for an empty mask).  Rows without entries (index -1 throughout) give 0.  Unlike the losses above this is an engine operator
-    (GPU tensors only); the gradient reaches the logits, the teacher's side is constant."""
+    class of its own, without it the entries are renormalised.  weight: per-row, e.g. the frame's valid mask as float32, a factor of each row's loss
+    for every reduction; "mean" divides by its sum (0 for an empty mask).  Rows without entries (index -1 throughout) give 0.  Unlike the
+    losses above this is an engine operator (GPU tensors only); the gradient reaches the logits, the teacher's side is constant."""
 
     def __init__(self, temperature=1.0, dim=-1, reduction="mean"):
         super().__init__()

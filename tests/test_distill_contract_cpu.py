@@ -1,4 +1,5 @@
-"""CPU: the distillation oracle against itself -- its gradient is the derivative of the loss that it returns -- and against the formula."""
+"""CPU: the distillation oracle against itself (its gradient is the derivative of the loss that it returns) and the formula; sizes that the 8-bit
+linear layer's entries refuse."""
 import pytest
 import torch
 
